@@ -191,7 +191,8 @@ def _own(s):
     from datago_b200 import tokens as tk
     case, ctx, op = s["case"], s["ctx"], s["case"]["op"]
     if op == "patch":
-        r = tk.patch_rows(ctx, s["pixels"], case["patch"], MEAN, STD)
+        c = case["channels"]
+        r = tk.patch_rows(ctx, s["pixels"], case["patch"], MEAN[:c], STD[:c])
         return r.values, r.scales
     if op == "columns":
         r = tk.quantize_rows(ctx, s["x"], transpose=True)
