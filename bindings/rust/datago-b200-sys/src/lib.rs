@@ -154,6 +154,34 @@ pub enum dg_ctx {}
 pub enum dg_batch {}
 pub enum dg_feeder {}
 pub type dg_ticket = u64;
+pub const DG_F32: i32 = 0;
+pub const DG_BF16: i32 = 1;
+pub const DG_F16: i32 = 2;
+
+/// A matrix in device memory; `ld` in elements.
+#[repr(C)]
+pub struct dg_matrix {
+    pub data: *mut c_void,
+    pub rows: u64,
+    pub cols: u64,
+    pub ld: u64,
+    pub dtype: i32,
+    pub reserved: u32,
+}
+
+/// Rows in 8 bits: e4m3 values, an E8M0 scale for each 128 columns of `block` rows; `ld` and `scale_ld` in bytes.
+#[repr(C)]
+pub struct dg_rows8 {
+    pub values: *mut u8,
+    pub scales: *mut u8,
+    pub rows: u64,
+    pub cols: u64,
+    pub ld: u64,
+    pub scale_ld: u64,
+    pub block: u32,
+    pub reserved: u32,
+}
+
 pub type dg_log_fn = Option<unsafe extern "C" fn(level: c_int, message: *const c_char, user: *mut c_void)>;
 
 extern "C" {
@@ -210,6 +238,21 @@ extern "C" {
 
     pub fn dg_resize_device_static(ctx: *mut dg_ctx, device_src: *const u8, w: u32, h: u32, channels: u32, forced_key: *const c_char,
                                    device_dst: *mut u8, plan_out: *mut dg_plan) -> c_int;
+    pub fn dg_patch_rows(ctx: *mut dg_ctx, stream: *mut c_void, pixels: *const u8, n: u32, h: u32, w: u32, channels: u32, patch: u32,
+                         mean: *const f32, std: *const f32, out8: *const dg_rows8, out: *const dg_matrix) -> c_int;
+    pub fn dg_quantize_rows(ctx: *mut dg_ctx, stream: *mut c_void, src: *const dg_matrix, transpose: c_int, out: *const dg_rows8) -> c_int;
+    pub fn dg_product_workspace(ctx: *mut dg_ctx, m: u64, n: u64, k: u64) -> u64;
+    pub fn dg_product(ctx: *mut dg_ctx, stream: *mut c_void, a: *const dg_rows8, b: *const dg_rows8, out: *const dg_matrix,
+                      workspace: *mut c_void, workspace_bytes: u64) -> c_int;
+    pub fn dg_product_status(ctx: *mut dg_ctx, stream: *mut c_void) -> c_int;
+    pub fn dg_rms_norm(ctx: *mut dg_ctx, stream: *mut c_void, x: *const dg_matrix, residual: *const dg_matrix, weight: *const dg_matrix,
+                       eps: f32, sum: *const dg_matrix, y: *const dg_matrix, y8: *const dg_rows8, rstd: *mut f32) -> c_int;
+    pub fn dg_rms_norm_backward_workspace(ctx: *mut dg_ctx, rows: u64, cols: u64, residual_rows: u64) -> u64;
+    pub fn dg_rms_norm_backward(ctx: *mut dg_ctx, stream: *mut c_void, dy: *const dg_matrix, h: *const dg_matrix, rstd: *const f32,
+                                weight: *const dg_matrix, dsum: *const dg_matrix, dx: *const dg_matrix, dresidual: *mut f32,
+                                residual_rows: u64, dweight: *mut f32, workspace: *mut c_void, workspace_bytes: u64) -> c_int;
+    pub fn dg_dropout(ctx: *mut dg_ctx, stream: *mut c_void, x: *const dg_matrix, p: f64, seed: u64, offset: u64, per_row: c_int,
+                      y: *const dg_matrix) -> c_int;
     pub fn dg_host_alloc(nbytes: u64, out: *mut *mut c_void) -> c_int;
     pub fn dg_host_release(block: *mut c_void);
     pub fn dg_copy_to_host(ctx: *mut dg_ctx, dst: *mut c_void, device_src: *const c_void, nbytes: u64) -> c_int;

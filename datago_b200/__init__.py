@@ -219,7 +219,8 @@ EXPORTS = ("dg_set_log_callback dg_ctx_get_counters dg_last_error dg_version dg_
            "dg_key_hash dg_key_rank dg_batch_create dg_batch_upload dg_batch_run dg_batch_download dg_batch_sync "
            "dg_batch_download_packed dg_batch_download_views dg_batch_packed_bytes dg_batch_bucket_count dg_batch_bucket "
            "dg_batch_result dg_batch_results dg_batch_stage_ms dg_batch_counters dg_batch_huffman_stats dg_batch_debug dg_batch_destroy dg_process "
-           "dg_copy_to_host dg_resize_device_static dg_feeder_create dg_feeder_ctx dg_submit dg_wait dg_fetch dg_peek dg_fetch_view dg_release dg_host_alloc dg_host_release "
+           "dg_copy_to_host dg_patch_rows dg_quantize_rows dg_product_workspace dg_product dg_product_status dg_rms_norm "
+           "dg_rms_norm_backward_workspace dg_rms_norm_backward dg_dropout dg_resize_device_static dg_feeder_create dg_feeder_ctx dg_submit dg_wait dg_fetch dg_peek dg_fetch_view dg_release dg_host_alloc dg_host_release "
            "dg_feeder_get_stats dg_feeder_destroy").split()
 
 
@@ -547,6 +548,21 @@ class Batch:
                             packed_offset=int(bk.packed_offset), nbytes=int(bk.nbytes),
                             array=DeviceArray(bk.device_data, shape, self)))
         return out
+
+    def patch_rows(self, k, patch, mean, std, dtype=None):
+        """Bucket k of a BATCH_COLLATE batch (see buckets()) cut into patches and normalised, one row a patch: what a transformer reads.
+        Rows8, or with a torch `dtype` a tensor (see tokens.patch_rows).  Queued behind run() without waiting; the rows are torch's own
+        and outlive the batch, those of damaged items are undefined (look at the items' status after sync())."""
+        if not self._h:
+            raise DatagoB200Error(1, "the batch is closed")
+        import torch
+        from . import tokens
+        bucket = self.buckets()[k]
+        own, current = torch.cuda.ExternalStream(self.ctx.stream, self.ctx.device), torch.cuda.current_stream(self.ctx.device)
+        current.wait_stream(own)
+        rows = tokens.patch_rows(self.ctx, bucket["array"], patch, mean, std, dtype)
+        own.wait_stream(current)  # the batch's memory is handed on in the order of its own stream
+        return rows
 
     def stage_ms(self):
         ms = (C.c_float * len(STAGES))()

@@ -226,6 +226,9 @@ extern "C" void dg_ctx_destroy(dg_ctx* c) {
     delete c;
 }
 
+int dg::ctx_device(const dg_ctx* c) { return c->device; }
+void* dg::encode_tiled_entry() { return (void*)encode_tiled_fn(); }
+
 extern "C" void* dg_ctx_stream(dg_ctx* c) { return c ? (void*)c->stream : nullptr; }
 
 extern "C" int dg_ctx_get_counters(dg_ctx* c, dg_ctx_counters* out) {

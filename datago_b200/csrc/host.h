@@ -59,6 +59,10 @@ bool huff_lengths_valid(const JpegHeader::RawHuff& raw);  // what build_huff_tab
 // Stores msg as the calling thread's dg_last_error text and returns code.
 int dg_set_error(int code, const char* msg);
 
+// ---- contexts ---------------------------------------------------------------------------------------------------------
+int ctx_device(const dg_ctx* ctx);    // DG_DEVICE_NONE for planning-only ones
+void* encode_tiled_entry();           // cuTensorMapEncodeTiled, or NULL where the driver does not have it
+
 // ---- batches --------------------------------------------------------------------------------------------------------
 // Queues copies of all ok payloads into blocks of the page-locked pool: host[i] and blocks[i] (a reference of the caller's,
 // see host_blocks.h) per item, NULL where there is no payload.  On an error the caller gets no references.

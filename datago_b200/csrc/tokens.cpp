@@ -1,0 +1,327 @@
+// C entry points of the token rows (declared in include/datago_b200.h): checks of the arguments, tensor maps, launches.  None of them
+// allocates, waits (dg_product_status apart) or keeps anything, so calls need no lock and can be captured.
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+
+#include "host.h"
+#include "tokens.h"
+
+using namespace dg;
+
+// ---- how the work is dealt out ------------------------------------------------------------------------------------------
+namespace dg {
+
+ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t k) {
+    ProductPlan p{};
+    if (m == 0 || n == 0) return p;
+    const uint32_t groups = (uint32_t)scale_groups(k);
+    p.tiles_m = (uint32_t)((m + kProductTileM - 1) / kProductTileM);
+    // as few column tiles as the widest allows, all of them equally wide
+    p.tiles_n = (uint32_t)((n + kProductMaxTileN - 1) / kProductMaxTileN);
+    auto equal_widths = [&] {
+        p.tile_n = (uint32_t)((n + p.tiles_n - 1) / p.tiles_n + 15) / 16 * 16;
+        p.tiles_n = (uint32_t)((n + p.tile_n - 1) / p.tile_n);
+    };
+    equal_widths();
+    // few rows: narrower tiles, so that more SMs fetch the other operand
+    while ((uint64_t)p.tiles_m * p.tiles_n * 2 <= kTokenSms && p.tile_n >= 64) {
+        p.tiles_n *= 2;
+        equal_widths();
+    }
+    const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
+    p.splits = 1;
+    if (tiles < kTokenSms && groups >= 16) p.splits = (uint32_t)std::min<uint64_t>(kTokenSms / tiles, groups / 8);
+    if (p.splits < 1) p.splits = 1;
+    // parts begin at multiples of four groups: the scales come in words
+    p.split_groups = ((groups + p.splits - 1) / p.splits + 3) / 4 * 4;
+    p.splits = (groups + p.split_groups - 1) / p.split_groups;
+    return p;
+}
+
+// threads of a row, rows of a CTA
+namespace {
+struct BackwardShape {
+    uint32_t threads, rows;
+};
+BackwardShape backward_shape(uint64_t cols) {
+    const uint64_t vecs = (cols + 7) / 8;
+    return vecs <= 160 ? BackwardShape{256, 8} : vecs <= 512 ? BackwardShape{256, 2} : BackwardShape{512, 1};
+}
+}  // namespace
+
+NormBackwardSplit norm_backward_split(uint64_t rows, uint64_t cols, uint64_t period, bool residual) {
+    const BackwardShape sh = backward_shape(cols);
+    const uint64_t at_once = (uint64_t)kTokenSms * 2 * sh.rows;  // rows that the chip works on at a time
+    const uint64_t images = residual ? rows / period : 1;
+    uint64_t parts = 1;
+    if (residual && period < at_once) parts = std::max<uint64_t>(1, std::min(images, at_once / period));
+    const uint64_t units = (residual ? period : rows) * parts;
+    return {(uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((units + sh.rows - 1) / sh.rows, (uint64_t)kTokenSms * 2)), (uint32_t)parts};
+}
+
+}  // namespace dg
+
+namespace {
+
+int fail(int code, const char* fmt, ...) {
+    char msg[256];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(msg, sizeof msg, fmt, ap);
+    va_end(ap);
+    return dg_set_error(code, msg);
+}
+
+// The context's device while a call lasts.
+struct OnDevice {
+    int before = -1, device;
+    cudaError_t error;
+    explicit OnDevice(int d) : device(d) {
+        error = cudaGetDevice(&before);
+        if (error == cudaSuccess && before != d) error = cudaSetDevice(d);
+    }
+    ~OnDevice() {
+        if (before >= 0 && before != device) cudaSetDevice(before);
+    }
+};
+
+constexpr uint64_t kMostCols = (1ull << 31) - 1024, kMostRows = 1ull << 40, kMostElements = 1ull << 60;
+
+int check_ctx(const dg_ctx* ctx) {
+    if (!ctx) return fail(DG_E_INVALID, "ctx is NULL");
+    if (ctx_device(ctx) == DG_DEVICE_NONE) return fail(DG_E_INVALID, "planning-only context: token rows need a CUDA device");
+    return DG_OK;
+}
+uint64_t element(int32_t dtype) { return dtype == DG_F32 ? 4 : 2; }
+int check_matrix(const dg_matrix* m, const char* name) {
+    if (!m) return fail(DG_E_INVALID, "%s is NULL", name);
+    if (m->dtype < DG_F32 || m->dtype > DG_F16) return fail(DG_E_INVALID, "%s: unknown dtype %d", name, (int)m->dtype);
+    if (m->cols == 0 || m->cols > kMostCols || m->rows > kMostRows) return fail(DG_E_INVALID, "%s: %llu x %llu elements", name, (unsigned long long)m->rows, (unsigned long long)m->cols);
+    if (m->ld < m->cols || m->ld > kMostElements / (m->rows + 1)) return fail(DG_E_INVALID, "%s: rows of %llu elements %llu apart", name, (unsigned long long)m->cols, (unsigned long long)m->ld);
+    if (m->rows && !m->data) return fail(DG_E_INVALID, "%s: data is NULL", name);
+    if ((uintptr_t)m->data % element(m->dtype)) return fail(DG_E_INVALID, "%s: data is not aligned to its elements", name);
+    return DG_OK;
+}
+int check_rows8(const dg_rows8* r, const char* name) {
+    if (!r) return fail(DG_E_INVALID, "%s is NULL", name);
+    if (r->block != 1 && r->block != kScaleGroup) return fail(DG_E_INVALID, "%s: block is 1 or 128", name);
+    if (r->cols == 0 || r->cols > kMostCols || r->rows > kMostRows) return fail(DG_E_INVALID, "%s: %llu x %llu elements", name, (unsigned long long)r->rows, (unsigned long long)r->cols);
+    if (r->ld < r->cols || r->ld % 16 || r->ld > kMostElements / (r->rows + 1)) return fail(DG_E_INVALID, "%s: ld is a multiple of 16 and at least cols", name);
+    if (r->scale_ld < scale_groups(r->cols) || r->scale_ld % 4 || r->scale_ld > kMostElements / (r->rows + 1))
+        return fail(DG_E_INVALID, "%s: scale_ld is a multiple of 4 and at least a byte per 128 columns", name);
+    if (r->rows && (!r->values || !r->scales)) return fail(DG_E_INVALID, "%s: values or scales are NULL", name);
+    if ((uintptr_t)r->values % 16 || (uintptr_t)r->scales % 4) return fail(DG_E_INVALID, "%s: values are 16-byte aligned, scales 4-byte", name);
+    return DG_OK;
+}
+int check_like(const dg_matrix* m, const char* name, uint64_t rows, uint64_t cols, int32_t dtype) {
+    if (int rc = check_matrix(m, name)) return rc;
+    if (m->rows != rows || m->cols != cols) return fail(DG_E_INVALID, "%s: %llu x %llu elements, %llu x %llu wanted", name, (unsigned long long)m->rows, (unsigned long long)m->cols, (unsigned long long)rows, (unsigned long long)cols);
+    if (m->dtype != dtype) return fail(DG_E_INVALID, "%s: another dtype than the input's", name);
+    return DG_OK;
+}
+int check_rows8_like(const dg_rows8* r, const char* name, uint64_t rows, uint64_t cols) {
+    if (int rc = check_rows8(r, name)) return rc;
+    if (r->rows != rows || r->cols != cols) return fail(DG_E_INVALID, "%s: %llu x %llu elements, %llu x %llu wanted", name, (unsigned long long)r->rows, (unsigned long long)r->cols, (unsigned long long)rows, (unsigned long long)cols);
+    return DG_OK;
+}
+int check_weight(const dg_matrix* w, uint64_t cols) {
+    if (!w) return DG_OK;
+    if (int rc = check_matrix(w, "weight")) return rc;
+    if (w->rows != 1 || w->cols != cols) return fail(DG_E_INVALID, "weight: 1 x %llu elements wanted", (unsigned long long)cols);
+    return DG_OK;
+}
+int check_floats(const float* p, const char* name) { return (uintptr_t)p % 4 ? fail(DG_E_INVALID, "%s is not aligned to its elements", name) : DG_OK; }
+int check_workspace(const void* p, uint64_t bytes, uint64_t needed) {
+    if (bytes < needed || (needed && !p)) return fail(DG_E_INVALID, "workspace of %llu bytes, %llu needed", (unsigned long long)bytes, (unsigned long long)needed);
+    if (needed && (uintptr_t)p % 16) return fail(DG_E_INVALID, "workspace is not 16-byte aligned");
+    return DG_OK;
+}
+
+cudaStream_t stream_of(dg_ctx* ctx, void* stream) { return stream ? (cudaStream_t)stream : (cudaStream_t)dg_ctx_stream(ctx); }
+// Runs `launch` (which returns a cudaError_t or nothing) on the context's device.
+template <class F>
+int launched(dg_ctx* ctx, F&& launch) {
+    OnDevice on(ctx_device(ctx));
+    if (on.error != cudaSuccess) return fail(DG_E_CUDA, "device %d: %s", ctx_device(ctx), cudaGetErrorString(on.error));
+    launch();
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? DG_OK : fail(DG_E_CUDA, "launch: %s", cudaGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" int dg_patch_rows(dg_ctx* ctx, void* stream, const uint8_t* pixels, uint32_t n, uint32_t h, uint32_t w, uint32_t channels,
+                             uint32_t patch, const float* mean, const float* std, const dg_rows8* out8, const dg_matrix* out) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (!mean || !std || !out8 == !out) return fail(DG_E_INVALID, "mean and std, and one of out8 and out, are wanted");
+    if (channels < 1 || channels > 4) return fail(DG_E_INVALID, "%u channels: 1 to 4 are wanted", channels);
+    if (patch == 0 || patch > 4096 || h == 0 || w == 0 || h % patch || w % patch) return fail(DG_E_INVALID, "%u x %u pixels are no whole number of %u x %u patches", h, w, patch, patch);
+    const uint64_t per_image = (uint64_t)(h / patch) * (w / patch), rows = n * per_image, cols = (uint64_t)patch * patch * channels;
+    if (per_image >> 32 || (uint64_t)w * channels >> 32) return fail(DG_E_INVALID, "%u x %u pixels are too many", h, w);
+    if (n && !pixels) return fail(DG_E_INVALID, "pixels is NULL");
+    if (out) {
+        if (int rc = check_matrix(out, "out")) return rc;
+        if (out->rows != rows || out->cols != cols) return fail(DG_E_INVALID, "out: %llu x %llu elements wanted", (unsigned long long)rows, (unsigned long long)cols);
+    } else {
+        if (int rc = check_rows8_like(out8, "out8", rows, cols)) return rc;
+        if (out8->block != 1) return fail(DG_E_INVALID, "out8: patches have block 1");
+    }
+    PatchJob j{pixels, n, h, w, channels, patch, {}, {}};
+    for (uint32_t c = 0; c < channels; ++c) {
+        if (!(std[c] > 0) || !std::isfinite(std[c]) || !std::isfinite(mean[c])) return fail(DG_E_INVALID, "channel %u: mean and std are finite, std above 0", c);
+        j.gain[c] = (float)(1.0 / (255.0 * std[c]));
+        j.shift[c] = (float)(-(double)mean[c] / std[c]);
+    }
+    if (rows == 0) return DG_OK;
+    return launched(ctx, [&] { launch_patch_rows(j, out8, out, stream_of(ctx, stream)); });
+}
+
+extern "C" int dg_quantize_rows(dg_ctx* ctx, void* stream, const dg_matrix* src, int transpose, const dg_rows8* out) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (int rc = check_matrix(src, "src")) return rc;
+    if (transpose && src->rows == 0) return fail(DG_E_INVALID, "the transpose of a matrix without rows has no columns");
+    if (int rc = check_rows8_like(out, "out", transpose ? src->cols : src->rows, transpose ? src->rows : src->cols)) return rc;
+    if (src->rows == 0) return DG_OK;
+    return launched(ctx, [&] { launch_quantize_rows(*src, transpose != 0, *out, stream_of(ctx, stream)); });
+}
+
+extern "C" uint64_t dg_product_workspace(dg_ctx* ctx, uint64_t m, uint64_t n, uint64_t k) {
+    if (!ctx || m > kMostCols || n > kMostCols || k > kMostCols) return 0;
+    return product_workspace(plan_product(m, n, k), m, n);
+}
+
+extern "C" int dg_product(dg_ctx* ctx, void* stream, const dg_rows8* a, const dg_rows8* b, const dg_matrix* out, void* workspace,
+                          uint64_t workspace_bytes) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (int rc = check_rows8(a, "a")) return rc;
+    if (int rc = check_rows8(b, "b")) return rc;
+    if (a->cols != b->cols) return fail(DG_E_INVALID, "a has %llu columns, b %llu", (unsigned long long)a->cols, (unsigned long long)b->cols);
+    if (a->rows > kMostCols || b->rows == 0 || b->rows > kMostCols) return fail(DG_E_INVALID, "a has %llu rows, b %llu", (unsigned long long)a->rows, (unsigned long long)b->rows);
+    if (int rc = check_matrix(out, "out")) return rc;
+    if (out->rows != a->rows || out->cols != b->rows) return fail(DG_E_INVALID, "out: %llu x %llu elements wanted", (unsigned long long)a->rows, (unsigned long long)b->rows);
+    if (a->rows == 0) return DG_OK;
+    ProductJob j{};
+    j.plan = plan_product(a->rows, b->rows, a->cols);
+    if ((uint64_t)j.plan.tiles_m * j.plan.tiles_n * j.plan.splits > kMostCols) return fail(DG_E_TOO_LARGE, "more tiles than a launch can count");
+    if (int rc = check_workspace(workspace, workspace_bytes, product_workspace(j.plan, a->rows, b->rows))) return rc;
+    const auto encode = (CUresult(*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                     const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill))encode_tiled_entry();
+    if (!encode) return fail(DG_E_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    // rows of bytes; a copy brings 128 bytes of a tile's rows, what lies outside the matrix as zeros
+    auto map = [&](CUtensorMap* m, const dg_rows8& r, uint32_t box_rows) {
+        const cuuint64_t dim[2] = {r.cols, r.rows}, pitch[1] = {r.ld};
+        const cuuint32_t box[2] = {128, box_rows}, step[2] = {1, 1};
+        return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, r.values, dim, pitch, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    if (!map(&j.a, *a, 128) || !map(&j.b, *b, j.plan.tile_n)) return fail(DG_E_CUDA, "cuTensorMapEncodeTiled rejected an operand");
+    j.a_scales = a->scales; j.b_scales = b->scales;
+    j.a_scale_ld = a->scale_ld; j.b_scale_ld = b->scale_ld;
+    j.a_block = a->block; j.b_block = b->block;
+    j.m = a->rows; j.n = b->rows; j.k = a->cols;
+    j.out = out->data; j.ld = out->ld; j.dtype = out->dtype;
+    j.parts = (float*)workspace;
+    OnDevice on(ctx_device(ctx));
+    if (on.error != cudaSuccess) return fail(DG_E_CUDA, "device %d: %s", ctx_device(ctx), cudaGetErrorString(on.error));
+    const cudaError_t e = launch_product(j, stream_of(ctx, stream));
+    return e == cudaSuccess ? DG_OK : fail(DG_E_CUDA, "launch: %s", cudaGetErrorString(e));
+}
+
+extern "C" int dg_product_status(dg_ctx* ctx, void* stream) {
+    if (int rc = check_ctx(ctx)) return rc;
+    OnDevice on(ctx_device(ctx));
+    unsigned int count = 0;
+    const cudaError_t e = on.error != cudaSuccess ? on.error : product_gave_up(&count, stream_of(ctx, stream));
+    if (e != cudaSuccess) return fail(DG_E_CUDA, "%s", cudaGetErrorString(e));
+    return count ? fail(DG_E_SYNC_LIMIT, "%u CTAs of products gave up waiting for a copy", count) : DG_OK;
+}
+
+extern "C" int dg_rms_norm(dg_ctx* ctx, void* stream, const dg_matrix* x, const dg_matrix* residual, const dg_matrix* weight, float eps,
+                           const dg_matrix* sum, const dg_matrix* y, const dg_rows8* y8, float* rstd) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (int rc = check_matrix(x, "x")) return rc;
+    if (x->cols > kNormMaxCols) return fail(DG_E_TOO_LARGE, "rows of %llu elements: at most %llu", (unsigned long long)x->cols, (unsigned long long)kNormMaxCols);
+    if (residual) {
+        if (int rc = check_matrix(residual, "residual")) return rc;
+        if (residual->cols != x->cols || residual->dtype != x->dtype) return fail(DG_E_INVALID, "residual: the columns and dtype of x are wanted");
+        if (residual->rows == 0 || x->rows % residual->rows || residual->rows >> 32) return fail(DG_E_INVALID, "residual: %llu rows do not divide %llu", (unsigned long long)residual->rows, (unsigned long long)x->rows);
+    }
+    if (int rc = check_weight(weight, x->cols)) return rc;
+    if (!(eps >= 0) || !std::isfinite(eps)) return fail(DG_E_INVALID, "eps is finite and not below 0");
+    if (sum) {
+        if (int rc = check_like(sum, "sum", x->rows, x->cols, x->dtype)) return rc;
+        if (sum->data == x->data && sum->ld != x->ld) return fail(DG_E_INVALID, "sum: in place of x its rows are as far apart");
+    }
+    if (y) if (int rc = check_like(y, "y", x->rows, x->cols, x->dtype)) return rc;
+    if (y8) {
+        if (int rc = check_rows8_like(y8, "y8", x->rows, x->cols)) return rc;
+        if (y8->block != 1) return fail(DG_E_INVALID, "y8: a norm's rows have block 1");
+    }
+    if (int rc = check_floats(rstd, "rstd")) return rc;
+    if (!sum && !y && !y8 && !rstd) return fail(DG_E_INVALID, "no output is wanted");
+    if (x->rows == 0) return DG_OK;
+    NormJob j{};
+    j.rows = x->rows; j.cols = (uint32_t)x->cols; j.dtype = x->dtype; j.eps = eps;
+    j.x = x->data; j.x_ld = x->ld;
+    if (residual) { j.residual = residual->data; j.residual_ld = residual->ld; j.residual_rows = (uint32_t)residual->rows; }
+    if (weight) { j.weight = weight->data; j.weight_dtype = weight->dtype; }
+    if (sum) { j.sum = sum->data; j.sum_ld = sum->ld; }
+    if (y) { j.y = y->data; j.y_ld = y->ld; }
+    if (y8) j.y8 = *y8;
+    j.rstd = rstd;
+    return launched(ctx, [&] { launch_rms_norm(j, stream_of(ctx, stream)); });
+}
+
+extern "C" uint64_t dg_rms_norm_backward_workspace(dg_ctx* ctx, uint64_t rows, uint64_t cols, uint64_t residual_rows) {
+    if (!ctx || rows == 0 || cols == 0 || cols > kNormMaxCols || rows > kMostRows || (residual_rows && rows % residual_rows)) return 0;
+    const uint64_t period = residual_rows ? residual_rows : rows;
+    return norm_backward_workspace(norm_backward_split(rows, cols, period, residual_rows != 0), cols, period);
+}
+
+extern "C" int dg_rms_norm_backward(dg_ctx* ctx, void* stream, const dg_matrix* dy, const dg_matrix* h, const float* rstd, const dg_matrix* weight,
+                                    const dg_matrix* dsum, const dg_matrix* dx, float* dresidual, uint64_t residual_rows, float* dweight,
+                                    void* workspace, uint64_t workspace_bytes) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (int rc = check_matrix(dy, "dy")) return rc;
+    if (dy->cols > kNormMaxCols) return fail(DG_E_TOO_LARGE, "rows of %llu elements: at most %llu", (unsigned long long)dy->cols, (unsigned long long)kNormMaxCols);
+    if (int rc = check_like(h, "h", dy->rows, dy->cols, dy->dtype)) return rc;
+    if (int rc = check_weight(weight, dy->cols)) return rc;
+    if (dsum) if (int rc = check_like(dsum, "dsum", dy->rows, dy->cols, dy->dtype)) return rc;
+    if (dx) {
+        if (int rc = check_like(dx, "dx", dy->rows, dy->cols, dy->dtype)) return rc;
+        if ((dx->data == dy->data && dx->ld != dy->ld) || (dsum && dx->data == dsum->data && dx->ld != dsum->ld))
+            return fail(DG_E_INVALID, "dx: in place of a gradient its rows are as far apart");
+    }
+    if (dy->rows && !rstd) return fail(DG_E_INVALID, "rstd is NULL");
+    if (!dx && !dresidual && !dweight) return fail(DG_E_INVALID, "no output is wanted");
+    for (const float* p : {rstd, (const float*)dresidual, (const float*)dweight})
+        if (int rc = check_floats(p, "rstd, dresidual or dweight")) return rc;
+    if (dresidual && (residual_rows == 0 || dy->rows % residual_rows || residual_rows > kMostRows))
+        return fail(DG_E_INVALID, "%llu residual rows do not divide %llu", (unsigned long long)residual_rows, (unsigned long long)dy->rows);
+    const uint64_t period = dresidual ? residual_rows : dy->rows;
+    if (dy->rows)
+        if (int rc = check_workspace(workspace, workspace_bytes, norm_backward_workspace(norm_backward_split(dy->rows, dy->cols, period, dresidual != nullptr), dy->cols, period))) return rc;
+    NormBackwardJob j{};
+    j.rows = dy->rows; j.period = period; j.cols = (uint32_t)dy->cols; j.dtype = dy->dtype;
+    j.dy = dy->data; j.dy_ld = dy->ld; j.h = h->data; j.h_ld = h->ld; j.rstd = rstd;
+    if (weight) { j.weight = weight->data; j.weight_dtype = weight->dtype; }
+    if (dsum) { j.dsum = dsum->data; j.dsum_ld = dsum->ld; }
+    if (dx) { j.dx = dx->data; j.dx_ld = dx->ld; }
+    j.dresidual = dresidual; j.dweight = dweight;
+    return launched(ctx, [&] { launch_rms_norm_backward(j, (float*)workspace, stream_of(ctx, stream)); });
+}
+
+extern "C" int dg_dropout(dg_ctx* ctx, void* stream, const dg_matrix* x, double p, uint64_t seed, uint64_t offset, int per_row, const dg_matrix* y) {
+    if (int rc = check_ctx(ctx)) return rc;
+    if (int rc = check_matrix(x, "x")) return rc;
+    if (int rc = check_like(y, "y", x->rows, x->cols, x->dtype)) return rc;
+    if (x->data == y->data && x->rows > 1 && x->ld != y->ld) return fail(DG_E_INVALID, "y: in place of x its rows are as far apart");
+    const double t = p >= 0 && p < 1 ? std::floor(p * 65536 + 0.5) : 65536;
+    if (t > 65535) return fail(DG_E_INVALID, "p is in [0, 1) and at most 65535 / 65536");
+    if (offset + x->rows * (per_row ? 1 : x->cols) < offset) return fail(DG_E_INVALID, "offset: the indices pass 2^64");
+    if (x->rows == 0) return DG_OK;
+    const DropoutJob j{x->data, y->data, x->rows, x->cols, x->ld, y->ld, seed, offset, (uint32_t)t, x->dtype, per_row != 0};
+    return launched(ctx, [&] { launch_dropout(j, stream_of(ctx, stream)); });
+}

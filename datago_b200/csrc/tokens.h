@@ -1,0 +1,94 @@
+// Launch interface between the token entry points (tokens.cu) and their kernels.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "../../include/datago_b200.h"
+
+namespace dg {
+
+constexpr uint32_t kScaleGroup = 128;  // columns of 8-bit rows that share a scale
+inline uint64_t scale_groups(uint64_t cols) { return (cols + kScaleGroup - 1) / kScaleGroup; }
+
+constexpr uint32_t kTokenSms = 148;    // of a B200
+
+// ---- 8-bit rows (kernels_tokens.cu) ---------------------------------------------------------------------------------
+struct PatchJob {
+    const uint8_t* pixels;
+    uint32_t n, h, w, channels, patch;
+    float gain[4], shift[4];  // value = pixel * gain + shift
+};
+void launch_patch_rows(const PatchJob& job, const dg_rows8* out8, const dg_matrix* out, cudaStream_t s);
+void launch_quantize_rows(const dg_matrix& src, bool transpose, const dg_rows8& out, cudaStream_t s);
+
+// ---- norm (kernels_tokens.cu) -----------------------------------------------------------------------------------------
+constexpr uint64_t kNormMaxCols = 16384;
+struct NormJob {
+    uint64_t rows;
+    uint32_t cols, residual_rows;
+    int32_t dtype, weight_dtype;
+    const void *x, *residual, *weight;
+    uint64_t x_ld, residual_ld, sum_ld, y_ld;
+    void *sum, *y;
+    dg_rows8 y8;  // values NULL: none
+    float* rstd;
+    float eps;
+};
+void launch_rms_norm(const NormJob& job, cudaStream_t s);
+
+struct NormBackwardJob {
+    uint64_t rows, period;   // period: rows of dresidual, or `rows` without one
+    uint32_t cols;
+    int32_t dtype, weight_dtype;
+    const void *dy, *h, *weight, *dsum;
+    const float* rstd;
+    uint64_t dy_ld, h_ld, dsum_ld, dx_ld;
+    void* dx;
+    float *dresidual, *dweight;
+};
+// How the rows are dealt out: CTAs of the kernel, and the parts that the rows of one residual row are split into.
+struct NormBackwardSplit {
+    uint32_t ctas, parts;
+};
+NormBackwardSplit norm_backward_split(uint64_t rows, uint64_t cols, uint64_t period, bool residual);
+inline uint64_t norm_backward_workspace(const NormBackwardSplit& d, uint64_t cols, uint64_t period) {
+    return 4 * cols * ((uint64_t)d.ctas + (d.parts > 1 ? d.parts * period : 0));
+}
+void launch_rms_norm_backward(const NormBackwardJob& job, float* workspace, cudaStream_t s);
+
+// ---- dropout (kernels_tokens.cu) ----------------------------------------------------------------------------------------
+struct DropoutJob {
+    const void* x;
+    void* y;
+    uint64_t rows, cols, x_ld, y_ld, seed, offset;
+    uint32_t threshold;  // of 65536
+    int32_t dtype;
+    bool per_row;
+};
+void launch_dropout(const DropoutJob& job, cudaStream_t s);
+
+// ---- product (kernels_product.cu) ------------------------------------------------------------------------------------------
+constexpr uint32_t kProductTileM = 128, kProductMaxTileN = 240;
+struct ProductPlan {
+    uint32_t tile_n;           // columns of an output tile
+    uint32_t tiles_m, tiles_n;
+    uint32_t splits, split_groups;  // the contraction is cut into `splits` parts of split_groups groups of 128
+};
+ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t k);
+inline uint64_t product_workspace(const ProductPlan& p, uint64_t m, uint64_t n) {
+    return p.splits > 1 ? (uint64_t)p.splits * m * ((n + 3) / 4 * 4) * 4 : 0;
+}
+struct ProductJob {
+    CUtensorMap a, b;  // boxes of 128 bytes x 128 rows, and of 128 bytes x tile_n rows, 128-byte swizzle
+    const uint8_t *a_scales, *b_scales;
+    uint64_t a_scale_ld, b_scale_ld, m, n, k, ld;
+    uint32_t a_block, b_block;
+    void* out;
+    int32_t dtype;
+    float* parts;
+    ProductPlan plan;
+};
+cudaError_t launch_product(const ProductJob& job, cudaStream_t s);
+cudaError_t product_gave_up(unsigned int* count, cudaStream_t s);  // waits for the stream; the count starts anew
+
+}  // namespace dg

@@ -1,0 +1,327 @@
+"""Token rows: from a bucket of pixels to what a transformer's first layer reads (the dg_patch_rows ... dg_dropout part of
+include/datago_b200.h), on torch tensors.
+
+Every function takes the Context of the tensors' device first, launches on torch's current stream of that device and returns
+without waiting; nothing is kept between calls, so calls can be captured into CUDA graphs.  Results are new tensors unless `out` is given.
+Matrices are 2-d tensors of float32, bfloat16 or float16 whose columns are neighbours in memory; rows may be any distance apart.
+Gradients are calls of their own (rms_norm_backward, dropout on the gradient, product on operands quantised along the contraction);
+PatchStem puts them together for the stem of a model.
+"""
+import ctypes as C
+
+import torch
+
+from . import DatagoB200Error, DeviceArray, _check, lib as _library
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_LEGACY_STREAM = 1  # cudaStreamLegacy: torch's default stream, which has no handle of its own
+GROUP = 128         # columns that share a scale
+
+
+class _Matrix(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("rows", C.c_uint64), ("cols", C.c_uint64), ("ld", C.c_uint64), ("dtype", C.c_int32),
+                ("reserved", C.c_uint32)]
+
+
+class _Rows8(C.Structure):
+    _fields_ = [("values", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_uint64), ("cols", C.c_uint64), ("ld", C.c_uint64),
+                ("scale_ld", C.c_uint64), ("block", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+_lib = None
+
+
+def lib():
+    """The library, with the signatures of the entry points that are used here."""
+    global _lib
+    L = _library()
+    if L is not _lib:
+        vp, mat, rows8, u32, u64 = C.c_void_p, C.POINTER(_Matrix), C.POINTER(_Rows8), C.c_uint32, C.c_uint64
+        sig = {
+            "dg_patch_rows": (C.c_int, [vp, vp, vp, u32, u32, u32, u32, u32, C.POINTER(C.c_float), C.POINTER(C.c_float), rows8, mat]),
+            "dg_quantize_rows": (C.c_int, [vp, vp, mat, C.c_int, rows8]),
+            "dg_product_workspace": (u64, [vp, u64, u64, u64]),
+            "dg_product": (C.c_int, [vp, vp, rows8, rows8, mat, vp, u64]),
+            "dg_product_status": (C.c_int, [vp, vp]),
+            "dg_rms_norm": (C.c_int, [vp, vp, mat, mat, mat, C.c_float, mat, mat, rows8, vp]),
+            "dg_rms_norm_backward_workspace": (u64, [vp, u64, u64, u64]),
+            "dg_rms_norm_backward": (C.c_int, [vp, vp, mat, mat, vp, mat, mat, mat, vp, u64, vp, vp, u64]),
+            "dg_dropout": (C.c_int, [vp, vp, mat, C.c_double, u64, u64, C.c_int, mat]),
+        }
+        for name, (res, args) in sig.items():
+            fn = getattr(L, name)
+            fn.restype, fn.argtypes = res, args
+        _lib = L
+    return L
+
+
+class Rows8:
+    """Rows in 8 bits: values float8_e4m3fn [rows, cols], scales float8_e8m0fnu [ceil(rows / block), ceil(cols / 128)].  Rows of values begin
+    at multiples of 16 bytes, rows of scales at multiples of 4 (what the functions here return, and empty() makes)."""
+    __slots__ = ("values", "scales", "block")
+
+    def __init__(self, values, scales, block=1):
+        self.values, self.scales, self.block = values, scales, block
+
+    @classmethod
+    def empty(cls, rows, cols, device, block=1):
+        groups = -(-cols // GROUP)
+        values = torch.empty((rows, -(-cols // 16) * 16), dtype=torch.float8_e4m3fn, device=device)
+        scales = torch.empty((-(-rows // block), -(-groups // 4) * 4), dtype=torch.float8_e8m0fnu, device=device)
+        return cls(values[:, :cols], scales[:, :groups], block)
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    def to_float(self):
+        """What the rows stand for, as float32."""
+        rows, cols = self.values.shape
+        scales = self.scales.float().repeat_interleave(self.block, 0)[:rows].repeat_interleave(GROUP, 1)[:, :cols]
+        return self.values.float() * scales
+
+
+class Norm:
+    """What rms_norm returns: y (a tensor, or Rows8), sum (h, what the backward pass and the next residual want) and rstd."""
+    __slots__ = ("y", "sum", "rstd")
+
+    def __init__(self, y, sum, rstd):
+        self.y, self.sum, self.rstd = y, sum, rstd
+
+    def __iter__(self):
+        return iter((self.y, self.sum, self.rstd))
+
+
+def _invalid(msg):
+    return DatagoB200Error(1, msg)
+
+
+def _on_device(ctx, t, name):
+    if not isinstance(t, torch.Tensor):
+        raise _invalid(f"{name}: a torch tensor is wanted")
+    if t.device.type != "cuda" or t.device.index != ctx.device:
+        raise _invalid(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
+
+
+def _matrix(ctx, t, name):
+    _on_device(ctx, t, name)
+    dtype = _DTYPES.get(t.dtype)
+    if dtype is None or t.dim() != 2:
+        raise _invalid(f"{name}: a 2-d tensor of float32, bfloat16 or float16 is wanted")
+    rows, cols = t.shape
+    step, one = t.stride()
+    if (one != 1 and cols > 1) or (rows > 1 and step < cols):
+        raise _invalid(f"{name}: columns have to be neighbours in memory, rows apart")
+    return _Matrix(t.data_ptr(), rows, cols, step if rows > 1 else cols, dtype, 0)
+
+
+def _vector(ctx, t, name, cols):
+    """A weight as a matrix of one row."""
+    if t is None:
+        return None
+    _on_device(ctx, t, name)
+    dtype = _DTYPES.get(t.dtype)
+    if dtype is None or t.dim() != 1 or t.shape[0] != cols or (cols > 1 and t.stride(0) != 1):
+        raise _invalid(f"{name}: {cols} neighbouring elements of float32, bfloat16 or float16 are wanted")
+    return _Matrix(t.data_ptr(), 1, cols, cols, dtype, 0)
+
+
+def _floats(ctx, t, name, count):
+    _on_device(ctx, t, name)
+    if t.dtype != torch.float32 or t.numel() != count or not t.is_contiguous():
+        raise _invalid(f"{name}: {count} neighbouring float32 are wanted")
+    return t.data_ptr()
+
+
+def _rows8(ctx, r, name):
+    if not isinstance(r, Rows8):
+        raise _invalid(f"{name}: Rows8 is wanted")
+    v, s = r.values, r.scales
+    _on_device(ctx, v, name)
+    _on_device(ctx, s, name)
+    if v.dtype != torch.float8_e4m3fn or s.dtype != torch.float8_e8m0fnu or v.dim() != 2 or s.dim() != 2 or r.block not in (1, GROUP):
+        raise _invalid(f"{name}: values float8_e4m3fn, scales float8_e8m0fnu, both 2-d, and block 1 or 128 are wanted")
+    (rows, cols), (srows, groups) = v.shape, s.shape
+    if srows != -(-rows // r.block) or groups != -(-cols // GROUP):
+        raise _invalid(f"{name}: {rows} x {cols} values have {-(-rows // r.block)} x {-(-cols // GROUP)} scales")
+    (ld, one), (scale_ld, sone) = v.stride(), s.stride()
+    if (one != 1 and cols > 1) or (sone != 1 and groups > 1):
+        raise _invalid(f"{name}: columns have to be neighbours in memory")
+    if rows <= 1:
+        ld = -(-cols // 16) * 16
+    if srows <= 1:
+        scale_ld = -(-groups // 4) * 4
+    room = s.untyped_storage().nbytes() - s.storage_offset()
+    if srows and (srows - 1) * scale_ld + -(-groups // 4) * 4 > room:
+        raise _invalid(f"{name}: the last row of scales has no room for a multiple of 4 bytes")
+    return _Rows8(v.data_ptr(), s.data_ptr(), rows, cols, ld, scale_ld, r.block, 0)
+
+
+def _ref(m):
+    return None if m is None else C.byref(m)
+
+
+def _stream(t):
+    return torch.cuda.current_stream(t.device).cuda_stream or _LEGACY_STREAM
+
+
+def _out(out, shape, dtype, like, name):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
+        raise _invalid(f"{name}: {tuple(shape)} of {dtype} is wanted")
+    return out
+
+
+def _workspace(nbytes, like):
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+
+
+def patch_rows(ctx, pixels, patch, mean, std, dtype=None, out=None):
+    """Patches of a bucket (uint8 [n, height, width, channels]: a tensor, or a DeviceArray of Batch.buckets()) as rows: Rows8, or with `dtype` a
+    tensor.  Row (i, Y, X), feature (y, x, c) is (pixel / 255 - mean[c]) / std[c]; height and width are multiples of `patch`."""
+    if isinstance(pixels, DeviceArray):
+        pixels = torch.as_tensor(pixels, device=f"cuda:{ctx.device}")
+    _on_device(ctx, pixels, "pixels")
+    if pixels.dtype != torch.uint8 or pixels.dim() != 4 or not pixels.is_contiguous():
+        raise _invalid("pixels: a contiguous uint8 [n, height, width, channels] tensor is wanted")
+    n, h, w, c = pixels.shape
+    if len(mean) != c or len(std) != c:
+        raise _invalid(f"mean and std: {c} numbers are wanted")
+    patch = int(patch)
+    if patch < 1 or h % patch or w % patch or h == 0 or w == 0:
+        raise _invalid(f"{h} x {w} pixels are no whole number of {patch} x {patch} patches")
+    shape = (n * (h // patch) * (w // patch), patch * patch * c)
+    if dtype is None:
+        out = Rows8.empty(*shape, pixels.device) if out is None else out
+        desc8, desc = _rows8(ctx, out, "out"), None
+    else:
+        if dtype not in _DTYPES:
+            raise _invalid("dtype: float32, bfloat16 or float16 is wanted")
+        out = _out(out, shape, dtype, pixels, "out")
+        desc8, desc = None, _matrix(ctx, out, "out")
+    floats = C.c_float * c
+    _check(lib().dg_patch_rows(ctx._h, _stream(pixels), pixels.data_ptr(), n, h, w, c, patch, floats(*mean), floats(*std), _ref(desc8), _ref(desc)))
+    return out
+
+
+def quantize_rows(ctx, x, transpose=False, block=1, out=None):
+    """A matrix, or its transpose, as Rows8, with a scale for each 128 columns of `block` (1 or 128) rows of the result."""
+    src = _matrix(ctx, x, "x")
+    rows, cols = (x.shape[1], x.shape[0]) if transpose else x.shape
+    if out is None:
+        if block not in (1, GROUP):
+            raise _invalid("block is 1 or 128")
+        out = Rows8.empty(rows, cols, x.device, block)
+    _check(lib().dg_quantize_rows(ctx._h, _stream(x), C.byref(src), int(transpose), C.byref(_rows8(ctx, out, "out"))))
+    return out
+
+
+def product(ctx, a, b, dtype=torch.bfloat16, out=None):
+    """a @ b^T of two Rows8 with the same columns, summed in 32 bits: [rows of a, rows of b] of `dtype`."""
+    da, db = _rows8(ctx, a, "a"), _rows8(ctx, b, "b")
+    if dtype not in _DTYPES:
+        raise _invalid("dtype: float32, bfloat16 or float16 is wanted")
+    out = _out(out, (da.rows, db.rows), dtype, a.values, "out")
+    L = lib()
+    nbytes = L.dg_product_workspace(ctx._h, da.rows, db.rows, da.cols)
+    work = _workspace(nbytes, a.values)
+    _check(L.dg_product(ctx._h, _stream(a.values), C.byref(da), C.byref(db), C.byref(_matrix(ctx, out, "out")),
+                        work.data_ptr() if work is not None else None, nbytes))
+    return out
+
+
+def product_status(ctx):
+    """Waits for torch's current stream of the context's device; raises when a product has given up waiting for a copy."""
+    _check(lib().dg_product_status(ctx._h, torch.cuda.current_stream(ctx.device).cuda_stream or _LEGACY_STREAM))
+
+
+def rms_norm(ctx, x, weight=None, residual=None, eps=1e-6, eight_bit=False, sum_out=None):
+    """h = x + residual (row r takes row r % len(residual)), y = h / sqrt(mean(h^2) + eps) * weight: Norm(y, sum=h, rstd).  y is Rows8 with
+    `eight_bit`, else of x's dtype.  sum_out may be x: h in its place."""
+    dx = _matrix(ctx, x, "x")
+    w = _vector(ctx, weight, "weight", dx.cols)
+    r = None if residual is None else _matrix(ctx, residual, "residual")
+    total = _out(sum_out, x.shape, x.dtype, x, "sum_out")
+    rstd = torch.empty(dx.rows, dtype=torch.float32, device=x.device)
+    if eight_bit:
+        y = Rows8.empty(dx.rows, dx.cols, x.device)
+        y16, y8 = None, _rows8(ctx, y, "y")
+    else:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y16, y8 = _matrix(ctx, y, "y"), None
+    _check(lib().dg_rms_norm(ctx._h, _stream(x), C.byref(dx), _ref(r), _ref(w), eps, C.byref(_matrix(ctx, total, "sum_out")), _ref(y16), _ref(y8),
+                             rstd.data_ptr()))
+    return Norm(y, total, rstd)
+
+
+def rms_norm_backward(ctx, dy, h, rstd, weight=None, dsum=None, residual_rows=None, dx_out=None):
+    """Gradients of rms_norm from the gradient of y (and, in dsum, of h): (dx, dresidual, dweight).  dresidual is float32 [residual_rows, cols],
+    or None without residual_rows; dweight float32 [cols].  dx_out may be dy or dsum."""
+    g, hm = _matrix(ctx, dy, "dy"), _matrix(ctx, h, "h")
+    w = _vector(ctx, weight, "weight", g.cols)
+    s = None if dsum is None else _matrix(ctx, dsum, "dsum")
+    dx = _out(dx_out, dy.shape, dy.dtype, dy, "dx_out")
+    period = int(residual_rows or 0)
+    if residual_rows is not None and (period < 1 or g.rows % period):
+        raise _invalid(f"{residual_rows} residual rows do not divide {g.rows}")
+    dweight = torch.empty(g.cols, dtype=torch.float32, device=dy.device)
+    dresidual = torch.empty((period, g.cols), dtype=torch.float32, device=dy.device) if period else None
+    L = lib()
+    nbytes = L.dg_rms_norm_backward_workspace(ctx._h, g.rows, g.cols, period)
+    work = _workspace(nbytes, dy)
+    _check(L.dg_rms_norm_backward(ctx._h, _stream(dy), C.byref(g), C.byref(hm), _floats(ctx, rstd, "rstd", g.rows), _ref(w), _ref(s),
+                                  C.byref(_matrix(ctx, dx, "dx_out")), dresidual.data_ptr() if period else None, period, dweight.data_ptr(),
+                                  work.data_ptr() if work is not None else None, nbytes))
+    return dx, dresidual, dweight
+
+
+def dropout(ctx, x, p, seed, offset=0, per_row=False, out=None):
+    """x with elements (or, per_row, rows) dropped with probability p and the others scaled up.  The mask is a function of (seed, offset + index):
+    the same call on the gradient is the backward pass.  out may be x."""
+    src = _matrix(ctx, x, "x")
+    out = _out(out, x.shape, x.dtype, x, "out")
+    seed, offset = int(seed), int(offset)
+    if not 0 <= seed < 1 << 64 or not 0 <= offset < 1 << 64:
+        raise _invalid("seed and offset are in [0, 2^64)")
+    _check(lib().dg_dropout(ctx._h, _stream(x), C.byref(src), p, seed, offset, int(per_row), C.byref(_matrix(ctx, out, "out"))))
+    return out
+
+
+class PatchStem:
+    """The stem of a model that reads buckets: patches as 8-bit rows, the product with the embedding weight, dropout, positions (shared by
+    the images of a bucket), norm, 8-bit rows for the first layer.
+
+    weight: [width, patch * patch * channels]; norm_weight: [width] or None.  The weight is laid out in 8 bits (scales of 128 x 128 blocks)
+    here and by set_weight, not with every call."""
+
+    def __init__(self, ctx, patch, mean, std, weight, norm_weight=None, p=0.0, seed=0, eps=1e-6, dtype=torch.bfloat16):
+        self.ctx, self.patch, self.mean, self.std = ctx, int(patch), tuple(mean), tuple(std)
+        self.norm_weight, self.p, self.seed, self.eps, self.dtype = norm_weight, float(p), int(seed), float(eps), dtype
+        self.set_weight(weight)
+
+    def set_weight(self, weight):
+        """After an optimizer step: the new weight in 8 bits."""
+        self.weight8 = quantize_rows(self.ctx, weight, block=GROUP)
+
+    def forward(self, pixels, positions, offset=0):
+        """(Norm with Rows8 for the first layer, what backward wants).  positions: [tokens of an image, width].  offset: where this batch's
+        elements begin in the run's count (see dropout)."""
+        if isinstance(pixels, DeviceArray):
+            pixels = torch.as_tensor(pixels, device=f"cuda:{self.ctx.device}")
+        x = product(self.ctx, patch_rows(self.ctx, pixels, self.patch, self.mean, self.std), self.weight8, self.dtype)
+        if self.p:
+            dropout(self.ctx, x, self.p, self.seed, offset, out=x)
+        norm = rms_norm(self.ctx, x, self.norm_weight, residual=positions, eps=self.eps, eight_bit=True, sum_out=x)
+        return norm, (pixels, norm.sum, norm.rstd, len(positions), offset)
+
+    def backward(self, saved, dy, dsum=None):
+        """Gradients (weight, positions, norm_weight), float32, from those of the norm's output and, in dsum, of its sum.  The pixels of
+        the bucket still have to be there."""
+        pixels, h, rstd, tokens, offset = saved
+        dx, dpositions, dnorm = rms_norm_backward(self.ctx, dy, h, rstd, self.norm_weight, dsum, tokens)
+        if self.p:
+            dropout(self.ctx, dx, self.p, self.seed, offset, out=dx)
+        x = patch_rows(self.ctx, pixels, self.patch, self.mean, self.std, self.dtype)
+        dweight = product(self.ctx, quantize_rows(self.ctx, dx, transpose=True), quantize_rows(self.ctx, x, transpose=True), torch.float32)
+        return dweight, dpositions, dnorm

@@ -334,6 +334,85 @@ DG_API int dg_resize_device_static(dg_ctx* ctx, const uint8_t* device_src, uint3
 DG_API int dg_host_alloc(uint64_t nbytes, void** out);
 DG_API void dg_host_release(void* block);
 
+/* ---- token rows: from a bucket of pixels to what a transformer's first layer reads --------------------------------------
+ * A bucket (dg_bucket) leaves the library as dense uint8 [n][height][width][channels] in device memory.  datago stops there
+ * (its user stacks to_numpy_array() copies, src/structs.rs:154-188, and runs torch operations on them); these entry points
+ * take it on: patches as 8-bit rows, the product with the patch-embedding weight, dropout, the norm after the positions
+ * have been added, and the backward pass of each.
+ *
+ * All of them only launch kernels: on `stream`, a cudaStream_t of the context's device (NULL: the ctx stream; the legacy default
+ * stream is cudaStreamLegacy), without allocating, waiting or copying, so they can be captured into a graph.  What they
+ * read has to be complete on that stream, and their results are complete in its order.  Buffers are the caller's, workspaces too: two
+ * calls (or captured graphs) that may run at the same time need workspaces of their own.  The calling thread's current device
+ * is the same after the call.  Outputs may not overlap inputs unless an entry point says so.  With rows == 0 a call does
+ * nothing (gradients of weights become zero). */
+enum { DG_F32 = 0, DG_BF16 = 1, DG_F16 = 2 };
+
+/* A matrix in device memory: row r begins `ld` elements behind row r - 1; data is aligned to its elements (16-byte aligned rows are
+ * faster). */
+typedef struct dg_matrix {
+    void* data;
+    uint64_t rows, cols, ld;
+    int32_t dtype;       /* DG_F32, DG_BF16, DG_F16 */
+    uint32_t reserved;
+} dg_matrix;
+
+/* Rows in 8 bits: e4m3 values and a power-of-two scale (E8M0: the byte e is 2^(e - 127), 255 is NaN) for each 128 columns.
+ * values: row r at r * ld, 16-byte aligned, ld a multiple of 16; bytes behind `cols` are neither read nor written.
+ * scales: row r of values has its bytes at (r / block) * scale_ld, one for each 128 columns, 4-byte aligned, scale_ld a multiple of 4
+ * (bytes behind the last group are read and ignored).  block: the rows that share a scale, 1 or 128. */
+typedef struct dg_rows8 {
+    uint8_t* values;
+    uint8_t* scales;
+    uint64_t rows, cols, ld, scale_ld;
+    uint32_t block, reserved;
+} dg_rows8;
+
+/* Patches of a bucket as rows.  Row (i * h/patch + Y) * w/patch + X, feature (y * patch + x) * channels + c is
+ * (pixels[i][Y * patch + y][X * patch + x][c] / 255 - mean[c]) / std[c].  Exactly one of out8 (block 1) and out (f32, bf16, f16) is
+ * not NULL.  h and w have to be multiples of patch; channels 1 to 4; mean and std hold `channels` host floats, std > 0. */
+DG_API int dg_patch_rows(dg_ctx* ctx, void* stream, const uint8_t* pixels, uint32_t n, uint32_t h, uint32_t w, uint32_t channels,
+                         uint32_t patch, const float* mean, const float* std, const dg_rows8* out8, const dg_matrix* out);
+
+/* A matrix, or its transpose, as 8-bit rows.  A group of 128 columns (and `block` rows) of the result with largest magnitude a
+ * gets the smallest scale s = 2^(e - 127), e in 0..254, with a <= 448 s, and values x / s rounded to the nearest e4m3 (ties to even).  A
+ * group with a NaN or an infinity in it becomes NaN as a whole (e = 255). */
+DG_API int dg_quantize_rows(dg_ctx* ctx, void* stream, const dg_matrix* src, int transpose, const dg_rows8* out);
+
+/* out[m][n] = sum over k of a[m][k] * b[n][k], scales included, accumulated in 32 bits and rounded once.  a->cols == b->cols.  The forward pass
+ * is product(x, w); the input's gradient product(dy, w^T), the weight's product(dy^T, x^T), on operands quantised along the
+ * contraction (dg_quantize_rows transposes).  workspace: dg_product_workspace bytes, 16-byte aligned (may be 0 and NULL). */
+DG_API uint64_t dg_product_workspace(dg_ctx* ctx, uint64_t m, uint64_t n, uint64_t k);
+DG_API int dg_product(dg_ctx* ctx, void* stream, const dg_rows8* a, const dg_rows8* b, const dg_matrix* out, void* workspace,
+                      uint64_t workspace_bytes);
+/* Waits for the stream.  DG_E_SYNC_LIMIT when a product on the device has given up waiting for a copy since the last call (its output is
+ * then undefined): the counterpart of what dg_batch_sync reports for resize passes.  Not inside a stream capture. */
+DG_API int dg_product_status(dg_ctx* ctx, void* stream);
+
+/* h = x + residual (row r takes residual row r % residual->rows, so positions can be shared by all images of a bucket; residual may be
+ * NULL), rstd = 1 / sqrt(mean(h^2) + eps), y = h * rstd * weight (NULL: ones).  x, residual, sum and y have one dtype, weight (1 x cols) any.
+ * Each output may be NULL: sum receives h, y the norm, y8 (block 1) the norm as 8-bit rows, rstd `rows` floats.  sum may be x.
+ * y and y8 come from h before it is rounded to sum's type.  cols at most 32768. */
+DG_API int dg_rms_norm(dg_ctx* ctx, void* stream, const dg_matrix* x, const dg_matrix* residual, const dg_matrix* weight, float eps,
+                       const dg_matrix* sum, const dg_matrix* y, const dg_rows8* y8, float* rstd);
+/* Its backward pass, from dy (gradient of y or, straight through the rounding, of y8), h (what sum received), rstd and weight:
+ *   dx = rstd * (dy * weight - hat * mean(dy * weight * hat)) + dsum,  hat = h * rstd   (dsum: gradient that reaches h otherwise; may be NULL)
+ *   dresidual[t] = sum of dx over the rows r with r % residual_rows == t     (before dx is rounded; residual_rows x cols floats, may be NULL)
+ *   dweight = sum over the rows of dy * hat                                  (cols floats, may be NULL)
+ * dx may be NULL, dy or dsum.  Sums have a fixed order.  residual_rows is ignored without dresidual.  workspace:
+ * dg_rms_norm_backward_workspace bytes, 16-byte aligned. */
+DG_API uint64_t dg_rms_norm_backward_workspace(dg_ctx* ctx, uint64_t rows, uint64_t cols, uint64_t residual_rows);
+DG_API int dg_rms_norm_backward(dg_ctx* ctx, void* stream, const dg_matrix* dy, const dg_matrix* h, const float* rstd, const dg_matrix* weight,
+                                const dg_matrix* dsum, const dg_matrix* dx, float* dresidual, uint64_t residual_rows, float* dweight,
+                                void* workspace, uint64_t workspace_bytes);
+
+/* Dropout whose mask is a function of (seed, index) and never stored: the same call on the output's gradient is the backward pass.
+ * Index: offset + r * cols + c, or offset + r with per_row (whole tokens).  Index i takes 16 bits of a Philox4x32-10 block (Salmon
+ * et al., 2011; counter i >> 3 in the two low words, key `seed`): half i & 7, low half of the first word first.  The element is kept when
+ * those bits are at least t = round(p * 65536), and then multiplied by 65536 / (65536 - t); others become 0, whatever they held.
+ * p in [0, 1) with t <= 65535.  y may be x.  An offset that counts the samples of a run gives every rank, and a resumed run, its own draws. */
+DG_API int dg_dropout(dg_ctx* ctx, void* stream, const dg_matrix* x, double p, uint64_t seed, uint64_t offset, int per_row, const dg_matrix* y);
+
 /* Device -> host copy helper for callers without a CUDA binding (tests). */
 DG_API int dg_copy_to_host(dg_ctx* ctx, void* dst, const void* device_src, uint64_t nbytes);
 
