@@ -169,7 +169,7 @@ pub struct dg_matrix {
     pub reserved: u32,
 }
 
-/// Rows in 8 bits: e4m3 values, an E8M0 scale for each 128 columns of `block` rows; `ld` and `scale_ld` in bytes.
+/// Rows in 8 bits: e4m3 values (by row, or by column), an E8M0 scale for each 128 columns of `block` rows; `ld` and `scale_ld` in bytes.
 #[repr(C)]
 pub struct dg_rows8 {
     pub values: *mut u8,
@@ -179,7 +179,7 @@ pub struct dg_rows8 {
     pub ld: u64,
     pub scale_ld: u64,
     pub block: u32,
-    pub reserved: u32,
+    pub by_column: u32,
 }
 
 pub type dg_log_fn = Option<unsafe extern "C" fn(level: c_int, message: *const c_char, user: *mut c_void)>;
@@ -240,7 +240,7 @@ extern "C" {
                                    device_dst: *mut u8, plan_out: *mut dg_plan) -> c_int;
     pub fn dg_patch_rows(ctx: *mut dg_ctx, stream: *mut c_void, pixels: *const u8, n: u32, h: u32, w: u32, channels: u32, patch: u32,
                          mean: *const f32, std: *const f32, out8: *const dg_rows8, out: *const dg_matrix) -> c_int;
-    pub fn dg_quantize_rows(ctx: *mut dg_ctx, stream: *mut c_void, src: *const dg_matrix, transpose: c_int, out: *const dg_rows8) -> c_int;
+    pub fn dg_quantize_rows(ctx: *mut dg_ctx, stream: *mut c_void, src: *const dg_matrix, out: *const dg_rows8) -> c_int;
     pub fn dg_product_workspace(ctx: *mut dg_ctx, m: u64, n: u64, k: u64) -> u64;
     pub fn dg_product(ctx: *mut dg_ctx, stream: *mut c_void, a: *const dg_rows8, b: *const dg_rows8, out: *const dg_matrix,
                       workspace: *mut c_void, workspace_bytes: u64) -> c_int;

@@ -251,108 +251,129 @@ void patch_rows(const PatchJob& j, const dg_rows8* out8, const dg_matrix* out, c
     else rows_as<PatchSource<C>, __half>(src, *out, s);
 }
 
-// ---- transposed rows, and scales of 128 x 128 blocks ----------------------------------------------------------------------
-// A CTA takes 128 x 128 elements of the source: a thread four neighbouring rows of eight columns.  Transposed, the four values of a
-// column are one word of a row of the result; the words of a row are exchanged by the column's place (word ^ 2 * (column / 8)) so
-// that the lanes of a store hit 32 different banks.
-constexpr uint32_t kTileThreads = 512;
+// ---- scales along the rows of the source, and of 128 x 128 blocks -------------------------------------------------------------
+// The transpose of a matrix stays in the order of the matrix (dg_rows8.by_column): only its scales run along the rows.  A warp holds 256 columns
+// of ROWS rows as they were loaded; the warps of a CTA have 128 rows, the group of a scale, and meet twice over its 256 columns' maxima.
+template <class T> constexpr int kColumnRows = sizeof(T) == 4 ? 8 : 16;  // what fits the registers
+template <class T> constexpr uint32_t kColumnThreads = 128 / kColumnRows<T> * 32;
+constexpr uint32_t kColumnTile = 256;
 
-template <class T, bool TRANSPOSE, bool BLOCK>
-__global__ void __launch_bounds__(kTileThreads) k_tile8(const T* src, uint64_t rows, uint64_t cols, uint64_t ld, bool whole, uint32_t tiles_x,
-                                                        uint64_t tiles, uint8_t* values, uint64_t out_ld, uint8_t* scales, uint64_t scale_ld) {
-    __shared__ uint32_t s_top[128];
-    __shared__ __align__(16) uint32_t s_word[TRANSPOSE ? 128 * 32 : 4];
+template <class T> struct Raw8 {  // eight neighbouring elements as they are in memory
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void widen(float v[8]) const {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = *reinterpret_cast<const float4*>(&w[0]), b = *reinterpret_cast<const float4*>(&w[1]);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            unpack8(w[0], v, T());
+        }
+    }
+    __device__ __forceinline__ void load(const T* p, uint32_t valid, bool whole) {
+        if (whole && valid >= 8) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else {
+            T e[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) e[j] = j < valid ? p[j] : narrow<T>(0.f);
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(e)[i];
+        }
+    }
+};
+// Magnitudes of two 16-bit elements compared at once: like those of 32 bits, they order as whole numbers.
+__device__ __forceinline__ uint32_t larger(uint32_t top, uint32_t v, bf16) { return __vmaxu2(top, v & 0x7FFF7FFFu); }
+__device__ __forceinline__ uint32_t larger(uint32_t top, uint32_t v, __half) { return __vmaxu2(top, v & 0x7FFF7FFFu); }
+__device__ __forceinline__ uint32_t larger(uint32_t top, uint32_t v, float) { return max(top, v & 0x7FFFFFFFu); }
+// the magnitude of 32 bits of one of them
+__device__ __forceinline__ uint32_t magnitude_of(uint32_t half, bf16) { return half << 16; }
+__device__ __forceinline__ uint32_t magnitude_of(uint32_t half, __half) { return __float_as_uint(__half2float(__ushort_as_half((unsigned short)half))); }
+
+// BLOCK: one scale for 128 columns too.  scale_row / scale_col: how far apart the scales of neighbouring groups of rows and of neighbouring
+// columns (blocks of 128 columns) are.
+template <class T, bool BLOCK>
+__global__ void __launch_bounds__(kColumnThreads<T>, 2) k_columns8(const T* src, uint64_t rows, uint64_t cols, uint64_t ld, bool whole, uint32_t tiles_x, uint64_t tiles,
+                                                                   uint8_t* values, uint64_t out_ld, uint8_t* scales, uint64_t scale_row, uint64_t scale_col) {
+    constexpr int R = kColumnRows<T>, kWarps = 128 / R, kWords = sizeof(T) * 2;
+    __shared__ __align__(16) uint32_t s_top[kWarps][32][kWords];
+    __shared__ __align__(16) float s_inverse[kColumnTile];
     let_next_start();
     wait_for_previous();
     src = from_previous(src);
-    const uint32_t cv = threadIdx.x & 15u, rl = threadIdx.x >> 4;  // eight columns from 8 cv, four rows from 4 rl
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     for (uint64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const uint64_t ty = tile / tiles_x, r0 = ty * 128, c0 = (tile - ty * tiles_x) * 128;
-        if (threadIdx.x < 128) s_top[threadIdx.x] = 0;
-        const uint64_t col = c0 + 8 * cv;
+        const uint64_t ty = tile / tiles_x, c0 = (tile - ty * tiles_x) * kColumnTile, col = c0 + 8 * lane, r0 = ty * 128 + warp * R;
         const uint32_t valid = col < cols ? (uint32_t)min((uint64_t)8, cols - col) : 0;
-        float v[4][8];
+        Raw8<T> x[R];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint64_t row = r0 + 4 * rl + i;
-            const bool live = valid && row < rows;
+        for (int i = 0; i < R; ++i) x[i].load(src + (r0 + i) * ld + col, r0 + i < rows ? valid : 0, whole);
+        uint32_t top[kWords] = {};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-            if (live) load8(src + row * ld + col, valid, whole, v[i]);
-        }
-        __syncthreads();  // s_top is 0 (and the tile before this one has left s_word)
-        if constexpr (BLOCK) {
-            uint32_t m = max(max(largest8(v[0]), largest8(v[1])), max(largest8(v[2]), largest8(v[3])));
-            m = __reduce_max_sync(0xFFFFFFFFu, m);
-            if ((threadIdx.x & 31u) == 0) atomicMax(&s_top[0], m);
-        } else {
+        for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                uint32_t m = max(max(magnitude(v[0][j]), magnitude(v[1][j])), max(magnitude(v[2][j]), magnitude(v[3][j])));
-                m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));  // the other four rows of this warp
-                if ((threadIdx.x & 31u) < 16) atomicMax(&s_top[8 * cv + j], m);  // the same whatever the order
+            for (int k = 0; k < kWords / 4; ++k) {
+                top[4 * k] = larger(top[4 * k], x[i].w[k].x, T());
+                top[4 * k + 1] = larger(top[4 * k + 1], x[i].w[k].y, T());
+                top[4 * k + 2] = larger(top[4 * k + 2], x[i].w[k].z, T());
+                top[4 * k + 3] = larger(top[4 * k + 3], x[i].w[k].w, T());
             }
+#pragma unroll
+        for (int k = 0; k < kWords / 4; ++k) *reinterpret_cast<uint4*>(&s_top[warp][lane][4 * k]) = make_uint4(top[4 * k], top[4 * k + 1], top[4 * k + 2], top[4 * k + 3]);
+        __syncthreads();
+        for (uint32_t c = threadIdx.x; c < kColumnTile; c += kColumnThreads<T>) {  // a thread per column
+            uint32_t m = 0;
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) m = max(m, s_top[w][c >> 3][c & 7u]);
+            } else {
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) m = max(m, s_top[w][c >> 3][(c & 7u) >> 1] >> (16 * (c & 1u)) & 0xFFFFu);
+                m = magnitude_of(m, T());
+            }
+            if constexpr (BLOCK) {  // 128 columns are four whole warps
+                m = __reduce_max_sync(0xFFFFFFFFu, m);
+                __shared__ uint32_t s_warp[kColumnTile / 32];
+                if (lane == 0) s_warp[c >> 5] = m;
+                asm volatile("bar.sync 1, 256;" ::: "memory");  // the 256 threads that are here
+                const uint32_t first = c >> 7 << 2;
+                m = max(max(s_warp[first], s_warp[first + 1]), max(s_warp[first + 2], s_warp[first + 3]));
+                if ((c & 127u) == 0 && c0 + c < cols) scales[ty * scale_row + (c0 + c) / 128 * scale_col] = (uint8_t)scale_byte(m);
+            } else if (c0 + c < cols) {
+                scales[ty * scale_row + (c0 + c) * scale_col] = (uint8_t)scale_byte(m);
+            }
+            s_inverse[c] = inverse_scale(scale_byte(m));
         }
         __syncthreads();
-        if constexpr (TRANSPOSE) {
+        float inverse[8];
+        *reinterpret_cast<float4*>(inverse) = *reinterpret_cast<const float4*>(&s_inverse[8 * lane]);
+        *reinterpret_cast<float4*>(inverse + 4) = *reinterpret_cast<const float4*>(&s_inverse[8 * lane + 4]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float inverse = inverse_scale(scale_byte(s_top[BLOCK ? 0 : 8 * cv + j]));
-                s_word[(8 * cv + j) * 32 + (rl ^ (2 * cv))] = e4m3x4(v[0][j] * inverse, v[1][j] * inverse, v[2][j] * inverse, v[3][j] * inverse);
-            }
-            __syncthreads();
-            // rows of the result: columns of the source; eight threads bring the 128 bytes of one
-            for (uint32_t i = threadIdx.x; i < 128 * 8; i += kTileThreads) {
-                const uint32_t c = i >> 3, k = i & 7u, at = c >> 3;  // sixteen bytes from 16 k
-                uint4 q = *reinterpret_cast<const uint4*>(&s_word[c * 32 + ((k ^ (at >> 1)) << 2)]);
-                if (at & 1u) q = make_uint4(q.z, q.w, q.x, q.y);
-                const uint64_t first = r0 + 16 * k;
-                if (c0 + c < cols && first < rows) {
-                    uint8_t* const p = values + (c0 + c) * out_ld + first;
-                    if (first + 16 <= rows) *reinterpret_cast<uint4*>(p) = q;
-                    else {
-                        const uint32_t w[4] = {q.x, q.y, q.z, q.w}, left = (uint32_t)(rows - first);
-#pragma unroll
-                        for (uint32_t j = 0; j < 16; ++j)
-                            if (j < left) p[j] = (uint8_t)(w[j >> 2] >> (8 * (j & 3)));
-                    }
-                }
-            }
-            if constexpr (BLOCK) {
-                if (threadIdx.x == 0) scales[(c0 / 128) * scale_ld + ty] = (uint8_t)scale_byte(s_top[0]);
-            } else {
-                if (threadIdx.x < 128 && c0 + threadIdx.x < cols) scales[(c0 + threadIdx.x) * scale_ld + ty] = (uint8_t)scale_byte(s_top[threadIdx.x]);
-            }
-        } else {
-            const uint32_t e = scale_byte(s_top[0]);
-            const float inverse = inverse_scale(e);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint64_t row = r0 + 4 * rl + i;
-                if (valid && row < rows) store_values8(values + row * out_ld + col, valid, quantize8(v[i], inverse));
-            }
-            if (threadIdx.x == 0) scales[ty * scale_ld + c0 / 128] = (uint8_t)e;
+        for (int i = 0; i < R; ++i) {
+            if (!valid || r0 + i >= rows) continue;
+            float v[8];
+            x[i].widen(v);
+            store_values8(values + (r0 + i) * out_ld + col, valid,
+                          make_uint2(e4m3x4(v[0] * inverse[0], v[1] * inverse[1], v[2] * inverse[2], v[3] * inverse[3]),
+                                     e4m3x4(v[4] * inverse[4], v[5] * inverse[5], v[6] * inverse[6], v[7] * inverse[7])));
         }
-        __syncthreads();  // s_top and s_word are free again
     }
 }
 
 template <class T>
-void quantize_rows(const dg_matrix& m, bool transpose, const dg_rows8& out, cudaStream_t s) {
+void quantize_rows(const dg_matrix& m, const dg_rows8& out, cudaStream_t s) {
     const bool whole = rows_aligned<T>(m.data, m.ld);
-    if (!transpose && out.block == 1) {
+    if (!out.by_column && out.block == 1) {
         rows8(MatrixSource<T>{(const T*)m.data, m.ld, whole}, out, s);
         return;
     }
-    const uint32_t tiles_x = (uint32_t)scale_groups(m.cols);
+    const uint32_t tiles_x = (uint32_t)((m.cols + kColumnTile - 1) / kColumnTile);
     const uint64_t tiles = scale_groups(m.rows) * tiles_x;
     auto go = [&](auto kernel) {
-        launch_after(kernel, grid_for(tiles, 1, 4), kTileThreads, 0, s, (const T*)m.data, m.rows, m.cols, m.ld, whole, tiles_x, tiles, out.values, out.ld,
-                     out.scales, out.scale_ld);
+        launch_after(kernel, grid_for(tiles, 1, 32), kColumnThreads<T>, 0, s, (const T*)m.data, m.rows, m.cols, m.ld, whole, tiles_x, tiles, out.values, out.ld,
+                     out.scales, out.by_column ? 1 : out.scale_ld, out.by_column ? out.scale_ld : 1);
     };
-    if (!transpose) go(k_tile8<T, false, true>);
-    else if (out.block == 1) go(k_tile8<T, true, false>);
-    else go(k_tile8<T, true, true>);
+    if (out.block == 1) go(k_columns8<T, false>);
+    else go(k_columns8<T, true>);
 }
 
 // ---- norm ----------------------------------------------------------------------------------------------------------------------
@@ -703,10 +724,10 @@ void launch_patch_rows(const PatchJob& j, const dg_rows8* out8, const dg_matrix*
     }
 }
 
-void launch_quantize_rows(const dg_matrix& src, bool transpose, const dg_rows8& out, cudaStream_t s) {
-    if (src.dtype == DG_F32) quantize_rows<float>(src, transpose, out, s);
-    else if (src.dtype == DG_BF16) quantize_rows<bf16>(src, transpose, out, s);
-    else quantize_rows<__half>(src, transpose, out, s);
+void launch_quantize_rows(const dg_matrix& src, const dg_rows8& out, cudaStream_t s) {
+    if (src.dtype == DG_F32) quantize_rows<float>(src, out, s);
+    else if (src.dtype == DG_BF16) quantize_rows<bf16>(src, out, s);
+    else quantize_rows<__half>(src, out, s);
 }
 
 void launch_rms_norm(const NormJob& j, cudaStream_t s) {

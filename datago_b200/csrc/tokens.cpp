@@ -13,30 +13,42 @@ using namespace dg;
 // ---- how the work is dealt out ------------------------------------------------------------------------------------------
 namespace dg {
 
-ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t k) {
+ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t k, bool b_by_column) {
     ProductPlan p{};
     if (m == 0 || n == 0) return p;
+    constexpr uint32_t kPairs = kTokenSms / 2;
     const uint32_t groups = (uint32_t)scale_groups(k);
     p.tiles_m = (uint32_t)((m + kProductTileM - 1) / kProductTileM);
-    // as few column tiles as the widest allows, all of them equally wide
-    p.tiles_n = (uint32_t)((n + kProductMaxTileN - 1) / kProductMaxTileN);
-    auto equal_widths = [&] {
-        p.tile_n = (uint32_t)((n + p.tiles_n - 1) / p.tiles_n + 15) / 16 * 16;
-        p.tiles_n = (uint32_t)((n + p.tile_n - 1) / p.tile_n);
-    };
-    equal_widths();
-    // few rows: narrower tiles, so that more SMs fetch the other operand
-    while ((uint64_t)p.tiles_m * p.tiles_n * 2 <= kTokenSms && p.tile_n >= 64) {
-        p.tiles_n *= 2;
-        equal_widths();
+    // Column tiles of one width, as wide as can be (with two accumulators while the contraction is short), or narrower so that more SMs have
+    // one; the contraction whole or in parts.  The cheapest by this measure: a pair takes a group of 128 in a time that goes with its tile's
+    // columns, but no less than that of 96, and as long as for four groups before and after a tile; parts are added up by a launch more.
+    uint64_t best = ~0ull;
+    for (uint64_t want = (n + kProductMaxTileN - 1) / kProductMaxTileN;; want *= 2) {
+        for (const uint32_t widest : {kProductMaxTileN, kProductTwoSums}) {
+            const uint64_t count = std::max<uint64_t>(want, (n + widest - 1) / widest);
+            const uint32_t tile_n = (uint32_t)((n + count - 1) / count + 31) / 32 * 32, tiles_n = (uint32_t)((n + tile_n - 1) / tile_n);
+            const uint64_t tiles = (uint64_t)p.tiles_m * tiles_n;
+            for (uint32_t s = 1; s <= 16 && (s == 1 || s * 8 <= groups); ++s) {
+                const uint32_t each = s == 1 ? groups : ((groups + s - 1) / s + 3) / 4 * 4;  // parts begin at multiples of four groups: the scales come in words
+                const uint64_t parts = (groups + each - 1) / each, rounds = (tiles * parts + kPairs - 1) / kPairs;
+                const uint64_t around = tile_n <= kProductTwoSums ? 256 + (rounds - 1) * 64 : rounds * 256;  // hidden behind the next tile, or not
+                const uint64_t cost = rounds * each * std::max(tile_n, 96u) + 4 * around + (parts > 1 ? 2048 : 0);
+                if (cost < best) {
+                    best = cost;
+                    p.tile_n = tile_n;
+                    p.tiles_n = tiles_n;
+                    p.splits = (uint32_t)parts;
+                    p.split_groups = each;
+                }
+            }
+        }
+        if (p.tiles_m * want * 2 > kPairs || n / want <= 32) break;
     }
-    const uint64_t tiles = (uint64_t)p.tiles_m * p.tiles_n;
-    p.splits = 1;
-    if (tiles < kTokenSms && groups >= 16) p.splits = (uint32_t)std::min<uint64_t>(kTokenSms / tiles, groups / 8);
-    if (p.splits < 1) p.splits = 1;
-    // parts begin at multiples of four groups: the scales come in words
-    p.split_groups = ((groups + p.splits - 1) / p.splits + 3) / 4 * 4;
-    p.splits = (groups + p.split_groups - 1) / p.split_groups;
+    p.sums = p.tile_n <= kProductTwoSums ? 2 : 1;
+    // a stays where its rows leave room for three slots of b and most pairs walk tiles of the same rows
+    const uint32_t b_bytes = (b_by_column ? 128 : p.tile_n / 2) * 128;
+    p.a_stays = p.splits == 1 && groups <= 2 * kProductSlots && groups * kProductABytes + 3 * 2 * b_bytes <= kProductRingBytes && (uint64_t)p.tiles_m * p.tiles_n >= 2 * kPairs && p.tiles_n > 1;
+    p.slots = std::min(kProductSlots, (kProductRingBytes - (p.a_stays ? groups * kProductABytes : 0)) / (2 * (b_bytes + (p.a_stays ? 0 : kProductABytes))));
     return p;
 }
 
@@ -108,7 +120,9 @@ int check_rows8(const dg_rows8* r, const char* name) {
     if (!r) return fail(DG_E_INVALID, "%s is NULL", name);
     if (r->block != 1 && r->block != kScaleGroup) return fail(DG_E_INVALID, "%s: block is 1 or 128", name);
     if (r->cols == 0 || r->cols > kMostCols || r->rows > kMostRows) return fail(DG_E_INVALID, "%s: %llu x %llu elements", name, (unsigned long long)r->rows, (unsigned long long)r->cols);
-    if (r->ld < r->cols || r->ld % 16 || r->ld > kMostElements / (r->rows + 1)) return fail(DG_E_INVALID, "%s: ld is a multiple of 16 and at least cols", name);
+    if (r->by_column > 1) return fail(DG_E_INVALID, "%s: by_column is 0 or 1", name);
+    const uint64_t line = r->by_column ? r->rows : r->cols, lines = r->by_column ? r->cols : r->rows;
+    if (r->ld < line || r->ld % 16 || r->ld > kMostElements / (lines + 1)) return fail(DG_E_INVALID, "%s: ld is a multiple of 16 and at least the %s", name, r->by_column ? "rows" : "cols");
     if (r->scale_ld < scale_groups(r->cols) || r->scale_ld % 4 || r->scale_ld > kMostElements / (r->rows + 1))
         return fail(DG_E_INVALID, "%s: scale_ld is a multiple of 4 and at least a byte per 128 columns", name);
     if (r->rows && (!r->values || !r->scales)) return fail(DG_E_INVALID, "%s: values or scales are NULL", name);
@@ -166,7 +180,7 @@ extern "C" int dg_patch_rows(dg_ctx* ctx, void* stream, const uint8_t* pixels, u
         if (out->rows != rows || out->cols != cols) return fail(DG_E_INVALID, "out: %llu x %llu elements wanted", (unsigned long long)rows, (unsigned long long)cols);
     } else {
         if (int rc = check_rows8_like(out8, "out8", rows, cols)) return rc;
-        if (out8->block != 1) return fail(DG_E_INVALID, "out8: patches have block 1");
+        if (out8->block != 1 || out8->by_column) return fail(DG_E_INVALID, "out8: patches have block 1 and are stored by row");
     }
     PatchJob j{pixels, n, h, w, channels, patch, {}, {}};
     for (uint32_t c = 0; c < channels; ++c) {
@@ -178,13 +192,14 @@ extern "C" int dg_patch_rows(dg_ctx* ctx, void* stream, const uint8_t* pixels, u
     return launched(ctx, [&] { launch_patch_rows(j, out8, out, stream_of(ctx, stream)); });
 }
 
-extern "C" int dg_quantize_rows(dg_ctx* ctx, void* stream, const dg_matrix* src, int transpose, const dg_rows8* out) {
+extern "C" int dg_quantize_rows(dg_ctx* ctx, void* stream, const dg_matrix* src, const dg_rows8* out) {
     if (int rc = check_ctx(ctx)) return rc;
     if (int rc = check_matrix(src, "src")) return rc;
-    if (transpose && src->rows == 0) return fail(DG_E_INVALID, "the transpose of a matrix without rows has no columns");
-    if (int rc = check_rows8_like(out, "out", transpose ? src->cols : src->rows, transpose ? src->rows : src->cols)) return rc;
+    if (!out) return fail(DG_E_INVALID, "out is NULL");
+    if (out->by_column && src->rows == 0) return fail(DG_E_INVALID, "the transpose of a matrix without rows has no columns");
+    if (int rc = check_rows8_like(out, "out", out->by_column ? src->cols : src->rows, out->by_column ? src->rows : src->cols)) return rc;
     if (src->rows == 0) return DG_OK;
-    return launched(ctx, [&] { launch_quantize_rows(*src, transpose != 0, *out, stream_of(ctx, stream)); });
+    return launched(ctx, [&] { launch_quantize_rows(*src, *out, stream_of(ctx, stream)); });
 }
 
 extern "C" uint64_t dg_product_workspace(dg_ctx* ctx, uint64_t m, uint64_t n, uint64_t k) {
@@ -203,20 +218,37 @@ extern "C" int dg_product(dg_ctx* ctx, void* stream, const dg_rows8* a, const dg
     if (out->rows != a->rows || out->cols != b->rows) return fail(DG_E_INVALID, "out: %llu x %llu elements wanted", (unsigned long long)a->rows, (unsigned long long)b->rows);
     if (a->rows == 0) return DG_OK;
     ProductJob j{};
-    j.plan = plan_product(a->rows, b->rows, a->cols);
+    j.plan = plan_product(a->rows, b->rows, a->cols, b->by_column != 0);
     if ((uint64_t)j.plan.tiles_m * j.plan.tiles_n * j.plan.splits > kMostCols) return fail(DG_E_TOO_LARGE, "more tiles than a launch can count");
     if (int rc = check_workspace(workspace, workspace_bytes, product_workspace(j.plan, a->rows, b->rows))) return rc;
     const auto encode = (CUresult(*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                      const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill))encode_tiled_entry();
     if (!encode) return fail(DG_E_CUDA, "the driver has no cuTensorMapEncodeTiled");
-    // rows of bytes; a copy brings 128 bytes of a tile's rows, what lies outside the matrix as zeros
-    auto map = [&](CUtensorMap* m, const dg_rows8& r, uint32_t box_rows) {
-        const cuuint64_t dim[2] = {r.cols, r.rows}, pitch[1] = {r.ld};
-        const cuuint32_t box[2] = {128, box_rows}, step[2] = {1, 1};
-        return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, r.values, dim, pitch, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    auto map = [&](CUtensorMap* m, CUtensorMapDataType type, cuuint32_t dims, void* at, const cuuint64_t* dim, const cuuint64_t* pitch, const cuuint32_t* box,
+                   CUtensorMapSwizzle swizzle) {
+        const cuuint32_t step[3] = {1, 1, 1};
+        return encode(m, type, dims, at, dim, pitch, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
     };
-    if (!map(&j.a, *a, 128) || !map(&j.b, *b, j.plan.tile_n)) return fail(DG_E_CUDA, "cuTensorMapEncodeTiled rejected an operand");
+    // lines of bytes (rows, or columns); a copy brings 128 bytes of them, what lies outside the matrix as zeros
+    auto operand = [&](CUtensorMap* m, const dg_rows8& r, uint32_t rows) {
+        const cuuint64_t dim[2] = {r.by_column ? r.rows : r.cols, r.by_column ? r.cols : r.rows}, pitch[1] = {r.ld};
+        const cuuint32_t box[2] = {128, r.by_column ? 128 : rows};
+        return map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, r.values, dim, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    if (!operand(&j.a, *a, kProductTileM / 2) || !operand(&j.b, *b, j.plan.tile_n / 2)) return fail(DG_E_CUDA, "cuTensorMapEncodeTiled rejected an operand");
+    {  // the output, or its parts; rows that do not start at multiples of 16 bytes are stored without a map
+        const bool split = j.plan.splits > 1;
+        void* const at = split ? workspace : out->data;
+        const int32_t dtype = split ? (int32_t)DG_F32 : out->dtype;
+        const uint64_t ld = (split ? product_part_ld(b->rows) : out->ld) * element(dtype);
+        const cuuint64_t dim[3] = {b->rows, a->rows, j.plan.splits}, pitch[2] = {ld, ld * a->rows};
+        const cuuint32_t box[3] = {(cuuint32_t)(64 / element(dtype)), 32, 1};
+        const CUtensorMapDataType types[3] = {CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16};
+        j.out_by_map = ((uintptr_t)at | ld) % 16 == 0 && pitch[1] < 1ull << 40 &&
+                       map(&j.out_map, types[dtype], 3, at, dim, pitch, box, CU_TENSOR_MAP_SWIZZLE_64B);
+    }
+    j.a_by_column = a->by_column != 0; j.b_by_column = b->by_column != 0;
     j.a_scales = a->scales; j.b_scales = b->scales;
     j.a_scale_ld = a->scale_ld; j.b_scale_ld = b->scale_ld;
     j.a_block = a->block; j.b_block = b->block;
@@ -257,7 +289,7 @@ extern "C" int dg_rms_norm(dg_ctx* ctx, void* stream, const dg_matrix* x, const 
     if (y) if (int rc = check_like(y, "y", x->rows, x->cols, x->dtype)) return rc;
     if (y8) {
         if (int rc = check_rows8_like(y8, "y8", x->rows, x->cols)) return rc;
-        if (y8->block != 1) return fail(DG_E_INVALID, "y8: a norm's rows have block 1");
+        if (y8->block != 1 || y8->by_column) return fail(DG_E_INVALID, "y8: a norm's rows have block 1 and are stored by row");
     }
     if (int rc = check_floats(rstd, "rstd")) return rc;
     if (!sum && !y && !y8 && !rstd) return fail(DG_E_INVALID, "no output is wanted");

@@ -19,7 +19,7 @@ struct PatchJob {
     float gain[4], shift[4];  // value = pixel * gain + shift
 };
 void launch_patch_rows(const PatchJob& job, const dg_rows8* out8, const dg_matrix* out, cudaStream_t s);
-void launch_quantize_rows(const dg_matrix& src, bool transpose, const dg_rows8& out, cudaStream_t s);
+void launch_quantize_rows(const dg_matrix& src, const dg_rows8& out, cudaStream_t s);
 
 // ---- norm (kernels_tokens.cu) -----------------------------------------------------------------------------------------
 constexpr uint64_t kNormMaxCols = 16384;
@@ -68,21 +68,29 @@ struct DropoutJob {
 void launch_dropout(const DropoutJob& job, cudaStream_t s);
 
 // ---- product (kernels_product.cu) ------------------------------------------------------------------------------------------
-constexpr uint32_t kProductTileM = 128, kProductMaxTileN = 240;
+// Tiles of 256 x at most 256; up to 224 columns a tile's sums leave tensor memory while the next tile's are made.
+constexpr uint32_t kProductTileM = 256, kProductMaxTileN = 256, kProductTwoSums = 224;
+constexpr uint32_t kProductRingBytes = 192 * 1024, kProductABytes = kProductTileM / 2 * 128, kProductSlots = 6;
 struct ProductPlan {
-    uint32_t tile_n;           // columns of an output tile
+    uint32_t tile_n;           // columns of an output tile, a multiple of 32
     uint32_t tiles_m, tiles_n;
     uint32_t splits, split_groups;  // the contraction is cut into `splits` parts of split_groups groups of 128
+    uint32_t sums;                  // accumulators
+    uint32_t slots;                 // of 256 columns each, of the ring of b, and of a unless it stays
+    bool a_stays;                   // all groups of a row of tiles have room
 };
-ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t k);
+ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t k, bool b_by_column = false);
+inline uint64_t product_part_ld(uint64_t n) { return (n + 3) / 4 * 4; }
 inline uint64_t product_workspace(const ProductPlan& p, uint64_t m, uint64_t n) {
-    return p.splits > 1 ? (uint64_t)p.splits * m * ((n + 3) / 4 * 4) * 4 : 0;
+    return p.splits > 1 ? (uint64_t)p.splits * m * product_part_ld(n) * 4 : 0;
 }
 struct ProductJob {
-    CUtensorMap a, b;  // boxes of 128 bytes x 128 rows, and of 128 bytes x tile_n rows, 128-byte swizzle
+    // boxes of 128 bytes x 128 (a), tile_n / 2 (b) or, of an operand by column, 128 lines, 128-byte swizzle; of 64 bytes x 32 rows x 1 part, 64-byte swizzle
+    CUtensorMap a, b, out_map;
     const uint8_t *a_scales, *b_scales;
     uint64_t a_scale_ld, b_scale_ld, m, n, k, ld;
     uint32_t a_block, b_block;
+    bool a_by_column, b_by_column, out_by_map;
     void* out;
     int32_t dtype;
     float* parts;

@@ -8,6 +8,7 @@ Gradients are calls of their own (rms_norm_backward, dropout on the gradient, pr
 PatchStem puts them together for the stem of a model.
 """
 import ctypes as C
+import struct
 
 import torch
 
@@ -18,15 +19,10 @@ _LEGACY_STREAM = 1  # cudaStreamLegacy: torch's default stream, which has no han
 GROUP = 128         # columns that share a scale
 
 
-class _Matrix(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("rows", C.c_uint64), ("cols", C.c_uint64), ("ld", C.c_uint64), ("dtype", C.c_int32),
-                ("reserved", C.c_uint32)]
-
-
-class _Rows8(C.Structure):
-    _fields_ = [("values", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_uint64), ("cols", C.c_uint64), ("ld", C.c_uint64),
-                ("scale_ld", C.c_uint64), ("block", C.c_uint32), ("reserved", C.c_uint32)]
-
+# dg_matrix and dg_rows8 of the header as bytes, whose address ctypes passes on: a call makes up to six of them, and a Structure costs
+# four times as much
+_matrix_desc = struct.Struct("QQQQiI").pack  # data, rows, cols, ld, dtype
+_rows8_desc = struct.Struct("QQQQQQII").pack  # values, scales, rows, cols, ld, scale_ld, block
 
 _lib = None
 
@@ -36,17 +32,17 @@ def lib():
     global _lib
     L = _library()
     if L is not _lib:
-        vp, mat, rows8, u32, u64 = C.c_void_p, C.POINTER(_Matrix), C.POINTER(_Rows8), C.c_uint32, C.c_uint64
+        i, u32, u64, vp, f32, f64 = C.c_int, C.c_uint32, C.c_uint64, C.c_void_p, C.c_float, C.c_double
         sig = {
-            "dg_patch_rows": (C.c_int, [vp, vp, vp, u32, u32, u32, u32, u32, C.POINTER(C.c_float), C.POINTER(C.c_float), rows8, mat]),
-            "dg_quantize_rows": (C.c_int, [vp, vp, mat, C.c_int, rows8]),
+            "dg_patch_rows": (i, [vp, vp, vp, u32, u32, u32, u32, u32, vp, vp, vp, vp]),
+            "dg_quantize_rows": (i, [vp, vp, vp, vp]),
             "dg_product_workspace": (u64, [vp, u64, u64, u64]),
-            "dg_product": (C.c_int, [vp, vp, rows8, rows8, mat, vp, u64]),
-            "dg_product_status": (C.c_int, [vp, vp]),
-            "dg_rms_norm": (C.c_int, [vp, vp, mat, mat, mat, C.c_float, mat, mat, rows8, vp]),
+            "dg_product": (i, [vp, vp, vp, vp, vp, vp, u64]),
+            "dg_product_status": (i, [vp, vp]),
+            "dg_rms_norm": (i, [vp, vp, vp, vp, vp, f32, vp, vp, vp, vp]),
             "dg_rms_norm_backward_workspace": (u64, [vp, u64, u64, u64]),
-            "dg_rms_norm_backward": (C.c_int, [vp, vp, mat, mat, vp, mat, mat, mat, vp, u64, vp, vp, u64]),
-            "dg_dropout": (C.c_int, [vp, vp, mat, C.c_double, u64, u64, C.c_int, mat]),
+            "dg_rms_norm_backward": (i, [vp, vp, vp, vp, vp, vp, vp, vp, vp, u64, vp, vp, u64]),
+            "dg_dropout": (i, [vp, vp, vp, f64, u64, u64, i, vp]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(L, name)
@@ -56,19 +52,21 @@ def lib():
 
 
 class Rows8:
-    """Rows in 8 bits: values float8_e4m3fn [rows, cols], scales float8_e8m0fnu [ceil(rows / block), ceil(cols / 128)].  Rows of values begin
-    at multiples of 16 bytes, rows of scales at multiples of 4 (what the functions here return, and empty() makes)."""
+    """Rows in 8 bits: values float8_e4m3fn [rows, cols], scales float8_e8m0fnu [ceil(rows / block), ceil(cols / 128)].  Rows of values, or of
+    a transpose (by_column) columns of values, are neighbours in memory and begin at multiples of 16 bytes, rows of scales at multiples of 4: what
+    the functions here return, and empty() makes."""
     __slots__ = ("values", "scales", "block")
 
     def __init__(self, values, scales, block=1):
         self.values, self.scales, self.block = values, scales, block
 
     @classmethod
-    def empty(cls, rows, cols, device, block=1):
+    def empty(cls, rows, cols, device, block=1, by_column=False):
         groups = -(-cols // GROUP)
-        values = torch.empty((rows, -(-cols // 16) * 16), dtype=torch.float8_e4m3fn, device=device)
-        scales = torch.empty((-(-rows // block), -(-groups // 4) * 4), dtype=torch.float8_e8m0fnu, device=device)
-        return cls(values[:, :cols], scales[:, :groups], block)
+        strides = (1, -(-rows // 16) * 16) if by_column else (-(-cols // 16) * 16, 1)
+        values = torch.empty_strided((rows, cols), strides, dtype=torch.float8_e4m3fn, device=device)
+        scales = torch.empty_strided((-(-rows // block), groups), (-(-groups // 4) * 4, 1), dtype=torch.float8_e8m0fnu, device=device)
+        return cls(values, scales, block)
 
     @property
     def shape(self):
@@ -99,7 +97,7 @@ def _invalid(msg):
 def _on_device(ctx, t, name):
     if not isinstance(t, torch.Tensor):
         raise _invalid(f"{name}: a torch tensor is wanted")
-    if t.device.type != "cuda" or t.device.index != ctx.device:
+    if not t.is_cuda or t.get_device() != ctx.device:
         raise _invalid(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
 
 
@@ -112,7 +110,7 @@ def _matrix(ctx, t, name):
     step, one = t.stride()
     if (one != 1 and cols > 1) or (rows > 1 and step < cols):
         raise _invalid(f"{name}: columns have to be neighbours in memory, rows apart")
-    return _Matrix(t.data_ptr(), rows, cols, step if rows > 1 else cols, dtype, 0)
+    return _matrix_desc(t.data_ptr(), rows, cols, step if rows > 1 else cols, dtype, 0)
 
 
 def _vector(ctx, t, name, cols):
@@ -123,17 +121,11 @@ def _vector(ctx, t, name, cols):
     dtype = _DTYPES.get(t.dtype)
     if dtype is None or t.dim() != 1 or t.shape[0] != cols or (cols > 1 and t.stride(0) != 1):
         raise _invalid(f"{name}: {cols} neighbouring elements of float32, bfloat16 or float16 are wanted")
-    return _Matrix(t.data_ptr(), 1, cols, cols, dtype, 0)
+    return _matrix_desc(t.data_ptr(), 1, cols, cols, dtype, 0)
 
 
-def _floats(ctx, t, name, count):
-    _on_device(ctx, t, name)
-    if t.dtype != torch.float32 or t.numel() != count or not t.is_contiguous():
-        raise _invalid(f"{name}: {count} neighbouring float32 are wanted")
-    return t.data_ptr()
-
-
-def _rows8(ctx, r, name):
+def _rows8(ctx, r, name, transposed=None):
+    """transposed: whether values have to be by column, where the sizes leave it open"""
     if not isinstance(r, Rows8):
         raise _invalid(f"{name}: Rows8 is wanted")
     v, s = r.values, r.scales
@@ -145,36 +137,38 @@ def _rows8(ctx, r, name):
     if srows != -(-rows // r.block) or groups != -(-cols // GROUP):
         raise _invalid(f"{name}: {rows} x {cols} values have {-(-rows // r.block)} x {-(-cols // GROUP)} scales")
     (ld, one), (scale_ld, sone) = v.stride(), s.stride()
-    if (one != 1 and cols > 1) or (sone != 1 and groups > 1):
-        raise _invalid(f"{name}: columns have to be neighbours in memory")
-    if rows <= 1:
-        ld = -(-cols // 16) * 16
-    if srows <= 1:
-        scale_ld = -(-groups // 4) * 4
-    room = s.untyped_storage().nbytes() - s.storage_offset()
-    if srows and (srows - 1) * scale_ld + -(-groups // 4) * 4 > room:
-        raise _invalid(f"{name}: the last row of scales has no room for a multiple of 4 bytes")
-    return _Rows8(v.data_ptr(), s.data_ptr(), rows, cols, ld, scale_ld, r.block, 0)
+    if sone != 1 and groups > 1:
+        raise _invalid(f"{name}: scales have to be neighbours in memory")
+    by_row, by_column = one == 1 or cols <= 1, ld == 1 or rows <= 1
+    if transposed is not None:
+        by_row, by_column = by_row and not transposed, by_column and transposed
+    if by_row:
+        ld, column = ld if rows > 1 else -(-cols // 16) * 16, 0
+    elif by_column:
+        ld, column = one if cols > 1 else -(-rows // 16) * 16, 1
+    else:
+        raise _invalid(f"{name}: rows{' or columns' if transposed is None else ' by column' if transposed else ''} have to be neighbours in memory")
+    return _rows8_desc(v.data_ptr(), s.data_ptr(), rows, cols, ld, scale_ld if srows > 1 else -(-groups // 4) * 4, r.block, column)
 
 
-def _ref(m):
-    return None if m is None else C.byref(m)
-
-
-def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream or _LEGACY_STREAM
+# The current stream's handle without an object around it, where torch has that.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _out(out, shape, dtype, like, name):
     if out is None:
         return torch.empty(shape, dtype=dtype, device=like.device)
-    if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
-        raise _invalid(f"{name}: {tuple(shape)} of {dtype} is wanted")
+    if not isinstance(out, torch.Tensor) or tuple(out.shape) != tuple(shape) or out.dtype != dtype:
+        raise _invalid(f"{name}: a tensor {tuple(shape)} of {dtype} is wanted")
     return out
 
 
 def _workspace(nbytes, like):
-    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+    """(the tensor that keeps it, its address)"""
+    if not nbytes:
+        return None, None
+    work = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    return work, work.data_ptr()
 
 
 def patch_rows(ctx, pixels, patch, mean, std, dtype=None, out=None):
@@ -201,19 +195,21 @@ def patch_rows(ctx, pixels, patch, mean, std, dtype=None, out=None):
         out = _out(out, shape, dtype, pixels, "out")
         desc8, desc = None, _matrix(ctx, out, "out")
     floats = C.c_float * c
-    _check(lib().dg_patch_rows(ctx._h, _stream(pixels), pixels.data_ptr(), n, h, w, c, patch, floats(*mean), floats(*std), _ref(desc8), _ref(desc)))
+    _check(lib().dg_patch_rows(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, pixels.data_ptr(), n, h, w, c, patch, floats(*mean), floats(*std),
+                               desc8, desc))
     return out
 
 
 def quantize_rows(ctx, x, transpose=False, block=1, out=None):
-    """A matrix, or its transpose, as Rows8, with a scale for each 128 columns of `block` (1 or 128) rows of the result."""
+    """A matrix, or its transpose, as Rows8, with a scale for each 128 columns of `block` (1 or 128) rows of the result.  The transpose
+    keeps the matrix's order in memory."""
     src = _matrix(ctx, x, "x")
-    rows, cols = (x.shape[1], x.shape[0]) if transpose else x.shape
+    rows, cols = x.shape
     if out is None:
         if block not in (1, GROUP):
             raise _invalid("block is 1 or 128")
-        out = Rows8.empty(rows, cols, x.device, block)
-    _check(lib().dg_quantize_rows(ctx._h, _stream(x), C.byref(src), int(transpose), C.byref(_rows8(ctx, out, "out"))))
+        out = Rows8.empty(cols, rows, x.device, block, True) if transpose else Rows8.empty(rows, cols, x.device, block)
+    _check(lib().dg_quantize_rows(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, src, _rows8(ctx, out, "out", transpose)))
     return out
 
 
@@ -222,36 +218,37 @@ def product(ctx, a, b, dtype=torch.bfloat16, out=None):
     da, db = _rows8(ctx, a, "a"), _rows8(ctx, b, "b")
     if dtype not in _DTYPES:
         raise _invalid("dtype: float32, bfloat16 or float16 is wanted")
-    out = _out(out, (da.rows, db.rows), dtype, a.values, "out")
+    (m, k), n = a.values.shape, b.values.shape[0]
+    out = _out(out, (m, n), dtype, a.values, "out")
     L = lib()
-    nbytes = L.dg_product_workspace(ctx._h, da.rows, db.rows, da.cols)
-    work = _workspace(nbytes, a.values)
-    _check(L.dg_product(ctx._h, _stream(a.values), C.byref(da), C.byref(db), C.byref(_matrix(ctx, out, "out")),
-                        work.data_ptr() if work is not None else None, nbytes))
+    nbytes = L.dg_product_workspace(ctx._h, m, n, k)
+    work, at = _workspace(nbytes, out)
+    _check(L.dg_product(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, da, db, _matrix(ctx, out, "out"), at, nbytes))
     return out
 
 
 def product_status(ctx):
     """Waits for torch's current stream of the context's device; raises when a product has given up waiting for a copy."""
-    _check(lib().dg_product_status(ctx._h, torch.cuda.current_stream(ctx.device).cuda_stream or _LEGACY_STREAM))
+    _check(lib().dg_product_status(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM))
 
 
 def rms_norm(ctx, x, weight=None, residual=None, eps=1e-6, eight_bit=False, sum_out=None):
     """h = x + residual (row r takes row r % len(residual)), y = h / sqrt(mean(h^2) + eps) * weight: Norm(y, sum=h, rstd).  y is Rows8 with
     `eight_bit`, else of x's dtype.  sum_out may be x: h in its place."""
-    dx = _matrix(ctx, x, "x")
-    w = _vector(ctx, weight, "weight", dx.cols)
+    src = _matrix(ctx, x, "x")
+    rows, cols = x.shape
+    w = _vector(ctx, weight, "weight", cols)
     r = None if residual is None else _matrix(ctx, residual, "residual")
-    total = _out(sum_out, x.shape, x.dtype, x, "sum_out")
-    rstd = torch.empty(dx.rows, dtype=torch.float32, device=x.device)
+    total = _out(sum_out, (rows, cols), x.dtype, x, "sum_out")
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    y16 = y8 = None
     if eight_bit:
-        y = Rows8.empty(dx.rows, dx.cols, x.device)
-        y16, y8 = None, _rows8(ctx, y, "y")
+        y = Rows8.empty(rows, cols, x.device)
+        y8 = _rows8(ctx, y, "y")
     else:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        y16, y8 = _matrix(ctx, y, "y"), None
-    _check(lib().dg_rms_norm(ctx._h, _stream(x), C.byref(dx), _ref(r), _ref(w), eps, C.byref(_matrix(ctx, total, "sum_out")), _ref(y16), _ref(y8),
-                             rstd.data_ptr()))
+        y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+        y16 = _matrix(ctx, y, "y")
+    _check(lib().dg_rms_norm(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, src, r, w, eps, _matrix(ctx, total, "sum_out"), y16, y8, rstd.data_ptr()))
     return Norm(y, total, rstd)
 
 
@@ -259,20 +256,23 @@ def rms_norm_backward(ctx, dy, h, rstd, weight=None, dsum=None, residual_rows=No
     """Gradients of rms_norm from the gradient of y (and, in dsum, of h): (dx, dresidual, dweight).  dresidual is float32 [residual_rows, cols],
     or None without residual_rows; dweight float32 [cols].  dx_out may be dy or dsum."""
     g, hm = _matrix(ctx, dy, "dy"), _matrix(ctx, h, "h")
-    w = _vector(ctx, weight, "weight", g.cols)
+    rows, cols = dy.shape
+    w = _vector(ctx, weight, "weight", cols)
     s = None if dsum is None else _matrix(ctx, dsum, "dsum")
-    dx = _out(dx_out, dy.shape, dy.dtype, dy, "dx_out")
+    _on_device(ctx, rstd, "rstd")
+    if rstd.dtype != torch.float32 or rstd.numel() != rows or not rstd.is_contiguous():
+        raise _invalid(f"rstd: {rows} neighbouring float32 are wanted")
+    dx = _out(dx_out, (rows, cols), dy.dtype, dy, "dx_out")
     period = int(residual_rows or 0)
-    if residual_rows is not None and (period < 1 or g.rows % period):
-        raise _invalid(f"{residual_rows} residual rows do not divide {g.rows}")
-    dweight = torch.empty(g.cols, dtype=torch.float32, device=dy.device)
-    dresidual = torch.empty((period, g.cols), dtype=torch.float32, device=dy.device) if period else None
+    if residual_rows is not None and (period < 1 or rows % period):
+        raise _invalid(f"{residual_rows} residual rows do not divide {rows}")
+    dweight = torch.empty(cols, dtype=torch.float32, device=dy.device)
+    dresidual = torch.empty((period, cols), dtype=torch.float32, device=dy.device) if period else None
     L = lib()
-    nbytes = L.dg_rms_norm_backward_workspace(ctx._h, g.rows, g.cols, period)
-    work = _workspace(nbytes, dy)
-    _check(L.dg_rms_norm_backward(ctx._h, _stream(dy), C.byref(g), C.byref(hm), _floats(ctx, rstd, "rstd", g.rows), _ref(w), _ref(s),
-                                  C.byref(_matrix(ctx, dx, "dx_out")), dresidual.data_ptr() if period else None, period, dweight.data_ptr(),
-                                  work.data_ptr() if work is not None else None, nbytes))
+    nbytes = L.dg_rms_norm_backward_workspace(ctx._h, rows, cols, period)
+    work, at = _workspace(nbytes, dy)
+    _check(L.dg_rms_norm_backward(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, g, hm, rstd.data_ptr(), w, s, _matrix(ctx, dx, "dx_out"),
+                                  dresidual.data_ptr() if period else None, period, dweight.data_ptr(), at, nbytes))
     return dx, dresidual, dweight
 
 
@@ -280,11 +280,14 @@ def dropout(ctx, x, p, seed, offset=0, per_row=False, out=None):
     """x with elements (or, per_row, rows) dropped with probability p and the others scaled up.  The mask is a function of (seed, offset + index):
     the same call on the gradient is the backward pass.  out may be x."""
     src = _matrix(ctx, x, "x")
-    out = _out(out, x.shape, x.dtype, x, "out")
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    else:
+        _out(out, x.shape, x.dtype, x, "out")
     seed, offset = int(seed), int(offset)
     if not 0 <= seed < 1 << 64 or not 0 <= offset < 1 << 64:
         raise _invalid("seed and offset are in [0, 2^64)")
-    _check(lib().dg_dropout(ctx._h, _stream(x), C.byref(src), p, seed, offset, int(per_row), C.byref(_matrix(ctx, out, "out"))))
+    _check(lib().dg_dropout(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, src, p, seed, offset, per_row, _matrix(ctx, out, "out")))
     return out
 
 

@@ -358,14 +358,15 @@ typedef struct dg_matrix {
 } dg_matrix;
 
 /* Rows in 8 bits: e4m3 values and a power-of-two scale (E8M0: the byte e is 2^(e - 127), 255 is NaN) for each 128 columns.
- * values: row r at r * ld, 16-byte aligned, ld a multiple of 16; bytes behind `cols` are neither read nor written.
- * scales: row r of values has its bytes at (r / block) * scale_ld, one for each 128 columns, 4-byte aligned, scale_ld a multiple of 4
- * (bytes behind the last group are read and ignored).  block: the rows that share a scale, 1 or 128. */
+ * values: column c of row r at r * ld + c, or (by_column 1) at c * ld + r; 16-byte aligned, ld a multiple of 16; bytes behind the
+ * last column (row) are neither read nor written.
+ * scales: row r of values has its bytes at (r / block) * scale_ld, one for each 128 columns, 4-byte aligned, scale_ld a multiple of 4;
+ * bytes behind the last group are neither read nor written.  block: the rows that share a scale, 1 or 128. */
 typedef struct dg_rows8 {
     uint8_t* values;
     uint8_t* scales;
     uint64_t rows, cols, ld, scale_ld;
-    uint32_t block, reserved;
+    uint32_t block, by_column;
 } dg_rows8;
 
 /* Patches of a bucket as rows.  Row (i * h/patch + Y) * w/patch + X, feature (y * patch + x) * channels + c is
@@ -374,14 +375,15 @@ typedef struct dg_rows8 {
 DG_API int dg_patch_rows(dg_ctx* ctx, void* stream, const uint8_t* pixels, uint32_t n, uint32_t h, uint32_t w, uint32_t channels,
                          uint32_t patch, const float* mean, const float* std, const dg_rows8* out8, const dg_matrix* out);
 
-/* A matrix, or its transpose, as 8-bit rows.  A group of 128 columns (and `block` rows) of the result with largest magnitude a
+/* A matrix, or with out->by_column its transpose, as 8-bit rows (either way the values keep the order of the matrix; by_column, the
+ * scales run along its rows: an operand whose contraction runs over them).  A group of 128 columns (and `block` rows) of the result with largest magnitude a
  * gets the smallest scale s = 2^(e - 127), e in 0..254, with a <= 448 s, and values x / s rounded to the nearest e4m3 (ties to even).  A
  * group with a NaN or an infinity in it becomes NaN as a whole (e = 255). */
-DG_API int dg_quantize_rows(dg_ctx* ctx, void* stream, const dg_matrix* src, int transpose, const dg_rows8* out);
+DG_API int dg_quantize_rows(dg_ctx* ctx, void* stream, const dg_matrix* src, const dg_rows8* out);
 
 /* out[m][n] = sum over k of a[m][k] * b[n][k], scales included, accumulated in 32 bits and rounded once.  a->cols == b->cols.  The forward pass
  * is product(x, w); the input's gradient product(dy, w^T), the weight's product(dy^T, x^T), on operands quantised along the
- * contraction (dg_quantize_rows transposes).  workspace: dg_product_workspace bytes, 16-byte aligned (may be 0 and NULL). */
+ * contraction (dg_quantize_rows, by_column).  workspace: dg_product_workspace bytes, 16-byte aligned (may be 0 and NULL). */
 DG_API uint64_t dg_product_workspace(dg_ctx* ctx, uint64_t m, uint64_t n, uint64_t k);
 DG_API int dg_product(dg_ctx* ctx, void* stream, const dg_rows8* a, const dg_rows8* b, const dg_matrix* out, void* workspace,
                       uint64_t workspace_bytes);

@@ -7,10 +7,10 @@ static unsigned int gave_up = 0;
 extern "C" {
 int fake_launches() { int n = launches; launches = 0; return n; }
 void fake_gave_up(unsigned int n) { gave_up = n; }
-void fake_product_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t out[5]) {
+void fake_product_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t out[6]) {
     const dg::ProductPlan p = dg::plan_product(m, n, k);
-    const uint32_t v[5] = {p.tile_n, p.tiles_m, p.tiles_n, p.splits, p.split_groups};
-    for (int i = 0; i < 5; ++i) out[i] = v[i];
+    const uint32_t v[6] = {p.tile_n, p.tiles_m, p.tiles_n, p.splits, p.split_groups, p.sums};
+    for (int i = 0; i < 6; ++i) out[i] = v[i];
 }
 void fake_backward_split(uint64_t rows, uint64_t cols, uint64_t period, int residual, uint32_t out[2]) {
     const dg::NormBackwardSplit d = dg::norm_backward_split(rows, cols, period, residual != 0);
@@ -21,7 +21,7 @@ void fake_backward_split(uint64_t rows, uint64_t cols, uint64_t period, int resi
 
 namespace dg {
 void launch_patch_rows(const PatchJob&, const dg_rows8*, const dg_matrix*, cudaStream_t) { ++launches; }
-void launch_quantize_rows(const dg_matrix&, bool, const dg_rows8&, cudaStream_t) { ++launches; }
+void launch_quantize_rows(const dg_matrix&, const dg_rows8&, cudaStream_t) { ++launches; }
 void launch_rms_norm(const NormJob&, cudaStream_t) { ++launches; }
 void launch_rms_norm_backward(const NormBackwardJob&, float*, cudaStream_t) { ++launches; }
 void launch_dropout(const DropoutJob&, cudaStream_t) { ++launches; }

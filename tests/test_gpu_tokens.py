@@ -184,6 +184,16 @@ def test_product_of_every_kind_of_scales(ctx, a_block, b_block):
     check_product(ctx, operand(ctx, 130, 5000, a_block, 3), operand(ctx, 140, 5000, b_block, 4), F32)
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (33, 47, 130), (130, 200, 300), (257, 520, 1000), (1152, 768, 5000), (300, 96, 40)])
+@pytest.mark.parametrize("a_turned,b_turned", [(True, True), (True, False), (False, True)])
+@pytest.mark.parametrize("block", [1, 128])
+def test_product_of_transposed_operands(ctx, m, n, k, a_turned, b_turned, block):
+    def operand_of(rows, seed, turned):
+        x = rand((k, rows) if turned else (rows, k), F32, seed)
+        return tk.quantize_rows(ctx, placed(x, 3, 5)[0], transpose=turned, block=block)
+    check_product(ctx, operand_of(m, 1, a_turned), operand_of(n, 2, b_turned), F32)
+
+
 def test_product_of_more_tiles_than_the_chip_holds(ctx):
     check_product(ctx, operand(ctx, 20001, 200, 1, 5), operand(ctx, 1000, 200, 128, 6), BF16)
 
@@ -511,8 +521,7 @@ def test_the_stream_of_the_context_is_used_without_one():
     own = dg.Context(0)
     src = tk._matrix(own, x, "x")
     out = tk.Rows8.empty(300, 256, "cuda")
-    import ctypes as C
-    assert tk.lib().dg_quantize_rows(own._h, None, C.byref(src), 0, C.byref(tk._rows8(own, out, "out"))) == 0
+    assert tk.lib().dg_quantize_rows(own._h, None, src, tk._rows8(own, out, "out")) == 0
     torch.cuda.ExternalStream(own.stream).synchronize()
     same_rows8(out, x.double(), 1)
 

@@ -43,15 +43,11 @@ def ctx(L):
 
 
 def matrix(rows=4, cols=256, ld=None, dtype=1, data=AT):
-    return tk._Matrix(data, rows, cols, cols if ld is None else ld, dtype, 0)
+    return tk._matrix_desc(data or 0, rows, cols, cols if ld is None else ld, dtype, 0)
 
 
-def rows8(rows=4, cols=256, ld=None, scale_ld=None, block=1, values=AT, scales=AT):
-    return tk._Rows8(values, scales, rows, cols, -(-cols // 16) * 16 if ld is None else ld, -(-cols // 512) * 4 if scale_ld is None else scale_ld, block, 0)
-
-
-def ref(m):
-    return None if m is None else C.byref(m)
+def rows8(rows=4, cols=256, ld=None, scale_ld=None, block=1, values=AT, scales=AT, by_column=0):
+    return tk._rows8_desc(values or 0, scales or 0, rows, cols, -(-(rows if by_column else cols) // 16) * 16 if ld is None else ld, -(-cols // 512) * 4 if scale_ld is None else scale_ld, block, by_column)
 
 
 BAD_MATRICES = [None, matrix(cols=0), matrix(ld=255), matrix(dtype=3), matrix(dtype=-1), matrix(data=None), matrix(data=AT + 1), matrix(dtype=0, data=AT + 2),
@@ -75,48 +71,51 @@ def test_a_planning_context_and_no_context_have_no_token_rows(L):
     planning = dg.Context(dg.DG_DEVICE_NONE)
     for ctx in (planning._h, None):
         m, r = matrix(), rows8()
-        refused(L, L.dg_quantize_rows(ctx, None, ref(m), 0, ref(r)))
-        refused(L, L.dg_product(ctx, None, ref(r), ref(r), ref(matrix(4, 4)), None, 0))
+        refused(L, L.dg_quantize_rows(ctx, None, (m), (r)))
+        refused(L, L.dg_product(ctx, None, (r), (r), (matrix(4, 4)), None, 0))
         refused(L, L.dg_product_status(ctx, None))
-        refused(L, L.dg_dropout(ctx, None, ref(m), 0.1, 0, 0, 0, ref(m)))
-        refused(L, L.dg_rms_norm(ctx, None, ref(m), None, None, 1e-6, None, ref(matrix(data=2 * AT)), None, None))
+        refused(L, L.dg_dropout(ctx, None, (m), 0.1, 0, 0, 0, (m)))
+        refused(L, L.dg_rms_norm(ctx, None, (m), None, None, 1e-6, None, (matrix(data=2 * AT)), None, None))
         one = (C.c_float * 3)(1, 1, 1)
-        refused(L, L.dg_patch_rows(ctx, None, AT, 1, 16, 16, 3, 16, one, one, ref(rows8(1, 768)), None))
+        refused(L, L.dg_patch_rows(ctx, None, AT, 1, 16, 16, 3, 16, one, one, (rows8(1, 768)), None))
 
 
 def test_quantize_rows_refuses(L, ctx):
-    call = lambda m, t, r: L.dg_quantize_rows(ctx._h, None, ref(m), t, ref(r))  # noqa: E731
+    call = lambda m, r: L.dg_quantize_rows(ctx._h, None, m, r)  # noqa: E731
     for m in BAD_MATRICES:
-        refused(L, call(m, 0, rows8()))
+        refused(L, call(m, rows8()))
     for r in BAD_ROWS8:
-        refused(L, call(matrix(), 0, r))
-    refused(L, call(matrix(), 1, rows8()))                       # the transpose has 256 rows
-    refused(L, call(matrix(rows=0), 1, rows8(256, 16)))
-    launched(L, call(matrix(), 0, rows8()))
-    launched(L, call(matrix(), 0, rows8(block=128)))
-    launched(L, call(matrix(ld=300), 1, rows8(256, 4)))
-    launched(L, call(matrix(rows=0, data=None), 0, rows8(0, values=None, scales=None)), 0)
+        refused(L, call(matrix(), r))
+    refused(L, call(matrix(), rows8(by_column=1)))               # the transpose has 256 rows
+    refused(L, call(matrix(), rows8(256, 4, by_column=1, ld=240)))
+    refused(L, call(matrix(), rows8(256, 4, by_column=2)))
+    refused(L, call(matrix(rows=0), rows8(256, 16, by_column=1)))
+    launched(L, call(matrix(), rows8()))
+    launched(L, call(matrix(), rows8(block=128)))
+    launched(L, call(matrix(ld=300), rows8(256, 4, by_column=1)))
+    launched(L, call(matrix(rows=0, data=None), rows8(0, values=None, scales=None)), 0)
 
 
 def test_patch_rows_refuses(L, ctx):
     one, zero, nan = (C.c_float * 4)(1, 1, 1, 1), (C.c_float * 4)(1, 0, 1, 1), (C.c_float * 4)(1, float("nan"), 1, 1)
 
     def call(n=2, h=32, w=48, c=3, p=16, mean=one, std=one, out8=rows8(12, 768), out=None, pixels=AT):
-        return L.dg_patch_rows(ctx._h, None, pixels, n, h, w, c, p, mean, std, ref(out8), ref(out))
+        return L.dg_patch_rows(ctx._h, None, pixels, n, h, w, c, p, mean, std, (out8), (out))
     launched(L, call())
     launched(L, call(out8=None, out=matrix(12, 768)))
     launched(L, call(n=0, pixels=None, out8=rows8(0, 768)), 0)
     for bad in (dict(out8=None), dict(out=matrix(12, 768)), dict(mean=None), dict(std=None), dict(c=0), dict(c=5), dict(p=0), dict(p=5), dict(h=0), dict(h=40), dict(w=40),
-                dict(std=zero), dict(std=nan), dict(mean=nan), dict(pixels=None), dict(out8=rows8(11, 768)), dict(out8=rows8(12, 256)), dict(out8=rows8(12, 768, block=128)),
+                dict(std=zero), dict(std=nan), dict(mean=nan), dict(pixels=None), dict(out8=rows8(11, 768)), dict(out8=rows8(12, 256)), dict(out8=rows8(12, 768, block=128)), dict(out8=rows8(12, 768, by_column=1)),
                 dict(out8=None, out=matrix(12, 767)), dict(n=1 << 20)):
         refused(L, call(**bad))
 
 
 def test_product_refuses(L, ctx):
     def call(a=rows8(), b=rows8(8), out=matrix(4, 8), work=None, nbytes=0):
-        return L.dg_product(ctx._h, None, ref(a), ref(b), ref(out), work, nbytes)
+        return L.dg_product(ctx._h, None, (a), (b), (out), work, nbytes)
     launched(L, call())
     launched(L, call(a=rows8(block=128), b=rows8(8, block=128)))
+    launched(L, call(a=rows8(by_column=1), b=rows8(8, by_column=1)))
     launched(L, call(a=rows8(0, values=None, scales=None), out=matrix(0, 8, data=None)), 0)
     for r in BAD_ROWS8:
         refused(L, call(a=r))
@@ -148,7 +147,7 @@ def test_rms_norm_refuses(L, ctx):
     out = matrix(data=2 * AT)
 
     def call(x=matrix(), residual=None, weight=None, eps=1e-6, sum=None, y=out, y8=None, rstd=None):
-        return L.dg_rms_norm(ctx._h, None, ref(x), ref(residual), ref(weight), eps, ref(sum), ref(y), ref(y8), rstd)
+        return L.dg_rms_norm(ctx._h, None, (x), (residual), (weight), eps, (sum), (y), (y8), rstd)
     launched(L, call())
     launched(L, call(residual=matrix(2), weight=matrix(1, dtype=0), sum=matrix(), y=None, y8=rows8(), rstd=AT))
     launched(L, call(x=matrix(0, data=None), y=matrix(0, data=None)), 0)
@@ -162,7 +161,7 @@ def test_rms_norm_refuses(L, ctx):
         refused(L, call(y8=r))
     for bad in (dict(residual=matrix(3)), dict(residual=matrix(0)), dict(residual=matrix(cols=128, ld=128)), dict(residual=matrix(dtype=0)), dict(weight=matrix(2)),
                 dict(weight=matrix(1, 128)), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")), dict(sum=matrix(ld=512)), dict(sum=matrix(5)),
-                dict(y=matrix(dtype=0)), dict(y8=rows8(block=128)), dict(y8=rows8(5)), dict(rstd=AT + 1), dict(y=None)):
+                dict(y=matrix(dtype=0)), dict(y8=rows8(block=128)), dict(y8=rows8(by_column=1)), dict(y8=rows8(5)), dict(rstd=AT + 1), dict(y=None)):
         refused(L, call(**bad))
     wide = matrix(cols=16392, ld=16392)
     refused(L, call(x=wide, y=wide), TOO_LARGE)
@@ -173,7 +172,7 @@ def test_rms_norm_backward_refuses(L, ctx):
     assert need > 0
 
     def call(dy=matrix(), h=matrix(), rstd=AT, weight=None, dsum=None, dx=matrix(), dr=AT, period=2, dw=AT, work=AT, nbytes=need):
-        return L.dg_rms_norm_backward(ctx._h, None, ref(dy), ref(h), rstd, ref(weight), ref(dsum), ref(dx), dr, period, dw, work, nbytes)
+        return L.dg_rms_norm_backward(ctx._h, None, (dy), (h), rstd, (weight), (dsum), (dx), dr, period, dw, work, nbytes)
     launched(L, call())
     launched(L, call(dx=None, dr=None, period=7))
     empty = matrix(0, data=None)
@@ -193,7 +192,7 @@ def test_rms_norm_backward_refuses(L, ctx):
 
 def test_dropout_refuses(L, ctx):
     def call(x=matrix(), p=0.1, seed=1, offset=0, per_row=0, y=matrix(data=2 * AT)):
-        return L.dg_dropout(ctx._h, None, ref(x), p, seed, offset, per_row, ref(y))
+        return L.dg_dropout(ctx._h, None, (x), p, seed, offset, per_row, (y))
     launched(L, call())
     launched(L, call(y=matrix()))
     launched(L, call(p=0.0))
@@ -210,13 +209,13 @@ def test_dropout_refuses(L, ctx):
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 48, 64), (7, 1024, 768), (128, 240, 128), (129, 241, 129), (200, 4801, 512), (1152, 768, 57600), (131072, 1152, 768),
                                    (37, 65, 1 << 20), (1 << 20, 16, 16), (5, 1 << 17, 640)])
 def test_product_plans_cover_the_output_and_the_contraction(L, m, n, k):
-    v = (C.c_uint32 * 5)()
+    v = (C.c_uint32 * 6)()
     L.fake_product_plan(C.c_uint64(m), C.c_uint64(n), C.c_uint64(k), v)
-    tile_n, tiles_m, tiles_n, splits, per_split = v
+    tile_n, tiles_m, tiles_n, splits, per_split, sums = v
     groups = -(-k // 128)
-    assert tile_n % 16 == 0 and 16 <= tile_n <= 256
-    assert (tiles_m - 1) * 128 < m <= tiles_m * 128 and (tiles_n - 1) * tile_n < n <= tiles_n * tile_n
-    assert per_split % 4 == 0 and (splits - 1) * per_split < groups <= splits * per_split
+    assert tile_n % 32 == 0 and 32 <= tile_n <= (256 if sums == 1 else 224)
+    assert (tiles_m - 1) * 256 < m <= tiles_m * 256 and (tiles_n - 1) * tile_n < n <= tiles_n * tile_n
+    assert (splits == 1 or per_split % 4 == 0) and (splits - 1) * per_split < groups <= splits * per_split
 
 
 @pytest.mark.parametrize("rows,cols,period,residual", [(1, 8, 1, 0), (1, 8, 1, 1), (100000, 1152, 1, 1), (55056, 1152, 2294, 1), (55056, 1152, 55056, 0), (64, 16384, 4, 1), (12, 300, 12, 1)])
