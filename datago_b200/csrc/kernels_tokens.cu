@@ -91,6 +91,34 @@ __device__ __forceinline__ void load8_any(const void* p, uint64_t at, int32_t dt
 }
 template <class T> bool rows_aligned(const void* p, uint64_t ld) { return ((reinterpret_cast<uintptr_t>(p) | (ld * sizeof(T))) & 15u) == 0; }
 
+template <class T> struct Raw8 {  // eight neighbouring elements as they are in memory
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void widen(float v[8]) const {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = *reinterpret_cast<const float4*>(&w[0]), b = *reinterpret_cast<const float4*>(&w[1]);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            unpack8(w[0], v, T());
+        }
+    }
+    __device__ __forceinline__ void load_whole(const T* p, bool there) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = there ? reinterpret_cast<const uint4*>(p)[i] : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(const T* p, uint32_t valid, bool whole) {
+        if (whole && valid >= 8) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else {
+            T e[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) e[j] = j < valid ? p[j] : narrow<T>(0.f);
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(e)[i];
+        }
+    }
+};
+
 // ---- scales -------------------------------------------------------------------------------------------------------------
 // Magnitudes are compared as bit patterns: those of finite numbers order like the numbers, an infinity is above them and a NaN above that.
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
@@ -131,124 +159,254 @@ __device__ __forceinline__ void store_values8(uint8_t* p, uint32_t valid, uint2 
             if (j < valid) p[j] = (uint8_t)((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
 }
 
-// ---- rows of a matrix or of a bucket's patches -----------------------------------------------------------------------------
-template <class T> struct MatrixSource {
-    const T* data;
-    uint64_t ld;
-    bool whole;
-    __device__ __forceinline__ void load(uint64_t row, uint32_t col, uint32_t valid, float v[8]) const {
-        load8(from_previous(data) + row * ld + col, valid, whole, v);
-    }
-};
-// C channels.  A patch's row of pixels is patch * C neighbouring bytes; whole: those begin at multiples of eight, everywhere.
-template <int C> struct PatchSource {
-    const uint8_t* pixels;
-    uint32_t grid_w, per_image, patch, segment;  // patches per row and per image; segment = patch * C
-    uint64_t pitch, image;                       // bytes of a row of pixels and of an image
-    float gain[C], shift[C];
-    bool whole;
-    __device__ __forceinline__ void load(uint64_t row, uint32_t col, uint32_t valid, float v[8]) const {
-        const uint64_t i = row / per_image;
-        const uint32_t r = (uint32_t)(row - i * per_image), Y = r / grid_w, X = r - Y * grid_w;
-        const uint8_t* p = from_previous(pixels) + i * image + (uint64_t)Y * patch * pitch + (uint64_t)X * segment;
-        uint32_t y = col / segment, b = col - y * segment;
-        const uint32_t phase = col % C;  // channel of the first feature
-        uint32_t px[8];
-        if (whole && valid >= 8) {
-            const uint2 w = *reinterpret_cast<const uint2*>(p + y * pitch + b);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) px[j] = ((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 255u;
-        } else {
-            const uint8_t* q = p + y * pitch;
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) {
-                px[j] = j < valid ? q[b] : 0;
-                if (++b == segment) { b = 0; q += pitch; }
-            }
-        }
-        float g[C], s[C];
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            g[c] = gain[c];
-            s[c] = shift[c];
-#pragma unroll
-            for (int k = 1; k < C; ++k)
-                if (phase == (uint32_t)k) { g[c] = gain[(c + k) % C]; s[c] = shift[(c + k) % C]; }
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) v[j] = j < valid ? fmaf((float)px[j], g[j % C], s[j % C]) : 0.f;
-    }
-};
-
 constexpr uint32_t kRowThreads = 256;
-
-// Sixteen lanes per group of 128 columns; four groups of a half-warp in flight.
-template <class Source>
-__global__ void __launch_bounds__(kRowThreads) k_rows8(Source src, uint64_t ngroups, uint32_t groups, uint32_t cols, uint8_t* values, uint64_t ld,
-                                                       uint8_t* scales, uint64_t scale_ld) {
-    let_next_start();
-    wait_for_previous();
-    const uint32_t lane = threadIdx.x & 15u;
-    const uint64_t stride = (uint64_t)gridDim.x * (kRowThreads / 16);
-    // whole half-warps leave together, and a warp's two halves differ by one group: both stay while the lower one has work
-    for (uint64_t g = (uint64_t)blockIdx.x * (kRowThreads / 16) + (threadIdx.x >> 4); (g & ~1ull) < ngroups; g += stride) {
-        const uint64_t row = g / groups;
-        const uint32_t group = (uint32_t)(g - row * groups), col = group * kScaleGroup + lane * 8;
-        const uint32_t valid = g < ngroups && col < cols ? min(8u, cols - col) : 0;
-        float v[8] = {};
-        if (valid) src.load(row, col, valid, v);
-        const uint32_t e = scale_byte(largest_of_16_lanes(largest8(v)));
-        if (valid) store_values8(values + row * ld + col, valid, quantize8(v, inverse_scale(e)));
-        if (lane == 0 && valid) scales[row * scale_ld + group] = (uint8_t)e;
-    }
-}
-
-template <class Source, class T>
-__global__ void __launch_bounds__(kRowThreads) k_rows(Source src, uint64_t nvec, uint32_t per_row, uint32_t cols, T* out, uint64_t ld, bool whole) {
-    let_next_start();
-    wait_for_previous();
-    for (uint64_t i = (uint64_t)blockIdx.x * kRowThreads + threadIdx.x; i < nvec; i += (uint64_t)gridDim.x * kRowThreads) {
-        const uint64_t row = i / per_row;
-        const uint32_t col = (uint32_t)(i - row * per_row) * 8, valid = min(8u, cols - col);
-        float v[8];
-        src.load(row, col, valid, v);
-        store8(out + row * ld + col, valid, whole, v);
-    }
-}
 
 uint32_t grid_for(uint64_t items, uint32_t per_cta, uint32_t ctas_per_sm) {
     return (uint32_t)std::min<uint64_t>((items + per_cta - 1) / per_cta, (uint64_t)kSms * ctas_per_sm);
 }
 
-template <class Source>
-void rows8(const Source& src, const dg_rows8& out, cudaStream_t s) {
-    const uint64_t groups = scale_groups(out.cols), n = out.rows * groups;
-    launch_after(k_rows8<Source>, grid_for(n, kRowThreads / 16, 32), kRowThreads, 0, s, src, n, (uint32_t)groups, (uint32_t)out.cols, out.values, out.ld,
-                 out.scales, out.scale_ld);
+// Division of n < 2^31 by a number that is the same for a whole launch: with 2^s >= d, n / d = n * ceil(2^(31 + s) / d) / 2^(31 + s) rounded down,
+// because the ceiling is off by less than n / 2^(31 + s) < 1 / d.
+struct Divisor {
+    uint32_t d, factor, shift;
+    explicit Divisor(uint32_t by) : d(by), factor(0), shift(31) {
+        while ((1ull << (shift - 31)) < by) ++shift;
+        factor = (uint32_t)(((1ull << shift) + by - 1) / by);
+    }
+    __device__ __forceinline__ uint32_t of(uint32_t n, uint32_t& rest) const {
+        const uint32_t q = (uint32_t)((uint64_t)n * factor >> shift);
+        rest = n - q * d;
+        return q;
+    }
+};
+constexpr uint64_t kMostItems = 1ull << 30;  // threads' worth of work of a launch; more rows go to further launches
+
+// ---- rows of a matrix --------------------------------------------------------------------------------------------------
+// Sixteen lanes per group of 128 columns, eight elements each; two groups of a half-warp under way.
+template <class T>
+__global__ void __launch_bounds__(kRowThreads) k_rows8(const T* src, uint64_t src_ld, bool whole, uint32_t items, Divisor per_row, uint32_t cols, uint8_t* values, uint64_t ld,
+                                                       uint8_t* scales, uint64_t scale_ld) {
+    let_next_start();
+    wait_for_previous();
+    src = from_previous(src);
+    constexpr uint32_t kVecs = 2;
+    // items are a multiple of 16 and steps of 32: the lanes of a half-warp stay together, and the shuffles have whole warps
+    for (uint32_t i0 = blockIdx.x * kRowThreads * kVecs + threadIdx.x; (i0 & ~31u) < items; i0 += gridDim.x * kRowThreads * kVecs) {
+        uint32_t row[kVecs], col[kVecs], valid[kVecs];
+        Raw8<T> x[kVecs];
+#pragma unroll
+        for (uint32_t k = 0; k < kVecs; ++k) {
+            const uint32_t i = i0 + k * kRowThreads;
+            row[k] = per_row.of(i, col[k]);
+            col[k] *= 8;
+            valid[k] = i < items && col[k] < cols ? min(8u, cols - col[k]) : 0;
+            x[k].load(src + row[k] * src_ld + col[k], valid[k], whole);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kVecs; ++k) {
+            float v[8];
+            x[k].widen(v);
+            const uint32_t e = scale_byte(largest_of_16_lanes(largest8(v)));
+            if (valid[k]) {
+                store_values8(values + row[k] * ld + col[k], valid[k], quantize8(v, inverse_scale(e)));
+                if ((threadIdx.x & 15u) == 0) scales[row[k] * scale_ld + col[k] / kScaleGroup] = (uint8_t)e;
+            }
+        }
+    }
 }
-template <class Source, class T>
-void rows_as(const Source& src, const dg_matrix& out, cudaStream_t s) {
-    const uint64_t per_row = (out.cols + 7) / 8, n = out.rows * per_row;
-    launch_after(k_rows<Source, T>, grid_for(n, kRowThreads, 32), kRowThreads, 0, s, src, n, (uint32_t)per_row, (uint32_t)out.cols, (T*)out.data, out.ld,
-                 rows_aligned<T>(out.data, out.ld));
+
+template <class T>
+void rows8(const dg_matrix& m, const dg_rows8& out, cudaStream_t s) {
+    const uint64_t per_row = scale_groups(m.cols) * 16, most = std::max<uint64_t>(1, kMostItems / per_row);
+    for (uint64_t r = 0; r < m.rows; r += most) {
+        const uint32_t items = (uint32_t)(std::min(most, m.rows - r) * per_row);
+        launch_after(k_rows8<T>, grid_for(items, kRowThreads * 2, 32), kRowThreads, 0, s, (const T*)m.data + r * m.ld, m.ld, rows_aligned<T>(m.data, m.ld), items,
+                     Divisor((uint32_t)per_row), (uint32_t)m.cols, out.values + r * out.ld, out.ld, out.scales + r * out.scale_ld, out.scale_ld);
+    }
+}
+
+// ---- patches ---------------------------------------------------------------------------------------------------------------
+// A thread makes sixteen neighbouring features of a patch, eight lanes the 128 of a scale.  A patch's row of pixels is `segment` = patch * C
+// neighbouring bytes, of which features 16 k .. 16 k + 15 are sixteen neighbouring ones where the segment is a multiple of sixteen.
+// Out: uint8_t for 8-bit rows, else the type of the matrix.
+template <int C> struct PatchView {
+    const uint8_t* pixels;
+    uint64_t pitch, image;  // bytes of a row of pixels and of an image
+    uint32_t patch, segment, cols, grid_w;
+    float gain[C], shift[C];
+};
+template <class Out> struct PatchOut {
+    Out* data;
+    uint64_t ld;
+    uint8_t* scales;
+    uint64_t scale_ld;
+    bool whole;
+};
+
+// pixel bytes (four to a word) to values; the first is of channel `phase`.  2^23 + pixel, as a float, has the pixel in its low byte.
+template <int C>
+__device__ __forceinline__ void normalise16(const PatchView<C>& in, const uint32_t w[4], uint32_t phase, float v[16]) {
+    float g[C], b[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        g[c] = in.gain[c];
+        b[c] = in.shift[c];
+#pragma unroll
+        for (int k = 1; k < C; ++k)
+            if (phase == (uint32_t)k) { g[c] = in.gain[(c + k) % C]; b[c] = in.shift[(c + k) % C]; }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = fmaf(__uint_as_float(__byte_perm(w[j >> 2], 0x4B000000u, 0x7650 + (j & 3))) - 8388608.f, g[j % C], b[j % C]);
+}
+
+// Sixteen features of a row from `col` on, `valid` of them; all lanes of a warp are here.
+template <class Out>
+__device__ __forceinline__ void store16(const PatchOut<Out>& out, uint64_t row, uint32_t col, uint32_t valid, float v[16]) {
+    if constexpr (sizeof(Out) == 1) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            if (valid < 16 && (uint32_t)j >= valid) v[j] = 0.f;
+            top = max(top, magnitude(v[j]));
+        }
+#pragma unroll
+        for (int d = 4; d; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+        const uint32_t e = scale_byte(top);
+        const float inverse = inverse_scale(e);
+        if (!valid) return;
+        uint8_t* const p = out.data + row * out.ld + col;
+        uint32_t q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = e4m3x4(v[4 * j] * inverse, v[4 * j + 1] * inverse, v[4 * j + 2] * inverse, v[4 * j + 3] * inverse);
+        if (valid >= 16) *reinterpret_cast<uint4*>(p) = make_uint4(q[0], q[1], q[2], q[3]);
+        else
+#pragma unroll
+            for (uint32_t j = 0; j < 16; ++j)
+                if (j < valid) p[j] = (uint8_t)(q[j >> 2] >> (8 * (j & 3)));
+        if ((threadIdx.x & 7u) == 0) out.scales[row * out.scale_ld + col / kScaleGroup] = (uint8_t)e;
+    } else {
+        Out* const p = out.data + row * out.ld + col;
+        store8(p, valid, out.whole, v);
+        if (valid > 8) store8(p + 8, valid - 8, out.whole, v + 8);
+    }
+}
+
+template <int C, class Out>
+__global__ void __launch_bounds__(kRowThreads) k_patches(const PatchView<C> in, const PatchOut<Out> out, uint32_t items, Divisor per_row, Divisor grid_w, Divisor grid_h, Divisor segment) {
+    let_next_start();
+    wait_for_previous();
+    const uint8_t* const pixels = from_previous(in.pixels);
+    constexpr uint32_t kPieces = 2;  // of a thread under way
+    for (uint32_t i0 = blockIdx.x * kRowThreads * kPieces + threadIdx.x; (i0 & ~31u) < items; i0 += gridDim.x * kRowThreads * kPieces) {
+        uint32_t row[kPieces], col[kPieces], valid[kPieces];
+        uint4 w[kPieces];
+#pragma unroll
+        for (uint32_t k = 0; k < kPieces; ++k) {
+            uint32_t X, Y, b;
+            row[k] = per_row.of(i0 + k * kRowThreads, col[k]);
+            const uint32_t i = grid_h.of(grid_w.of(row[k], X), Y);
+            col[k] *= 16;
+            const uint32_t y = segment.of(col[k], b);
+            valid[k] = i0 + k * kRowThreads < items && col[k] < in.cols ? 16 : 0;
+            w[k] = valid[k] ? *reinterpret_cast<const uint4*>(pixels + i * in.image + ((uint64_t)Y * in.patch + y) * in.pitch + (uint64_t)X * in.segment + b) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kPieces; ++k) {
+            const uint32_t words[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+            float v[16];
+            normalise16<C>(in, words, C == 3 ? col[k] % 3 : 0, v);  // 16 is a multiple of 1, 2 and 4
+            store16(out, row[k], col[k], valid[k], v);
+        }
+    }
+}
+
+// Segments that are no multiple of sixteen bytes, or do not start at one: a CTA brings its patches' rows of pixels (up to `across` patches of a row of
+// patches) into shared memory first, word by word where the bytes begin at words, and gathers the features from there.
+constexpr uint32_t kStripBytes = 40 * 1024;
+
+template <int C, class Out>
+__global__ void __launch_bounds__(kRowThreads) k_patches_staged(const PatchView<C> in, const PatchOut<Out> out, uint32_t across, Divisor strips_x, Divisor grid_h, uint32_t strips,
+                                                                uint32_t strip_pitch) {
+    extern __shared__ __align__(16) uint8_t s_strip[];
+    let_next_start();
+    wait_for_previous();
+    const uint8_t* const pixels = from_previous(in.pixels);
+    for (uint32_t strip = blockIdx.x; strip < strips; strip += gridDim.x) {
+        uint32_t sx, Y;
+        const uint32_t band = strips_x.of(strip, sx), i = grid_h.of(band, Y), x0 = sx * across, count = min(across, in.grid_w - x0), bytes = count * in.segment;
+        const uint8_t* const from = pixels + i * in.image + (uint64_t)Y * in.patch * in.pitch + (uint64_t)x0 * in.segment;
+        __syncthreads();  // the strip before this one has been read
+        for (uint32_t y = threadIdx.x >> 5; y < in.patch; y += kRowThreads / 32) {  // a warp per row of pixels
+            const uint8_t* const p = from + y * in.pitch;
+            const uint32_t lead = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 3u), lane = threadIdx.x & 31u;
+            uint8_t* const to = s_strip + y * strip_pitch + lead;  // words to words
+            const uint32_t head = min(bytes, (4 - lead) & 3u), words = (bytes - head) >> 2;
+            for (uint32_t k = lane; k < words; k += 32) *reinterpret_cast<uint32_t*>(to + head + 4 * k) = *reinterpret_cast<const uint32_t*>(p + head + 4 * k);
+            if (lane < head) to[lane] = p[lane];
+            if (lane < bytes - head - 4 * words) to[head + 4 * words + lane] = p[head + 4 * words + lane];
+        }
+        __syncthreads();
+        const uint32_t per_patch = (in.cols + kScaleGroup - 1) / kScaleGroup * 8, items = count * per_patch;
+        for (uint32_t k = threadIdx.x; (k & ~31u) < items; k += kRowThreads) {
+            const uint32_t x = k / per_patch, col = (k - x * per_patch) * 16, valid = k < items && col < in.cols ? min(16u, in.cols - col) : 0;
+            uint32_t y = col / in.segment, b = col - y * in.segment, w[4] = {};
+            auto line = [&] { return s_strip + y * strip_pitch + (uint32_t)((reinterpret_cast<uintptr_t>(from) + y * in.pitch) & 3u) + x * in.segment; };
+            if (valid) {
+                const uint8_t* q = line();
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) {
+                    if (j < valid) w[j >> 2] |= (uint32_t)q[b] << (8 * (j & 3));
+                    if (++b == in.segment && j + 1 < valid) { b = 0; ++y; q = line(); }
+                }
+            }
+            float v[16];
+            normalise16<C>(in, w, col % C, v);
+            store16(out, (uint64_t)band * in.grid_w + x0 + x, col, valid, v);
+        }
+    }
+}
+
+template <int C, class Out>
+void patches(const PatchJob& j, PatchOut<Out> out, cudaStream_t s) {
+    PatchView<C> in;
+    in.pixels = j.pixels;
+    in.pitch = (uint64_t)j.w * C;
+    in.image = in.pitch * j.h;
+    in.patch = j.patch;
+    in.segment = j.patch * C;
+    in.cols = j.patch * in.segment;
+    in.grid_w = j.w / j.patch;
+    for (int c = 0; c < C; ++c) { in.gain[c] = j.gain[c]; in.shift[c] = j.shift[c]; }
+    const uint32_t grid_h = j.h / j.patch, per_row = (in.cols + kScaleGroup - 1) / kScaleGroup * 8;
+    const uint64_t per_image = (uint64_t)in.grid_w * grid_h;
+    const bool straight = ((reinterpret_cast<uintptr_t>(j.pixels) | in.pitch | in.segment) & 15u) == 0;
+    const uint32_t most = (uint32_t)std::max<uint64_t>(1, kMostItems / (per_image * per_row));  // images of a launch
+    for (uint32_t i = 0; i < j.n; i += most) {
+        const uint32_t n = std::min(most, j.n - i);
+        PatchOut<Out> to = out;
+        in.pixels = j.pixels + i * in.image;
+        to.data += i * per_image * out.ld;
+        if (sizeof(Out) == 1) to.scales += i * per_image * out.scale_ld;
+        if (straight) {
+            const uint32_t items = (uint32_t)(n * per_image * per_row);
+            launch_after(k_patches<C, Out>, grid_for(items, kRowThreads * 2, 32), kRowThreads, 0, s, in, to, items, Divisor(per_row), Divisor(in.grid_w), Divisor(grid_h), Divisor(in.segment));
+        } else {
+            // patches of a strip: what the shared memory holds, but no more than spreads the work over the chip
+            const uint32_t bands = n * grid_h, wanted = (uint32_t)std::max<uint64_t>(1, (uint64_t)bands * in.grid_w / (kSms * 8));
+            const uint32_t across = std::max(1u, std::min({in.grid_w, (kStripBytes / j.patch - 8) / in.segment, std::max(wanted, 8u)}));
+            const uint32_t pitch = (across * in.segment + 3 + 7) / 4 * 4, strips_x = (in.grid_w + across - 1) / across;
+            launch_after(k_patches_staged<C, Out>, grid_for((uint64_t)bands * strips_x, 1, 16), kRowThreads, (size_t)pitch * j.patch, s, in, to, across, Divisor(strips_x), Divisor(grid_h),
+                         bands * strips_x, pitch);
+        }
+    }
 }
 
 template <int C>
 void patch_rows(const PatchJob& j, const dg_rows8* out8, const dg_matrix* out, cudaStream_t s) {
-    PatchSource<C> src;
-    src.pixels = j.pixels;
-    src.grid_w = j.w / j.patch;
-    src.per_image = src.grid_w * (j.h / j.patch);
-    src.patch = j.patch;
-    src.segment = j.patch * C;
-    src.pitch = (uint64_t)j.w * C;
-    src.image = src.pitch * j.h;
-    src.whole = ((reinterpret_cast<uintptr_t>(j.pixels) | src.pitch | src.segment) & 7u) == 0;
-    for (int c = 0; c < C; ++c) { src.gain[c] = j.gain[c]; src.shift[c] = j.shift[c]; }
-    if (out8) rows8(src, *out8, s);
-    else if (out->dtype == DG_F32) rows_as<PatchSource<C>, float>(src, *out, s);
-    else if (out->dtype == DG_BF16) rows_as<PatchSource<C>, bf16>(src, *out, s);
-    else rows_as<PatchSource<C>, __half>(src, *out, s);
+    if (out8) patches<C, uint8_t>(j, {out8->values, out8->ld, out8->scales, out8->scale_ld, true}, s);
+    else if (out->dtype == DG_F32) patches<C, float>(j, {(float*)out->data, out->ld, nullptr, 0, rows_aligned<float>(out->data, out->ld)}, s);
+    else if (out->dtype == DG_BF16) patches<C, bf16>(j, {(bf16*)out->data, out->ld, nullptr, 0, rows_aligned<bf16>(out->data, out->ld)}, s);
+    else patches<C, __half>(j, {(__half*)out->data, out->ld, nullptr, 0, rows_aligned<__half>(out->data, out->ld)}, s);
 }
 
 // ---- scales along the rows of the source, and of 128 x 128 blocks -------------------------------------------------------------
@@ -258,29 +416,6 @@ template <class T> constexpr int kColumnRows = sizeof(T) == 4 ? 8 : 16;  // what
 template <class T> constexpr uint32_t kColumnThreads = 128 / kColumnRows<T> * 32;
 constexpr uint32_t kColumnTile = 256;
 
-template <class T> struct Raw8 {  // eight neighbouring elements as they are in memory
-    uint4 w[sizeof(T) / 2];
-    __device__ __forceinline__ void widen(float v[8]) const {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = *reinterpret_cast<const float4*>(&w[0]), b = *reinterpret_cast<const float4*>(&w[1]);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            unpack8(w[0], v, T());
-        }
-    }
-    __device__ __forceinline__ void load(const T* p, uint32_t valid, bool whole) {
-        if (whole && valid >= 8) {
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
-        } else {
-            T e[8];
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) e[j] = j < valid ? p[j] : narrow<T>(0.f);
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(e)[i];
-        }
-    }
-};
 // Magnitudes of two 16-bit elements compared at once: like those of 32 bits, they order as whole numbers.
 __device__ __forceinline__ uint32_t larger(uint32_t top, uint32_t v, bf16) { return __vmaxu2(top, v & 0x7FFF7FFFu); }
 __device__ __forceinline__ uint32_t larger(uint32_t top, uint32_t v, __half) { return __vmaxu2(top, v & 0x7FFF7FFFu); }
@@ -363,7 +498,7 @@ template <class T>
 void quantize_rows(const dg_matrix& m, const dg_rows8& out, cudaStream_t s) {
     const bool whole = rows_aligned<T>(m.data, m.ld);
     if (!out.by_column && out.block == 1) {
-        rows8(MatrixSource<T>{(const T*)m.data, m.ld, whole}, out, s);
+        rows8<T>(m, out, s);
         return;
     }
     const uint32_t tiles_x = (uint32_t)((m.cols + kColumnTile - 1) / kColumnTile);
@@ -395,66 +530,104 @@ __device__ __forceinline__ float row_sum(float v, float* s_part) {
     return v;
 }
 
-template <class T, int V, int TPR, int THREADS>
-__global__ void __launch_bounds__(THREADS) k_rms_norm(const NormJob a, bool x_whole, bool r_whole, bool w_whole, bool s_whole, bool y_whole) {
+// WHOLE: every row of every matrix starts at a multiple of 16 bytes and holds whole vectors.  The weight waits in shared memory as floats.
+template <class T, int V, int TPR, int THREADS, bool WHOLE>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) k_rms_norm(const NormJob a, bool x_whole, bool r_whole, bool s_whole, bool y_whole) {
+    extern __shared__ __align__(16) float s_weight[];
     __shared__ float s_part[THREADS / 32];
     let_next_start();
     wait_for_previous();
     const T *const px = from_previous(reinterpret_cast<const T*>(a.x)), *const pr = from_previous(reinterpret_cast<const T*>(a.residual));
-    const void* const pw = from_previous(a.weight);
+    if (a.weight) {
+        const void* const pw = from_previous(a.weight);
+        for (uint32_t c = threadIdx.x; c < a.cols; c += THREADS)
+            s_weight[c] = a.weight_dtype == DG_F32 ? reinterpret_cast<const float*>(pw)[c] : a.weight_dtype == DG_BF16 ? widen(reinterpret_cast<const bf16*>(pw)[c]) : widen(reinterpret_cast<const __half*>(pw)[c]);
+        __syncthreads();
+    }
     constexpr uint32_t kRows = THREADS / TPR;
     const uint32_t t = threadIdx.x % TPR, mine = threadIdx.x / TPR;
     const float per_col = 1.f / (float)a.cols;
-    for (uint64_t r0 = (uint64_t)blockIdx.x * kRows; r0 < a.rows; r0 += (uint64_t)gridDim.x * kRows) {
-        const uint64_t row = r0 + mine;
+    // valid elements of vector k of a row
+    auto valid_at = [&](int k) {
+        const uint32_t col = (k * TPR + t) * 8;
+        return col >= a.cols ? 0u : WHOLE ? 8u : min(8u, a.cols - col);
+    };
+    const uint64_t stride = (uint64_t)gridDim.x * kRows;
+    uint64_t row = (uint64_t)blockIdx.x * kRows + mine, rr = pr ? row % a.residual_rows : 0;
+    const uint64_t rr_step = pr ? stride % a.residual_rows : 0;
+    // the next row is under way while this one is worked on
+    Raw8<T> x[V], r[V];
+    auto fetch = [&](uint64_t at, uint64_t residual_row) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const T* const p = px + at * a.x_ld + (k * TPR + t) * 8;
+            if constexpr (WHOLE) x[k].load_whole(p, at < a.rows && valid_at(k));
+            else x[k].load(p, at < a.rows ? valid_at(k) : 0, x_whole);
+        }
+        if (!pr) return;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const T* const p = pr + residual_row * a.residual_ld + (k * TPR + t) * 8;
+            if constexpr (WHOLE) r[k].load_whole(p, at < a.rows && valid_at(k));
+            else r[k].load(p, at < a.rows ? valid_at(k) : 0, r_whole);
+        }
+    };
+    fetch(row, rr);
+    for (uint64_t r0 = (uint64_t)blockIdx.x * kRows; r0 < a.rows; r0 += stride, row += stride) {
         const bool live = row < a.rows;
         float h[V][8];
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const uint32_t col = (k * TPR + t) * 8, valid = live && col < a.cols ? min(8u, a.cols - col) : 0;
+            x[k].widen(h[k]);
+            if (pr) {
+                float v[8];
+                r[k].widen(v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[k][j] = 0.f;
-            if (valid) load8(px + row * a.x_ld + col, valid, x_whole, h[k]);
-        }
-        if (pr) {
-            const uint64_t rr = row % a.residual_rows;
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const uint32_t col = (k * TPR + t) * 8, valid = live && col < a.cols ? min(8u, a.cols - col) : 0;
-                if (valid) {
-                    float r[8];
-                    load8(pr + rr * a.residual_ld + col, valid, r_whole, r);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) h[k][j] += r[j];
-                }
+                for (int j = 0; j < 8; ++j) h[k][j] += v[j];
             }
         }
+        rr += rr_step;
+        if (rr >= a.residual_rows) rr -= a.residual_rows;
+        fetch(row + stride, rr);
 #pragma unroll
         for (int k = 0; k < V; ++k)
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum = fmaf(h[k][j], h[k][j], sum);
         const float rstd = 1.f / sqrtf(row_sum<TPR>(sum, s_part) * per_col + a.eps);
         if (live && t == 0 && a.rstd) a.rstd[row] = rstd;
+        if (a.sum) {
+            T* const to = reinterpret_cast<T*>(a.sum) + row * a.sum_ld;
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (live && valid_at(k)) store8(to + (k * TPR + t) * 8, valid_at(k), WHOLE || s_whole, h[k]);
+        }
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            const uint32_t col = (k * TPR + t) * 8, valid = live && col < a.cols ? min(8u, a.cols - col) : 0;
-            if (a.sum && valid) store8(reinterpret_cast<T*>(a.sum) + row * a.sum_ld + col, valid, s_whole, h[k]);
-            float w[8];
-            if (pw && valid) {
-                load8_any(pw, col, a.weight_dtype, valid, w_whole, w);
+            if (a.weight) {
+                float w[8];
+                if (valid_at(k)) load8((const float*)s_weight + (k * TPR + t) * 8, valid_at(k), true, w);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[k][j] = h[k][j] * rstd * w[j];
+                for (int j = 0; j < 8; ++j) h[k][j] = valid_at(k) > (uint32_t)j ? h[k][j] * rstd * w[j] : 0.f;
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) h[k][j] *= rstd;
             }
-            if (a.y && valid) store8(reinterpret_cast<T*>(a.y) + row * a.y_ld + col, valid, y_whole, h[k]);
-            if (a.y8.values) {
+        }
+        if (a.y) {
+            T* const to = reinterpret_cast<T*>(a.y) + row * a.y_ld;
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (live && valid_at(k)) store8(to + (k * TPR + t) * 8, valid_at(k), WHOLE || y_whole, h[k]);
+        }
+        if (a.y8.values) {
+            uint8_t *const to = a.y8.values + row * a.y8.ld, *const scales = a.y8.scales + row * a.y8.scale_ld;
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
                 const uint32_t e = scale_byte(largest_of_16_lanes(largest8(h[k])));
-                if (valid) {
-                    store_values8(a.y8.values + row * a.y8.ld + col, valid, quantize8(h[k], inverse_scale(e)));
-                    if ((t & 15u) == 0) a.y8.scales[row * a.y8.scale_ld + col / kScaleGroup] = (uint8_t)e;
+                if (live && valid_at(k)) {
+                    store_values8(to + (k * TPR + t) * 8, valid_at(k), quantize8(h[k], inverse_scale(e)));
+                    if ((t & 15u) == 0) scales[(k * TPR + t) / 16] = (uint8_t)e;
                 }
             }
         }
@@ -463,133 +636,212 @@ __global__ void __launch_bounds__(THREADS) k_rms_norm(const NormJob a, bool x_wh
 
 template <class T>
 void rms_norm(const NormJob& j, cudaStream_t s) {
+    const bool x_whole = rows_aligned<T>(j.x, j.x_ld), r_whole = rows_aligned<T>(j.residual, j.residual_ld), s_whole = rows_aligned<T>(j.sum, j.sum_ld),
+               y_whole = rows_aligned<T>(j.y, j.y_ld), whole = x_whole && r_whole && s_whole && y_whole && j.cols % 8 == 0;
     auto go = [&](auto kernel, uint32_t threads, uint32_t rows_per_cta) {
-        launch_after(kernel, grid_for(j.rows, rows_per_cta, 2048 / threads * 4), threads, 0, s, j, rows_aligned<T>(j.x, j.x_ld), rows_aligned<T>(j.residual, j.residual_ld),
-                     (reinterpret_cast<uintptr_t>(j.weight) & 15u) == 0, rows_aligned<T>(j.sum, j.sum_ld), rows_aligned<T>(j.y, j.y_ld));
+        const size_t smem = j.weight ? (j.cols + 7) / 8 * 32 : 0;
+        if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kNormMaxCols * 4));
+        launch_after(kernel, grid_for(j.rows, rows_per_cta, 1024 / threads), threads, smem, s, j, x_whole, r_whole, s_whole, y_whole);
     };
+#define DG_NORM(V, TPR, THREADS) (whole ? go(k_rms_norm<T, V, TPR, THREADS, true>, THREADS, THREADS / TPR) : go(k_rms_norm<T, V, TPR, THREADS, false>, THREADS, THREADS / TPR))
     const uint32_t vecs = (j.cols + 7) / 8;
-    if (vecs <= 32) go(k_rms_norm<T, 1, 32, 256>, 256, 8);
-    else if (vecs <= 64) go(k_rms_norm<T, 2, 32, 256>, 256, 8);
-    else if (vecs <= 96) go(k_rms_norm<T, 3, 32, 256>, 256, 8);
-    else if (vecs <= 128) go(k_rms_norm<T, 4, 32, 256>, 256, 8);
-    else if (vecs <= 160) go(k_rms_norm<T, 5, 32, 256>, 256, 8);
-    else if (vecs <= 192) go(k_rms_norm<T, 6, 32, 256>, 256, 8);
-    else if (vecs <= 256) go(k_rms_norm<T, 8, 32, 256>, 256, 8);
-    else if (vecs <= 512) go(k_rms_norm<T, 2, 256, 256>, 256, 1);
-    else if (vecs <= 1024) go(k_rms_norm<T, 4, 256, 256>, 256, 1);
-    else go(k_rms_norm<T, 4, 512, 512>, 512, 1);
+    if (vecs <= 32) DG_NORM(1, 32, 256);
+    else if (vecs <= 64) DG_NORM(2, 32, 256);
+    else if constexpr (sizeof(T) == 4) {  // half as many elements to a thread
+        if (vecs <= 128) DG_NORM(2, 64, 256);
+        else if (vecs <= 256) DG_NORM(2, 128, 256);
+        else if (vecs <= 512) DG_NORM(2, 256, 256);
+        else if (vecs <= 1024) DG_NORM(2, 512, 512);
+        else DG_NORM(4, 512, 512);
+    } else {
+        if (vecs <= 96) DG_NORM(3, 32, 256);
+        else if (vecs <= 128) DG_NORM(4, 32, 256);
+        else if (vecs <= 160) DG_NORM(5, 32, 256);
+        else if (vecs <= 256) DG_NORM(4, 64, 256);
+        else if (vecs <= 512) DG_NORM(4, 128, 256);
+        else if (vecs <= 1024) DG_NORM(4, 256, 256);
+        else DG_NORM(4, 512, 512);
+    }
+#undef DG_NORM
 }
 
-// Backward.  A unit is a residual row t and a part of the rows r with r % period == t; TPR threads take a unit's rows one after the other
-// and keep the sums of dx (for dresidual) of the unit and of dy * hat (for dweight) of all their units in registers.  CTAs write their
-// dweight sums to the workspace; so do units their dresidual sums where a residual row has more than one unit.
-template <class T, int V, int TPR, int THREADS>
-__global__ void __launch_bounds__(THREADS) k_rms_norm_backward(const NormBackwardJob a, uint32_t parts, float* w_parts, float* r_parts, bool y_whole,
-                                                               bool h_whole, bool w_whole, bool s_whole, bool x_whole) {
-    constexpr uint32_t kRows = THREADS / TPR;
-    __shared__ float s_part[THREADS / 32];
-    __shared__ float s_sum[kRows > 1 ? V * TPR * 8 : 1];
+// Backward.  A worker (a.split.row_threads threads, whole warps) takes units one after the other, and a unit's rows R at a time, so that the loads of R
+// rows are under way at once and the R sums along them cross the worker's warps together.  A thread owns V vectors of eight columns of every row; it
+// keeps the elements as they were loaded and widens them twice, before and after those sums.
+//   Where a residual row has several images, a unit is a residual row t and a part of the rows r with r % period == t: their dx is added up in
+//   registers, for dresidual.  Elsewhere a unit is kNormChunk neighbouring rows, and a row of dx is a row of dresidual.
+// A worker adds dy * hat of all its rows up in registers, for dweight.  The sums of workers, and of units that share a residual row, go to the
+// workspace and are added up in their order.
+template <int R>
+__device__ __forceinline__ void sums_across(float v[R], uint32_t row_warps, uint32_t worker_warp, uint32_t barrier, uint32_t threads, float (*s_part)[R]) {
+    const uint32_t lane = threadIdx.x & 31u;
+    // halves of the warp take over half of the sums each, then quarters: lane l is left with sum l / (32 / R)
+    float mine;
+    if constexpr (R == 4) {
+        const bool up = lane & 16u;
+        const float a = (up ? v[2] : v[0]) + __shfl_xor_sync(0xFFFFFFFFu, up ? v[0] : v[2], 16), b = (up ? v[3] : v[1]) + __shfl_xor_sync(0xFFFFFFFFu, up ? v[1] : v[3], 16);
+        const bool odd = lane & 8u;
+        mine = (odd ? b : a) + __shfl_xor_sync(0xFFFFFFFFu, odd ? a : b, 8);
+    } else if constexpr (R == 2) {
+        const bool up = lane & 16u;
+        mine = (up ? v[1] : v[0]) + __shfl_xor_sync(0xFFFFFFFFu, up ? v[0] : v[1], 16);
+        mine += __shfl_xor_sync(0xFFFFFFFFu, mine, 8);
+    } else {
+        mine = v[0] + __shfl_xor_sync(0xFFFFFFFFu, v[0], 16);
+        mine += __shfl_xor_sync(0xFFFFFFFFu, mine, 8);
+    }
+#pragma unroll
+    for (int d = 4; d; d >>= 1) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, d);
+    if (row_warps == 1) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) v[r] = __shfl_sync(0xFFFFFFFFu, mine, r * (32 / R));
+        return;
+    }
+    if ((lane & (32 / R - 1)) == 0) s_part[threadIdx.x >> 5][lane / (32 / R)] = mine;
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
+    const uint32_t first = (threadIdx.x >> 5) - worker_warp;
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] = 0.f;
+    for (uint32_t w = 0; w < row_warps; ++w)
+#pragma unroll
+        for (int r = 0; r < R; ++r) v[r] += s_part[first + w][r];
+}
+
+template <class T, int V, int R, int MOST, bool WHOLE>
+__global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) k_rms_norm_backward(const NormBackwardJob a, float* w_parts, float* r_parts, bool y_whole, bool h_whole, bool w_whole,
+                                                                         bool s_whole, bool x_whole) {
+    __shared__ __align__(16) float s_part[2][MOST / 32][R];
     let_next_start();
     wait_for_previous();
     const T *const py = from_previous(reinterpret_cast<const T*>(a.dy)), *const ph = from_previous(reinterpret_cast<const T*>(a.h)),
             *const ps = from_previous(reinterpret_cast<const T*>(a.dsum));
-    const void* const pw = from_previous(a.weight);
     const float* const prstd = from_previous(a.rstd);
-    const uint32_t t = threadIdx.x % TPR, mine = threadIdx.x / TPR;
-    const uint64_t units = a.period * parts, images = a.rows / a.period;
+    const uint32_t row_threads = a.split.row_threads, parts = a.split.parts, worker = threadIdx.x / row_threads, t = threadIdx.x - worker * row_threads;
+    const uint32_t workers = gridDim.x * a.split.cta_workers, me = blockIdx.x * a.split.cta_workers + worker;
+    const bool by_image = a.split.by_image;
+    const uint64_t images = by_image ? a.rows / a.period : 0;
+    const uint64_t units = by_image ? a.period * parts : (a.rows + kNormChunk - 1) / kNormChunk;
     const float per_col = 1.f / (float)a.cols;
-    float dw[V][8] = {};
-    for (uint64_t u0 = (uint64_t)blockIdx.x * kRows; u0 < units; u0 += (uint64_t)gridDim.x * kRows) {
-        const uint64_t unit = u0 + mine, part = unit / a.period, at = unit - part * a.period;
-        const bool there = unit < units;
-        const uint64_t first = images * part / parts, last = there ? images * (part + 1) / parts : first;
+    uint32_t cols[V], valid[V];
+    float w[V][8], dw[V][8];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        cols[k] = (k * row_threads + t) * 8;
+        valid[k] = cols[k] >= a.cols ? 0u : WHOLE ? 8u : min(8u, a.cols - cols[k]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { w[k][j] = 1.f; dw[k][j] = 0.f; }
+        if (a.weight && valid[k]) load8_any(from_previous(a.weight), cols[k], a.weight_dtype, valid[k], w_whole, w[k]);
+    }
+    uint32_t turn = 0;
+    for (uint64_t unit = me; unit < units; unit += workers) {
+        uint64_t row0, stride, count;
+        if (by_image) {
+            const uint64_t part = unit / a.period, first = images * part / parts;
+            row0 = first * a.period + (unit - part * a.period);
+            stride = a.period;
+            count = images * (part + 1) / parts - first;
+        } else {
+            row0 = unit * kNormChunk;
+            stride = 1;
+            count = min((uint64_t)kNormChunk, a.rows - row0);
+        }
         float dr[V][8] = {};
-        // all threads of the CTA go through the same number of rows (they may meet in row_sum)
-        const uint64_t most = (images + parts - 1) / parts;
-        for (uint64_t i = 0; i < most; ++i) {
-            const bool live = first + i < last;
-            const uint64_t row = (first + i) * a.period + at;
-            const float rstd = live ? prstd[row] : 0.f;
-            float g[V][8], hat[V][8];
-            float along = 0.f;
+        Raw8<T> dy[R][V], h[R][V];
+        float rstd[R];
+        auto fetch = [&](uint64_t i) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const uint32_t col = (k * TPR + t) * 8, valid = live && col < a.cols ? min(8u, a.cols - col) : 0;
+            for (int r = 0; r < R; ++r) {
+                const bool live = i + r < count;
+                const uint64_t row = row0 + (i + r) * stride;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g[k][j] = hat[k][j] = 0.f;
-                if (valid) {
-                    load8(py + row * a.dy_ld + col, valid, y_whole, g[k]);
-                    load8(ph + row * a.h_ld + col, valid, h_whole, hat[k]);
+                for (int k = 0; k < V; ++k) {
+                    if constexpr (WHOLE) {
+                        dy[r][k].load_whole(py + row * a.dy_ld + cols[k], live && valid[k]);
+                        h[r][k].load_whole(ph + row * a.h_ld + cols[k], live && valid[k]);
+                    } else {
+                        dy[r][k].load(py + row * a.dy_ld + cols[k], live ? valid[k] : 0, y_whole);
+                        h[r][k].load(ph + row * a.h_ld + cols[k], live ? valid[k] : 0, h_whole);
+                    }
+                }
+                rstd[r] = live ? prstd[row] : 0.f;
+            }
+        };
+        fetch(0);
+        for (uint64_t i = 0; i < count; i += R, turn ^= 1u) {
+            Raw8<T> dy_now[R][V], h_now[R][V];
+            float rstd_now[R], along[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                rstd_now[r] = rstd[r];
+#pragma unroll
+                for (int k = 0; k < V; ++k) { dy_now[r][k] = dy[r][k]; h_now[r][k] = h[r][k]; }
+            }
+            if (i + R < count) fetch(i + R);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                along[r] = 0.f;
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    float g[8], hat[8];
+                    dy_now[r][k].widen(g);
+                    h_now[r][k].widen(hat);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        hat[j] *= rstd_now[r];
+                        dw[k][j] = fmaf(g[j], hat[j], dw[k][j]);
+                        along[r] = fmaf(g[j] * w[k][j], hat[j], along[r]);
+                    }
                 }
             }
+            sums_across<R>(along, row_threads / 32, t >> 5, worker + 1, row_threads, s_part[turn]);
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const uint32_t col = (k * TPR + t) * 8, valid = live && col < a.cols ? min(8u, a.cols - col) : 0;
-                float w[8];
-                if (pw && valid) load8_any(pw, col, a.weight_dtype, valid, w_whole, w);
+            for (int r = 0; r < R; ++r) {
+                if (i + r >= count) break;
+                const uint64_t row = row0 + (i + r) * stride;
+                const float mean = along[r] * per_col;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    hat[k][j] *= rstd;
-                    dw[k][j] = fmaf(g[k][j], hat[k][j], dw[k][j]);
-                    if (pw && valid) g[k][j] *= w[j];
-                    along = fmaf(g[k][j], hat[k][j], along);
+                for (int k = 0; k < V; ++k) {
+                    if (!valid[k]) continue;
+                    float d[8], hat[8];
+                    dy_now[r][k].widen(d);
+                    h_now[r][k].widen(hat);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) d[j] = rstd_now[r] * (d[j] * w[k][j] - hat[j] * rstd_now[r] * mean);
+                    if (ps) {
+                        float extra[8];
+                        load8(ps + row * a.dsum_ld + cols[k], valid[k], WHOLE || s_whole, extra);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) d[j] += extra[j];
+                    }
+                    if (a.dx) store8(reinterpret_cast<T*>(a.dx) + row * a.dx_ld + cols[k], valid[k], WHOLE || x_whole, d);
+                    if (by_image) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) dr[k][j] += d[j];
+                    } else if (a.dresidual) {
+                        store8(a.dresidual + row * a.cols + cols[k], valid[k], WHOLE && (reinterpret_cast<uintptr_t>(a.dresidual) & 15u) == 0, d);
+                    }
                 }
-            }
-            along = row_sum<TPR>(along, s_part) * per_col;
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const uint32_t col = (k * TPR + t) * 8, valid = live && col < a.cols ? min(8u, a.cols - col) : 0;
-                float d[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) d[j] = rstd * (g[k][j] - hat[k][j] * along);
-                if (ps && valid) {
-                    float extra[8];
-                    load8(ps + row * a.dsum_ld + col, valid, s_whole, extra);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) d[j] += extra[j];
-                }
-                if (a.dx && valid) store8(reinterpret_cast<T*>(a.dx) + row * a.dx_ld + col, valid, x_whole, d);
-                if (valid)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) dr[k][j] += d[j];
             }
         }
-        if (a.dresidual && there) {
-            float* const to = (parts > 1 ? r_parts + part * a.period * a.cols : a.dresidual) + at * a.cols;
+        if (by_image) {
+            float* const to = parts > 1 ? r_parts + unit * a.cols : a.dresidual + unit * a.cols;
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const uint32_t col = (k * TPR + t) * 8, valid = col < a.cols ? min(8u, a.cols - col) : 0;
-                if (valid) store8(to + col, valid, (a.cols & 3u) == 0 && (reinterpret_cast<uintptr_t>(to) & 15u) == 0, dr[k]);
-            }
+            for (int k = 0; k < V; ++k)
+                if (valid[k]) store8(to + cols[k], valid[k], WHOLE && (reinterpret_cast<uintptr_t>(to) & 15u) == 0, dr[k]);
         }
     }
     if (!a.dweight) return;
-    float* const to = w_parts + (uint64_t)blockIdx.x * a.cols;
-    if constexpr (kRows > 1) {  // the CTA's rows in their order
-        for (uint32_t r = 0; r < kRows; ++r) {
-            if (mine == r)
+    float* const to = w_parts + (uint64_t)me * a.cols;
 #pragma unroll
-                for (int k = 0; k < V; ++k)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        float& sum = s_sum[(k * TPR + t) * 8 + j];
-                        sum = r ? sum + dw[k][j] : dw[k][j];
-                    }
-            __syncthreads();
-        }
-        for (uint32_t c = threadIdx.x; c < a.cols; c += THREADS) to[c] = s_sum[c];
-    } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const uint32_t col = (k * TPR + t) * 8, valid = col < a.cols ? min(8u, a.cols - col) : 0;
-            if (valid) store8(to + col, valid, false, dw[k]);
-        }
-    }
+    for (int k = 0; k < V; ++k)
+        if (valid[k]) store8(to + cols[k], valid[k], WHOLE, dw[k]);  // the workspace is aligned, and so are its rows if they are whole vectors
 }
 
-// out[i] = the sum of parts[p][i] in a fixed order: eight threads a column, each every eighth part
-__global__ void __launch_bounds__(256) k_sum_parts(const float* parts, uint32_t count, uint64_t n, float* out) {
-    __shared__ float s_sum[8][33];
+// out[i] = the sum of parts[p][i] in a fixed order: sixteen threads a column, each every sixteenth part
+constexpr uint32_t kSumThreads = 512;
+__global__ void __launch_bounds__(kSumThreads) k_sum_parts(const float* parts, uint32_t count, uint64_t n, float* out) {
+    constexpr uint32_t kLanes = kSumThreads / 32;
+    __shared__ float s_sum[kLanes][33];
     let_next_start();
     wait_for_previous();
     parts = from_previous(parts);
@@ -597,13 +849,19 @@ __global__ void __launch_bounds__(256) k_sum_parts(const float* parts, uint32_t 
     for (uint64_t i0 = (uint64_t)blockIdx.x * 32; i0 < n; i0 += (uint64_t)gridDim.x * 32) {
         const uint64_t i = i0 + lane;
         float sum = 0.f;
-        if (i < n)
-            for (uint32_t p = part; p < count; p += 8) sum += parts[p * n + i];
+        if (i < n) {
+            uint32_t p = part;
+            for (; p + 3 * kLanes < count; p += 4 * kLanes) {
+                const float a = parts[p * n + i], b = parts[(p + kLanes) * n + i], c = parts[(p + 2 * kLanes) * n + i], d = parts[(p + 3 * kLanes) * n + i];
+                sum += (a + b) + (c + d);
+            }
+            for (; p < count; p += kLanes) sum += parts[p * n + i];
+        }
         s_sum[part][lane] = sum;
         __syncthreads();
         if (part == 0 && i < n) {
 #pragma unroll
-            for (int p = 1; p < 8; ++p) sum += s_sum[p][lane];
+            for (uint32_t p = 1; p < kLanes; ++p) sum += s_sum[p][lane];
             out[i] = sum;
         }
         __syncthreads();
@@ -616,27 +874,28 @@ __global__ void k_zero(float* out, uint64_t n) {
 
 template <class T>
 void rms_norm_backward(const NormBackwardJob& j, float* workspace, cudaStream_t s) {
-    const NormBackwardSplit d = norm_backward_split(j.rows, j.cols, j.period, j.dresidual != nullptr);
-    float* const r_parts = workspace + (uint64_t)d.ctas * j.cols;
-    auto go = [&](auto kernel, uint32_t threads) {
-        launch_after(kernel, d.ctas, threads, 0, s, j, d.parts, workspace, r_parts, rows_aligned<T>(j.dy, j.dy_ld), rows_aligned<T>(j.h, j.h_ld),
-                     (reinterpret_cast<uintptr_t>(j.weight) & 15u) == 0, rows_aligned<T>(j.dsum, j.dsum_ld), rows_aligned<T>(j.dx, j.dx_ld));
+    const NormBackwardSplit& d = j.split;
+    const uint64_t workers = (uint64_t)d.ctas * d.cta_workers;
+    float* const r_parts = workspace + workers * j.cols;
+    const bool y_whole = rows_aligned<T>(j.dy, j.dy_ld), h_whole = rows_aligned<T>(j.h, j.h_ld), s_whole = rows_aligned<T>(j.dsum, j.dsum_ld),
+               x_whole = rows_aligned<T>(j.dx, j.dx_ld), whole = y_whole && h_whole && s_whole && x_whole && j.cols % 8 == 0;
+    auto go = [&](auto kernel) {
+        launch_after(kernel, d.ctas, d.row_threads * d.cta_workers, 0, s, j, workspace, r_parts, y_whole, h_whole, (reinterpret_cast<uintptr_t>(j.weight) & 15u) == 0, s_whole,
+                     x_whole);
     };
-    const uint32_t vecs = (j.cols + 7) / 8;
-    if (vecs <= 32) go(k_rms_norm_backward<T, 1, 32, 256>, 256);
-    else if (vecs <= 64) go(k_rms_norm_backward<T, 2, 32, 256>, 256);
-    else if (vecs <= 96) go(k_rms_norm_backward<T, 3, 32, 256>, 256);
-    else if (vecs <= 128) go(k_rms_norm_backward<T, 4, 32, 256>, 256);
-    else if (vecs <= 160) go(k_rms_norm_backward<T, 5, 32, 256>, 256);
-    else if (vecs <= 256) go(k_rms_norm_backward<T, 2, 128, 256>, 256);
-    else if (vecs <= 512) go(k_rms_norm_backward<T, 4, 128, 256>, 256);
-    else if (vecs <= 1024) go(k_rms_norm_backward<T, 2, 512, 512>, 512);
-    else go(k_rms_norm_backward<T, 4, 512, 512>, 512);
+    // Rows at a time, and as many under way: what 128 registers hold.  Four at a time with none under way took 102 us (24 images of 2294 x 1152,
+    // bf16), two with 85 registers 118 and more CTAs, two with the next two under way 97.
+    constexpr int kRows = sizeof(T) == 4 ? 1 : 2;
+    const uint64_t vecs = (j.cols + 7) / 8;
+    if (vecs <= 256) whole ? go(k_rms_norm_backward<T, 1, kRows, 256, true>) : go(k_rms_norm_backward<T, 1, kRows, 256, false>);
+    else if (vecs <= 512) whole ? go(k_rms_norm_backward<T, 1, kRows, 512, true>) : go(k_rms_norm_backward<T, 1, kRows, 512, false>);
+    else if (vecs <= 1024) whole ? go(k_rms_norm_backward<T, 2, 1, 512, true>) : go(k_rms_norm_backward<T, 2, 1, 512, false>);
+    else whole ? go(k_rms_norm_backward<T, 2, 1, 1024, true>) : go(k_rms_norm_backward<T, 2, 1, 1024, false>);
     auto add_up = [&](const float* parts, uint32_t count, uint64_t n, float* out) {
-        launch_after(k_sum_parts, grid_for(n, 32, 8), 256, 0, s, parts, count, n, out);
+        launch_after(k_sum_parts, grid_for(n, 32, 4), kSumThreads, 0, s, parts, count, n, out);
     };
-    if (j.dweight) add_up(workspace, d.ctas, j.cols, j.dweight);
-    if (j.dresidual && d.parts > 1) add_up(r_parts, d.parts, j.period * j.cols, j.dresidual);
+    if (j.dweight) add_up(workspace, (uint32_t)workers, j.cols, j.dweight);
+    if (d.by_image && d.parts > 1) add_up(r_parts, d.parts, j.period * j.cols, j.dresidual);
 }
 
 // ---- dropout -------------------------------------------------------------------------------------------------------------------
@@ -674,43 +933,69 @@ __device__ __forceinline__ void bits_of_8(uint64_t index, uint64_t seed, uint32_
     }
 }
 
-template <class T>
+// One row: the matrix without gaps, as long as need be.  EIGHTS: every vector of eight begins with an index that is a multiple of eight.
+constexpr int kDropoutVecs = 2;  // of a thread under way at once
+
+template <class T, bool ONE_ROW, bool EIGHTS, bool PER_ROW>
 __global__ void __launch_bounds__(kRowThreads) k_dropout(const DropoutJob a, uint64_t nvec, uint64_t per_row, float scale, bool x_whole, bool y_whole) {
     let_next_start();
     wait_for_previous();
     const T* const x = from_previous(reinterpret_cast<const T*>(a.x));
     T* const y = reinterpret_cast<T*>(a.y);
-    for (uint64_t i = (uint64_t)blockIdx.x * kRowThreads + threadIdx.x; i < nvec; i += (uint64_t)gridDim.x * kRowThreads) {
-        const uint64_t row = i / per_row, col = (i - row * per_row) * 8;
-        const uint32_t valid = (uint32_t)min((uint64_t)8, a.cols - col);
-        float v[8];
-        load8(x + row * a.x_ld + col, valid, x_whole, v);
-        uint32_t bits[4];
-        if (a.per_row) {
-            bits_of_8(a.offset + row, a.seed, bits);
-            bits[0] = bits[1] = bits[2] = bits[3] = (bits[0] & 0xFFFFu) * 0x10001u;
-        } else {
-            bits_of_8(a.offset + row * a.cols + col, a.seed, bits);
+    const uint64_t step = (uint64_t)gridDim.x * kRowThreads * kDropoutVecs;
+    for (uint64_t i0 = (uint64_t)blockIdx.x * kRowThreads * kDropoutVecs + threadIdx.x; i0 < nvec; i0 += step) {
+        uint64_t row[kDropoutVecs], col[kDropoutVecs];
+        uint32_t valid[kDropoutVecs];
+        Raw8<T> raw[kDropoutVecs];
+#pragma unroll
+        for (int k = 0; k < kDropoutVecs; ++k) {
+            const uint64_t i = i0 + k * kRowThreads;
+            row[k] = ONE_ROW ? 0 : i / per_row;
+            col[k] = (i - row[k] * per_row) * 8;
+            valid[k] = i < nvec ? (uint32_t)min((uint64_t)8, a.cols - col[k]) : 0;
+            raw[k].load(x + row[k] * a.x_ld + col[k], valid[k], x_whole);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t b = j & 1 ? bits[j >> 1] >> 16 : bits[j >> 1] & 0xFFFFu;
-            v[j] = b >= a.threshold ? v[j] * scale : 0.f;
+        for (int k = 0; k < kDropoutVecs; ++k) {
+            if (!valid[k]) continue;
+            const uint64_t index = a.offset + (PER_ROW ? row[k] : row[k] * a.cols + col[k]);
+            uint32_t bits[4];
+            if constexpr (EIGHTS) {
+                const uint4 b = philox(index >> 3, a.seed);
+                bits[0] = b.x; bits[1] = b.y; bits[2] = b.z; bits[3] = b.w;
+            } else {
+                bits_of_8(index, a.seed, bits);
+            }
+            float v[8];
+            raw[k].widen(v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t b = PER_ROW ? bits[0] & 0xFFFFu : j & 1 ? bits[j >> 1] >> 16 : bits[j >> 1] & 0xFFFFu;
+                v[j] = b >= a.threshold ? v[j] * scale : 0.f;
+            }
+            store8(y + row[k] * a.y_ld + col[k], valid[k], y_whole, v);
         }
-        store8(y + row * a.y_ld + col, valid, y_whole, v);
     }
 }
 
 template <class T>
 void dropout(DropoutJob j, cudaStream_t s) {
-    if (!j.per_row && (j.rows == 1 || (j.x_ld == j.cols && j.y_ld == j.cols))) {  // one long row
+    const bool one_row = !j.per_row && (j.rows == 1 || (j.x_ld == j.cols && j.y_ld == j.cols));
+    if (one_row) {
         j.cols *= j.rows;
         j.x_ld = j.y_ld = (j.cols + 7) / 8 * 8;
         j.rows = 1;
     }
     const uint64_t per_row = (j.cols + 7) / 8, n = j.rows * per_row;
-    launch_after(k_dropout<T>, grid_for(n, kRowThreads, 32), kRowThreads, 0, s, j, n, per_row, 65536.f / (float)(65536u - j.threshold),
-                 rows_aligned<T>(j.x, j.x_ld), rows_aligned<T>(j.y, j.y_ld));
+    auto go = [&](auto kernel) {
+        launch_after(kernel, grid_for(n, kRowThreads * kDropoutVecs, 32), kRowThreads, 0, s, j, n, per_row, 65536.f / (float)(65536u - j.threshold),
+                     rows_aligned<T>(j.x, j.x_ld), rows_aligned<T>(j.y, j.y_ld));
+    };
+    const bool eights = j.offset % 8 == 0 && (one_row || j.cols % 8 == 0);
+    if (j.per_row) go(k_dropout<T, false, false, true>);
+    else if (one_row && eights) go(k_dropout<T, true, true, false>);
+    else if (one_row) go(k_dropout<T, true, false, false>);
+    else go(k_dropout<T, false, false, false>);
 }
 
 }  // namespace

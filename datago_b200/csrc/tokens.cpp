@@ -52,25 +52,21 @@ ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t k, bool b_by_column) {
     return p;
 }
 
-// threads of a row, rows of a CTA
-namespace {
-struct BackwardShape {
-    uint32_t threads, rows;
-};
-BackwardShape backward_shape(uint64_t cols) {
-    const uint64_t vecs = (cols + 7) / 8;
-    return vecs <= 160 ? BackwardShape{256, 8} : vecs <= 512 ? BackwardShape{256, 2} : BackwardShape{512, 1};
-}
-}  // namespace
-
 NormBackwardSplit norm_backward_split(uint64_t rows, uint64_t cols, uint64_t period, bool residual) {
-    const BackwardShape sh = backward_shape(cols);
-    const uint64_t at_once = (uint64_t)kTokenSms * 2 * sh.rows;  // rows that the chip works on at a time
+    NormBackwardSplit d{};
+    const uint64_t vecs = (cols + 7) / 8;
+    const uint64_t each = vecs > 512 ? 2 : 1;  // vectors of eight columns that a thread owns
+    d.row_threads = (uint32_t)((vecs + each - 1) / each + 31) / 32 * 32;
+    d.cta_workers = std::max(1u, 256 / d.row_threads);
+    const uint64_t ctas = (uint64_t)kTokenSms * std::max(1u, 480 / (d.row_threads * d.cta_workers)), workers = ctas * d.cta_workers;
     const uint64_t images = residual ? rows / period : 1;
-    uint64_t parts = 1;
-    if (residual && period < at_once) parts = std::max<uint64_t>(1, std::min(images, at_once / period));
-    const uint64_t units = (residual ? period : rows) * parts;
-    return {(uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((units + sh.rows - 1) / sh.rows, (uint64_t)kTokenSms * 2)), (uint32_t)parts};
+    d.by_image = images > 1;
+    d.parts = 1;
+    // few residual rows: their images go to several workers, four at least to each
+    if (d.by_image && period < workers) d.parts = (uint32_t)std::max<uint64_t>(1, std::min(images / 4, workers / period));
+    const uint64_t units = d.by_image ? period * d.parts : (rows + kNormChunk - 1) / kNormChunk;
+    d.ctas = (uint32_t)std::max<uint64_t>(1, std::min((units + d.cta_workers - 1) / d.cta_workers, ctas));
+    return d;
 }
 
 }  // namespace dg
@@ -173,7 +169,8 @@ extern "C" int dg_patch_rows(dg_ctx* ctx, void* stream, const uint8_t* pixels, u
     if (channels < 1 || channels > 4) return fail(DG_E_INVALID, "%u channels: 1 to 4 are wanted", channels);
     if (patch == 0 || patch > 4096 || h == 0 || w == 0 || h % patch || w % patch) return fail(DG_E_INVALID, "%u x %u pixels are no whole number of %u x %u patches", h, w, patch, patch);
     const uint64_t per_image = (uint64_t)(h / patch) * (w / patch), rows = n * per_image, cols = (uint64_t)patch * patch * channels;
-    if (per_image >> 32 || (uint64_t)w * channels >> 32) return fail(DG_E_INVALID, "%u x %u pixels are too many", h, w);
+    if ((uint64_t)patch * (patch * channels + 11) > 48 * 1024) return fail(DG_E_TOO_LARGE, "patches of %u x %u x %u: at most 48 KB", patch, patch, channels);
+    if (per_image > (1ull << 27) / scale_groups(cols)) return fail(DG_E_TOO_LARGE, "%u x %u pixels are too many for one image", h, w);
     if (n && !pixels) return fail(DG_E_INVALID, "pixels is NULL");
     if (out) {
         if (int rc = check_matrix(out, "out")) return rc;
@@ -187,6 +184,7 @@ extern "C" int dg_patch_rows(dg_ctx* ctx, void* stream, const uint8_t* pixels, u
         if (!(std[c] > 0) || !std::isfinite(std[c]) || !std::isfinite(mean[c])) return fail(DG_E_INVALID, "channel %u: mean and std are finite, std above 0", c);
         j.gain[c] = (float)(1.0 / (255.0 * std[c]));
         j.shift[c] = (float)(-(double)mean[c] / std[c]);
+        if (!std::isfinite(255 * j.gain[c]) || !std::isfinite(j.shift[c])) return fail(DG_E_INVALID, "channel %u: std is too small", c);
     }
     if (rows == 0) return DG_OK;
     return launched(ctx, [&] { launch_patch_rows(j, out8, out, stream_of(ctx, stream)); });
@@ -333,9 +331,11 @@ extern "C" int dg_rms_norm_backward(dg_ctx* ctx, void* stream, const dg_matrix* 
     if (dresidual && (residual_rows == 0 || dy->rows % residual_rows || residual_rows > kMostRows))
         return fail(DG_E_INVALID, "%llu residual rows do not divide %llu", (unsigned long long)residual_rows, (unsigned long long)dy->rows);
     const uint64_t period = dresidual ? residual_rows : dy->rows;
-    if (dy->rows)
-        if (int rc = check_workspace(workspace, workspace_bytes, norm_backward_workspace(norm_backward_split(dy->rows, dy->cols, period, dresidual != nullptr), dy->cols, period))) return rc;
     NormBackwardJob j{};
+    if (dy->rows) {
+        j.split = norm_backward_split(dy->rows, dy->cols, period, dresidual != nullptr);
+        if (int rc = check_workspace(workspace, workspace_bytes, norm_backward_workspace(j.split, dy->cols, period))) return rc;
+    }
     j.rows = dy->rows; j.period = period; j.cols = (uint32_t)dy->cols; j.dtype = dy->dtype;
     j.dy = dy->data; j.dy_ld = dy->ld; j.h = h->data; j.h_ld = h->ld; j.rstd = rstd;
     if (weight) { j.weight = weight->data; j.weight_dtype = weight->dtype; }

@@ -36,8 +36,19 @@ struct NormJob {
 };
 void launch_rms_norm(const NormJob& job, cudaStream_t s);
 
+// How the rows of the backward pass are dealt out: row_threads threads work on a row, cta_workers rows of threads make a CTA.
+constexpr uint32_t kNormChunk = 16;  // neighbouring rows that a worker takes at a time, where no images share a residual row
+struct NormBackwardSplit {
+    uint32_t row_threads, cta_workers, ctas;
+    uint32_t parts;  // that the images of a residual row are split into
+    bool by_image;   // images share residual rows, and their gradient is wanted
+};
+NormBackwardSplit norm_backward_split(uint64_t rows, uint64_t cols, uint64_t period, bool residual);
+inline uint64_t norm_backward_workspace(const NormBackwardSplit& d, uint64_t cols, uint64_t period) {
+    return 4 * cols * ((uint64_t)d.ctas * d.cta_workers + (d.parts > 1 ? d.parts * period : 0));
+}
 struct NormBackwardJob {
-    uint64_t rows, period;   // period: rows of dresidual, or `rows` without one
+    uint64_t rows, period;   // period: rows of dresidual
     uint32_t cols;
     int32_t dtype, weight_dtype;
     const void *dy, *h, *weight, *dsum;
@@ -45,15 +56,8 @@ struct NormBackwardJob {
     uint64_t dy_ld, h_ld, dsum_ld, dx_ld;
     void* dx;
     float *dresidual, *dweight;
+    NormBackwardSplit split;
 };
-// How the rows are dealt out: CTAs of the kernel, and the parts that the rows of one residual row are split into.
-struct NormBackwardSplit {
-    uint32_t ctas, parts;
-};
-NormBackwardSplit norm_backward_split(uint64_t rows, uint64_t cols, uint64_t period, bool residual);
-inline uint64_t norm_backward_workspace(const NormBackwardSplit& d, uint64_t cols, uint64_t period) {
-    return 4 * cols * ((uint64_t)d.ctas + (d.parts > 1 ? d.parts * period : 0));
-}
 void launch_rms_norm_backward(const NormBackwardJob& job, float* workspace, cudaStream_t s);
 
 // ---- dropout (kernels_tokens.cu) ----------------------------------------------------------------------------------------

@@ -14,7 +14,7 @@ void fake_product_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t out[6]) {
 }
 void fake_backward_split(uint64_t rows, uint64_t cols, uint64_t period, int residual, uint32_t out[2]) {
     const dg::NormBackwardSplit d = dg::norm_backward_split(rows, cols, period, residual != 0);
-    out[0] = d.ctas;
+    out[0] = d.ctas * d.cta_workers;
     out[1] = d.parts;
 }
 }

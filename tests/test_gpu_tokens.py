@@ -123,7 +123,7 @@ def patches_of(pixels, p):
 
 
 @pytest.mark.parametrize("channels", [1, 2, 3, 4])
-@pytest.mark.parametrize("n,grid,p", [(1, (1, 1), 1), (2, (3, 5), 3), (3, (2, 7), 14), (2, (5, 4), 16), (1, (3, 3), 20), (1, (9, 2), 8)])
+@pytest.mark.parametrize("n,grid,p", [(1, (1, 1), 1), (2, (3, 5), 3), (3, (2, 7), 14), (2, (5, 4), 16), (1, (3, 3), 20), (1, (9, 2), 8), (2, (2, 90), 5), (1, (2, 1), 109)])
 @pytest.mark.parametrize("lead", [0, 1, 8])
 def test_patch_rows(ctx, channels, n, grid, p, lead):
     h, w = grid[0] * p, grid[1] * p
@@ -254,7 +254,7 @@ def norm_of(x, residual, weight, eps):
     return h, rstd, h * rstd[:, None] * (1.0 if weight is None else weight.double())
 
 
-NORM_SIZES = [(1, 1, 1), (1, 1, 1152), (3, 5, 9), (2, 7, 255), (2, 3, 520), (2, 4, 800), (1, 9, 1280), (2, 3, 1500), (1, 4, 2048), (2, 2, 3000), (1, 3, 8000), (1, 2, 16384)]
+NORM_SIZES = [(1, 1, 1), (1, 1, 1152), (3, 5, 9), (2, 7, 255), (2, 3, 520), (2, 4, 800), (1, 9, 1280), (2, 3, 1500), (1, 4, 2048), (2, 2, 3000), (2, 3, 5000), (1, 3, 8000), (1, 2, 16384)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])

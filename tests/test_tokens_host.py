@@ -106,8 +106,10 @@ def test_patch_rows_refuses(L, ctx):
     launched(L, call(n=0, pixels=None, out8=rows8(0, 768)), 0)
     for bad in (dict(out8=None), dict(out=matrix(12, 768)), dict(mean=None), dict(std=None), dict(c=0), dict(c=5), dict(p=0), dict(p=5), dict(h=0), dict(h=40), dict(w=40),
                 dict(std=zero), dict(std=nan), dict(mean=nan), dict(pixels=None), dict(out8=rows8(11, 768)), dict(out8=rows8(12, 256)), dict(out8=rows8(12, 768, block=128)), dict(out8=rows8(12, 768, by_column=1)),
-                dict(out8=None, out=matrix(12, 767)), dict(n=1 << 20)):
+                dict(out8=None, out=matrix(12, 767)), dict(n=1 << 20), dict(std=(C.c_float * 4)(1, 1e-39, 1, 1))):
         refused(L, call(**bad))
+    refused(L, call(h=128, w=128, p=128, out8=rows8(2, 49152)), TOO_LARGE)
+    refused(L, call(n=1, h=1 << 14, w=1 << 14, c=1, p=1, out8=rows8(1 << 28, 1)), TOO_LARGE)
 
 
 def test_product_refuses(L, ctx):
@@ -222,10 +224,10 @@ def test_product_plans_cover_the_output_and_the_contraction(L, m, n, k):
 def test_norm_backward_deals_out_every_row(L, rows, cols, period, residual):
     v = (C.c_uint32 * 2)()
     L.fake_backward_split(C.c_uint64(rows), C.c_uint64(cols), C.c_uint64(period), residual, v)
-    ctas, parts = v
-    assert 1 <= ctas <= 148 * 8 and 1 <= parts <= rows // period
+    workers, parts = v
+    assert 1 <= workers <= 148 * 32 and 1 <= parts <= rows // period
     ctx = dg.Context(0)
-    assert L.dg_rms_norm_backward_workspace(ctx._h, rows, cols, period if residual else 0) >= 4 * cols * (ctas + (parts * period if parts > 1 else 0))
+    assert L.dg_rms_norm_backward_workspace(ctx._h, rows, cols, period if residual else 0) >= 4 * cols * (workers + (parts * period if parts > 1 else 0))
 
 
 def test_tensors_of_the_host_and_of_other_shapes_are_refused():
