@@ -10,7 +10,7 @@
 //   copier    a ring slot holds 256 columns of the CTA's share of both operands (four tensor-map copies, 128-byte swizzle).  Short contractions
 //             have a ring for b alone: the rows of a stay while the pair walks the tiles of those rows, which halves what crosses from L2.
 //   issuer    of the first CTA only; eight instructions per slot, and per eight groups the copies of the scales into tensor memory
-//   4 scalers fetch the scale bytes of eight groups (two words per row) and lay them out for those copies: row r of 128 at
+//   3 scalers fetch the scale bytes of eight groups (two words per row) and lay them out for those copies: row r of 128 at
 //             (r % 32) * 16 + (r / 32) * 4.  Both CTAs need all scales of b.  The words of the next octets are under way meanwhile: fetched
 //             one quad after the other by one warp, 131072 x 1152 x 768 took 200 us, by two with the next words under way 156, by four 138.
 //   4 storers read the sums of a finished tile out of tensor memory, one lane a row, round them and send them out through shared memory
@@ -32,12 +32,12 @@ namespace dg {
 namespace {
 
 constexpr uint32_t kTileM = kProductTileM, kRowsPerCta = kTileM / 2;
-constexpr uint32_t kScaleStages = 4, kScalers = 4;
+constexpr uint32_t kScalers = 3, kScaleStages = kScalers;  // a slot's fillings are all one warp's: it cannot miss one of them
 constexpr uint32_t kABytes = kProductABytes;  // of a group; a slot holds two
 constexpr uint32_t kScaleBytes = 512 * 3;  // of four groups: 128 rows of a, 256 of b; a slot holds eight groups'
-constexpr uint32_t kOutBytes = 32 * 64;    // a storer's piece of the output: 32 rows x 64 bytes, two of them
-constexpr uint32_t kThreads = 320, kSlots = kProductSlots;
-constexpr uint32_t kOutAt = kProductRingBytes, kScalesAt = kOutAt + 4 * 2 * kOutBytes;
+constexpr uint32_t kOutBytes = 32 * 64, kPieces = 3;  // a storer's piece of the output: 32 rows x 64 bytes; pieces it has room for
+constexpr uint32_t kThreads = 9 * 32, kSlots = kProductSlots;
+constexpr uint32_t kOutAt = kProductRingBytes, kScalesAt = kOutAt + 4 * kPieces * kOutBytes;
 constexpr uint32_t kSmemBytes = kScalesAt + kScaleStages * 2 * kScaleBytes + 1024;
 static_assert(kSmemBytes <= 232448 - 512, "what a CTA may have, and the barriers");
 // tensor memory: the accumulators from column 0 and, up to kProductTwoSums wide, from column kProductTwoSums; then, twice, scales of eight groups
@@ -399,10 +399,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_produ
         }
     } else {  // ---- storers
         constexpr uint32_t kPiece = 64 / sizeof(T);  // columns of a piece
-        const uint32_t rows = (warp & 3u) * 32, mine = smem + kOutAt + (warp & 3u) * 2 * kOutBytes;
-        const bool by_map = j.out_by_map;
+        const uint32_t rows = (warp & 3u) * 32, mine = smem + kOutAt + (warp & 3u) * kPieces * kOutBytes;
+        const bool by_map = j.out_by_map, by_word = sizeof(T) == 4 || ((reinterpret_cast<uintptr_t>(out) | (ld * sizeof(T)) | (part_elements * sizeof(T))) & 3u) == 0;
+        Place room;
         Place sum;
-        uint32_t pieces = 0;
         bool go_on = true;
         for (uint32_t i = first; go_on && i < end; i += step) {
             const Tile t = tile_at(i);
@@ -410,10 +410,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_produ
             if (!go_on) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t from = tmem + sum.slot * kSecond + (rows << 16);
-            const uint64_t row = (uint64_t)t.m0 + rows + lane;
-            T* const to = out + t.split * part_elements + row * ld + t.n0;
+            const uint64_t row0 = (uint64_t)t.m0 + rows;
+            const uint32_t live = row0 < j.m ? (uint32_t)min((uint64_t)32, j.m - row0) : 0;  // rows of this warp that the matrix has
             const uint32_t width = (uint32_t)min((uint64_t)tile_n, j.n - t.n0);
-            for (uint32_t c = 0; c < width; c += kPiece, ++pieces) {
+            for (uint32_t c = 0; c < width; c += kPiece) {
                 uint32_t v[kPiece], w[16];
 #pragma unroll
                 for (uint32_t k = 0; k < kPiece; k += 16) read_16(from + c + k, v + k);
@@ -423,22 +423,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_produ
                     if constexpr (sizeof(T) == 4) w[k] = v[k];
                     else w[k] = pair(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]), T());
                 }
-                if (by_map) {  // rows and columns outside the matrix are not written
-                    const uint32_t piece = mine + (pieces & 1u) * kOutBytes;
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the piece before the last has been read
-                    __syncwarp();
+                const uint32_t piece = mine + room.slot * kOutBytes;
+                room.next(kPieces);
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kPieces - 1) : "memory");  // the piece that was here has left
+                __syncwarp();
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k)  // 64-byte swizzle: 16 bytes k of row r at k ^ (r / 2 % 4)
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(piece + lane * 64 + ((k ^ ((lane >> 1) & 3u)) << 4)), "r"(w[4 * k]),
-                                     "r"(w[4 * k + 1]), "r"(w[4 * k + 2]), "r"(w[4 * k + 3]) : "memory");
+                for (uint32_t k = 0; k < 4; ++k)  // 64-byte swizzle: 16 bytes k of row r at k ^ (r / 2 % 4)
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(piece + lane * 64 + ((k ^ ((lane >> 1) & 3u)) << 4)), "r"(w[4 * k]), "r"(w[4 * k + 1]),
+                                 "r"(w[4 * k + 2]), "r"(w[4 * k + 3]) : "memory");
+                if (by_map) {  // rows and columns outside the matrix are not written
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0 && t.m0 + rows < j.m) store_box(&j.out_map, (int32_t)(t.n0 + c), (int32_t)(t.m0 + rows), (int32_t)t.split, piece);
-                } else if (row < j.m) {
-                    const uint32_t left = width - c;
-#pragma unroll
-                    for (uint32_t k = 0; k < kPiece; ++k)
-                        if (k < left) to[c + k] = one<T>(__uint_as_float(v[k]));
+                    if (lane == 0 && live) store_box(&j.out_map, (int32_t)(t.n0 + c), (int32_t)row0, (int32_t)t.split, piece);
+                } else {  // two rows at a time, neighbouring lanes neighbouring words (or elements, of rows that do not begin at words)
+                    __syncwarp();
+                    T* const to = out + t.split * part_elements + row0 * ld + t.n0 + c;
+                    const uint32_t left = width - c, k = lane & 15u;
+                    for (uint32_t r = lane >> 4; r < live; r += 2) {
+                        uint32_t word;
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(word) : "r"(piece + r * 64 + (((k >> 2) ^ ((r >> 1) & 3u)) << 4) + (k & 3u) * 4));
+                        if constexpr (sizeof(T) == 4) {
+                            if (k < left) reinterpret_cast<uint32_t*>(to + r * ld)[k] = word;
+                        } else {
+                            uint16_t* const p = reinterpret_cast<uint16_t*>(to + r * ld) + 2 * k;
+                            if (by_word && 2 * k + 1 < left) *reinterpret_cast<uint32_t*>(p) = word;
+                            else {
+                                if (2 * k < left) p[0] = (uint16_t)word;
+                                if (2 * k + 1 < left) p[1] = (uint16_t)(word >> 16);
+                            }
+                        }
+                    }
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
