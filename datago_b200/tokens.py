@@ -97,17 +97,21 @@ def _invalid(msg):
 def _on_device(ctx, t, name):
     if not isinstance(t, torch.Tensor):
         raise _invalid(f"{name}: a torch tensor is wanted")
-    if not t.is_cuda or t.get_device() != ctx.device:
+    if t.get_device() != ctx.device or not t.is_cuda:  # (-1 for tensors of the host)
         raise _invalid(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
+
+
+def _new(shape, dtype, like):
+    """torch.empty, in two thirds of its time"""
+    return torch.empty_strided(shape, (shape[1], 1) if len(shape) == 2 else (1,), dtype=dtype, device=like.device)
 
 
 def _matrix(ctx, t, name):
     _on_device(ctx, t, name)
-    dtype = _DTYPES.get(t.dtype)
-    if dtype is None or t.dim() != 2:
+    dtype, shape = _DTYPES.get(t.dtype), t.shape
+    if dtype is None or len(shape) != 2:
         raise _invalid(f"{name}: a 2-d tensor of float32, bfloat16 or float16 is wanted")
-    rows, cols = t.shape
-    step, one = t.stride()
+    (rows, cols), (step, one) = shape, t.stride()
     if (one != 1 and cols > 1) or (rows > 1 and step < cols):
         raise _invalid(f"{name}: columns have to be neighbours in memory, rows apart")
     return _matrix_desc(t.data_ptr(), rows, cols, step if rows > 1 else cols, dtype, 0)
@@ -131,10 +135,11 @@ def _rows8(ctx, r, name, transposed=None):
     v, s = r.values, r.scales
     _on_device(ctx, v, name)
     _on_device(ctx, s, name)
-    if v.dtype != torch.float8_e4m3fn or s.dtype != torch.float8_e8m0fnu or v.dim() != 2 or s.dim() != 2 or r.block not in (1, GROUP):
+    shape, sshape, block = v.shape, s.shape, r.block
+    if v.dtype != torch.float8_e4m3fn or s.dtype != torch.float8_e8m0fnu or len(shape) != 2 or len(sshape) != 2 or (block != 1 and block != GROUP):
         raise _invalid(f"{name}: values float8_e4m3fn, scales float8_e8m0fnu, both 2-d, and block 1 or 128 are wanted")
-    (rows, cols), (srows, groups) = v.shape, s.shape
-    if srows != -(-rows // r.block) or groups != -(-cols // GROUP):
+    (rows, cols), (srows, groups) = shape, sshape
+    if srows != -(-rows // block) or groups != -(-cols // GROUP):
         raise _invalid(f"{name}: {rows} x {cols} values have {-(-rows // r.block)} x {-(-cols // GROUP)} scales")
     (ld, one), (scale_ld, sone) = v.stride(), s.stride()
     if sone != 1 and groups > 1:
@@ -148,7 +153,7 @@ def _rows8(ctx, r, name, transposed=None):
         ld, column = one if cols > 1 else -(-rows // 16) * 16, 1
     else:
         raise _invalid(f"{name}: rows{' or columns' if transposed is None else ' by column' if transposed else ''} have to be neighbours in memory")
-    return _rows8_desc(v.data_ptr(), s.data_ptr(), rows, cols, ld, scale_ld if srows > 1 else -(-groups // 4) * 4, r.block, column)
+    return _rows8_desc(v.data_ptr(), s.data_ptr(), rows, cols, ld, scale_ld if srows > 1 else -(-groups // 4) * 4, block, column)
 
 
 # The current stream's handle without an object around it, where torch has that.
@@ -157,7 +162,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda de
 
 def _out(out, shape, dtype, like, name):
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return _new(shape, dtype, like)
     if not isinstance(out, torch.Tensor) or tuple(out.shape) != tuple(shape) or out.dtype != dtype:
         raise _invalid(f"{name}: a tensor {tuple(shape)} of {dtype} is wanted")
     return out
@@ -221,7 +226,7 @@ def product(ctx, a, b, dtype=torch.bfloat16, out=None):
     (m, k), n = a.values.shape, b.values.shape[0]
     out = _out(out, (m, n), dtype, a.values, "out")
     L = lib()
-    nbytes = L.dg_product_workspace(ctx._h, m, n, k)
+    nbytes = L.dg_product_workspace(ctx._h, m, n, k) if k > 1920 else 0
     work, at = _workspace(nbytes, out)
     _check(L.dg_product(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, da, db, _matrix(ctx, out, "out"), at, nbytes))
     return out
@@ -240,13 +245,13 @@ def rms_norm(ctx, x, weight=None, residual=None, eps=1e-6, eight_bit=False, sum_
     w = _vector(ctx, weight, "weight", cols)
     r = None if residual is None else _matrix(ctx, residual, "residual")
     total = _out(sum_out, (rows, cols), x.dtype, x, "sum_out")
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    rstd = _new((rows,), torch.float32, x)
     y16 = y8 = None
     if eight_bit:
         y = Rows8.empty(rows, cols, x.device)
         y8 = _rows8(ctx, y, "y")
     else:
-        y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+        y = _new((rows, cols), x.dtype, x)
         y16 = _matrix(ctx, y, "y")
     _check(lib().dg_rms_norm(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, src, r, w, eps, _matrix(ctx, total, "sum_out"), y16, y8, rstd.data_ptr()))
     return Norm(y, total, rstd)
@@ -266,8 +271,8 @@ def rms_norm_backward(ctx, dy, h, rstd, weight=None, dsum=None, residual_rows=No
     period = int(residual_rows or 0)
     if residual_rows is not None and (period < 1 or rows % period):
         raise _invalid(f"{residual_rows} residual rows do not divide {rows}")
-    dweight = torch.empty(cols, dtype=torch.float32, device=dy.device)
-    dresidual = torch.empty((period, cols), dtype=torch.float32, device=dy.device) if period else None
+    dweight = _new((cols,), torch.float32, dy)
+    dresidual = _new((period, cols), torch.float32, dy) if period else None
     L = lib()
     nbytes = L.dg_rms_norm_backward_workspace(ctx._h, rows, cols, period)
     work, at = _workspace(nbytes, dy)
@@ -280,10 +285,7 @@ def dropout(ctx, x, p, seed, offset=0, per_row=False, out=None):
     """x with elements (or, per_row, rows) dropped with probability p and the others scaled up.  The mask is a function of (seed, offset + index):
     the same call on the gradient is the backward pass.  out may be x."""
     src = _matrix(ctx, x, "x")
-    if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    else:
-        _out(out, x.shape, x.dtype, x, "out")
+    out = _out(out, x.shape, x.dtype, x, "out")
     seed, offset = int(seed), int(offset)
     if not 0 <= seed < 1 << 64 or not 0 <= offset < 1 << 64:
         raise _invalid("seed and offset are in [0, 2^64)")

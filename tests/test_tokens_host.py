@@ -217,6 +217,7 @@ def test_product_plans_cover_the_output_and_the_contraction(L, m, n, k):
     groups = -(-k // 128)
     assert tile_n % 32 == 0 and 32 <= tile_n <= (256 if sums == 1 else 224)
     assert (tiles_m - 1) * 256 < m <= tiles_m * 256 and (tiles_n - 1) * tile_n < n <= tiles_n * tile_n
+    assert splits == 1 or k > 1920  # what the binding counts on
     assert (splits == 1 or per_split % 4 == 0) and (splits - 1) * per_split < groups <= splits * per_split
 
 
