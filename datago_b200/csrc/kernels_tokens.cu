@@ -119,6 +119,48 @@ template <class T> struct Raw8 {  // eight neighbouring elements as they are in 
     }
 };
 
+// ---- two floats at a time ------------------------------------------------------------------------------------------------
+// The 32-bit units multiply and add pairs (fma.rn.f32x2): these kernels issue as many instructions as the chip can while memory is busy.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair_of(float lo, float hi) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+    return p;
+}
+__device__ __forceinline__ void parts_of(Pair p, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+// max(top, |lo|, |hi|); NaN as soon as one of them is
+__device__ __forceinline__ float larger2(float top, Pair p) {
+    float lo, hi, d;
+    parts_of(p, lo, hi);
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(top), "f"(lo), "f"(hi));
+    return d;
+}
+template <class T> __device__ __forceinline__ void pairs_of(const Raw8<T>& x, Pair p[4]) {
+    float v[8];
+    x.widen(v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = pair_of(v[2 * i], v[2 * i + 1]);
+}
+__device__ __forceinline__ void floats_of(const Pair p[4], float v[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) parts_of(p[i], v[2 * i], v[2 * i + 1]);
+}
+
 // ---- scales -------------------------------------------------------------------------------------------------------------
 // Magnitudes are compared as bit patterns: those of finite numbers order like the numbers, an infinity is above them and a NaN above that.
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
@@ -145,6 +187,12 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
     return (uint32_t)lo | (uint32_t)hi << 16;
+}
+__device__ __forceinline__ uint32_t e4m3x4(Pair a, Pair b) {
+    float v[4];
+    parts_of(a, v[0], v[1]);
+    parts_of(b, v[2], v[3]);
+    return e4m3x4(v[0], v[1], v[2], v[3]);
 }
 __device__ __forceinline__ uint2 quantize8(const float v[8], float inverse) {
     return make_uint2(e4m3x4(v[0] * inverse, v[1] * inverse, v[2] * inverse, v[3] * inverse),
@@ -245,7 +293,7 @@ template <class Out> struct PatchOut {
 
 // pixel bytes (four to a word) to values; the first is of channel `phase`.  2^23 + pixel, as a float, has the pixel in its low byte.
 template <int C>
-__device__ __forceinline__ void normalise16(const PatchView<C>& in, const uint32_t w[4], uint32_t phase, float v[16]) {
+__device__ __forceinline__ void normalise16(const PatchView<C>& in, const uint32_t w[4], uint32_t phase, Pair v[8]) {
     float g[C], b[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -255,29 +303,41 @@ __device__ __forceinline__ void normalise16(const PatchView<C>& in, const uint32
         for (int k = 1; k < C; ++k)
             if (phase == (uint32_t)k) { g[c] = in.gain[(c + k) % C]; b[c] = in.shift[(c + k) % C]; }
     }
+    const Pair less = pair_of(-8388608.f, -8388608.f);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = fmaf(__uint_as_float(__byte_perm(w[j >> 2], 0x4B000000u, 0x7650 + (j & 3))) - 8388608.f, g[j % C], b[j % C]);
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t word = w[j >> 1], at = 2 * (j & 1);
+        const Pair u = pair_of(__uint_as_float(__byte_perm(word, 0x4B000000u, 0x7650 + at)), __uint_as_float(__byte_perm(word, 0x4B000000u, 0x7651 + at)));
+        v[j] = fma2(add2(u, less), pair_of(g[(2 * j) % C], g[(2 * j + 1) % C]), pair_of(b[(2 * j) % C], b[(2 * j + 1) % C]));
+    }
 }
 
 // Sixteen features of a row from `col` on, `valid` of them; all lanes of a warp are here.
 template <class Out>
-__device__ __forceinline__ void store16(const PatchOut<Out>& out, uint64_t row, uint32_t col, uint32_t valid, float v[16]) {
+__device__ __forceinline__ void store16(const PatchOut<Out>& out, uint64_t row, uint32_t col, uint32_t valid, Pair v[8]) {
     if constexpr (sizeof(Out) == 1) {
-        uint32_t top = 0;
+        if (valid < 16) {  // what is not there has no part in the scale
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            if (valid < 16 && (uint32_t)j >= valid) v[j] = 0.f;
-            top = max(top, magnitude(v[j]));
+            for (uint32_t j = 0; j < 8; ++j) {
+                float lo, hi;
+                parts_of(v[j], lo, hi);
+                v[j] = pair_of(valid > 2 * j ? lo : 0.f, valid > 2 * j + 1 ? hi : 0.f);
+            }
         }
+        float largest = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) largest = larger2(largest, v[j]);
+        uint32_t top = magnitude(largest);
 #pragma unroll
         for (int d = 4; d; d >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
         const uint32_t e = scale_byte(top);
         const float inverse = inverse_scale(e);
         if (!valid) return;
         uint8_t* const p = out.data + row * out.ld + col;
+        const Pair by = pair_of(inverse, inverse);
         uint32_t q[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = e4m3x4(v[4 * j] * inverse, v[4 * j + 1] * inverse, v[4 * j + 2] * inverse, v[4 * j + 3] * inverse);
+        for (int j = 0; j < 4; ++j) q[j] = e4m3x4(mul2(v[2 * j], by), mul2(v[2 * j + 1], by));
         if (valid >= 16) *reinterpret_cast<uint4*>(p) = make_uint4(q[0], q[1], q[2], q[3]);
         else
 #pragma unroll
@@ -286,8 +346,11 @@ __device__ __forceinline__ void store16(const PatchOut<Out>& out, uint64_t row, 
         if ((threadIdx.x & 7u) == 0) out.scales[row * out.scale_ld + col / kScaleGroup] = (uint8_t)e;
     } else {
         Out* const p = out.data + row * out.ld + col;
-        store8(p, valid, out.whole, v);
-        if (valid > 8) store8(p + 8, valid - 8, out.whole, v + 8);
+        float f[16];
+        floats_of(v, f);
+        floats_of(v + 4, f + 8);
+        store8(p, valid, out.whole, f);
+        if (valid > 8) store8(p + 8, valid - 8, out.whole, f + 8);
     }
 }
 
@@ -313,7 +376,7 @@ __global__ void __launch_bounds__(kRowThreads) k_patches(const PatchView<C> in, 
 #pragma unroll
         for (uint32_t k = 0; k < kPieces; ++k) {
             const uint32_t words[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-            float v[16];
+            Pair v[8];
             normalise16<C>(in, words, C == 3 ? col[k] % 3 : 0, v);  // 16 is a multiple of 1, 2 and 4
             store16(out, row[k], col[k], valid[k], v);
         }
@@ -359,7 +422,7 @@ __global__ void __launch_bounds__(kRowThreads) k_patches_staged(const PatchView<
                     if (++b == in.segment && j + 1 < valid) { b = 0; ++y; q = line(); }
                 }
             }
-            float v[16];
+            Pair v[8];
             normalise16<C>(in, w, col % C, v);
             store16(out, (uint64_t)band * in.grid_w + x0 + x, col, valid, v);
         }
@@ -542,6 +605,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) k_rms_norm(co
         const void* const pw = from_previous(a.weight);
         for (uint32_t c = threadIdx.x; c < a.cols; c += THREADS)
             s_weight[c] = a.weight_dtype == DG_F32 ? reinterpret_cast<const float*>(pw)[c] : a.weight_dtype == DG_BF16 ? widen(reinterpret_cast<const bf16*>(pw)[c]) : widen(reinterpret_cast<const __half*>(pw)[c]);
+        for (uint32_t c = a.cols + threadIdx.x; c < (a.cols + 7) / 8 * 8; c += THREADS) s_weight[c] = 0.f;
         __syncthreads();
     }
     constexpr uint32_t kRows = THREADS / TPR;
@@ -575,16 +639,16 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) k_rms_norm(co
     fetch(row, rr);
     for (uint64_t r0 = (uint64_t)blockIdx.x * kRows; r0 < a.rows; r0 += stride, row += stride) {
         const bool live = row < a.rows;
-        float h[V][8];
-        float sum = 0.f;
+        Pair h[V][4];
+        Pair sums = pair_of(0.f, 0.f);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            x[k].widen(h[k]);
+            pairs_of(x[k], h[k]);
             if (pr) {
-                float v[8];
-                r[k].widen(v);
+                Pair v[4];
+                pairs_of(r[k], v);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[k][j] += v[j];
+                for (int j = 0; j < 4; ++j) h[k][j] = add2(h[k][j], v[j]);
             }
         }
         rr += rr_step;
@@ -593,40 +657,65 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) k_rms_norm(co
 #pragma unroll
         for (int k = 0; k < V; ++k)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf(h[k][j], h[k][j], sum);
-        const float rstd = 1.f / sqrtf(row_sum<TPR>(sum, s_part) * per_col + a.eps);
+            for (int j = 0; j < 4; ++j) sums = fma2(h[k][j], h[k][j], sums);
+        float even, odd;
+        parts_of(sums, even, odd);
+        const float rstd = 1.f / sqrtf(row_sum<TPR>(even + odd, s_part) * per_col + a.eps);
         if (live && t == 0 && a.rstd) a.rstd[row] = rstd;
         if (a.sum) {
             T* const to = reinterpret_cast<T*>(a.sum) + row * a.sum_ld;
 #pragma unroll
             for (int k = 0; k < V; ++k)
-                if (live && valid_at(k)) store8(to + (k * TPR + t) * 8, valid_at(k), WHOLE || s_whole, h[k]);
+                if (live && valid_at(k)) {
+                    float v[8];
+                    floats_of(h[k], v);
+                    store8(to + (k * TPR + t) * 8, valid_at(k), WHOLE || s_whole, v);
+                }
         }
+        const Pair rstds = pair_of(rstd, rstd);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-            if (a.weight) {
-                float w[8];
-                if (valid_at(k)) load8((const float*)s_weight + (k * TPR + t) * 8, valid_at(k), true, w);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[k][j] = valid_at(k) > (uint32_t)j ? h[k][j] * rstd * w[j] : 0.f;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) h[k][j] *= rstd;
+            for (int j = 0; j < 4; ++j) h[k][j] = mul2(h[k][j], rstds);
+            if (a.weight) {  // (the floats behind the last column are zeros)
+                const ulonglong2 *const w = reinterpret_cast<const ulonglong2*>(s_weight + (valid_at(k) ? (k * TPR + t) * 8 : 0)), lo = w[0], hi = w[1];
+                h[k][0] = mul2(h[k][0], lo.x);
+                h[k][1] = mul2(h[k][1], lo.y);
+                h[k][2] = mul2(h[k][2], hi.x);
+                h[k][3] = mul2(h[k][3], hi.y);
             }
         }
         if (a.y) {
             T* const to = reinterpret_cast<T*>(a.y) + row * a.y_ld;
 #pragma unroll
             for (int k = 0; k < V; ++k)
-                if (live && valid_at(k)) store8(to + (k * TPR + t) * 8, valid_at(k), WHOLE || y_whole, h[k]);
+                if (live && valid_at(k)) {
+                    float v[8];
+                    floats_of(h[k], v);
+                    store8(to + (k * TPR + t) * 8, valid_at(k), WHOLE || y_whole, v);
+                }
         }
         if (a.y8.values) {
             uint8_t *const to = a.y8.values + row * a.y8.ld, *const scales = a.y8.scales + row * a.y8.scale_ld;
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                const uint32_t e = scale_byte(largest_of_16_lanes(largest8(h[k])));
+                float top = 0.f;
+                if (valid_at(k)) {  // lanes behind the last column have no part in a scale
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (!WHOLE && valid_at(k) < 8) {  // nor have elements
+                            float lo, hi;
+                            parts_of(h[k][j], lo, hi);
+                            h[k][j] = pair_of(valid_at(k) > 2u * j ? lo : 0.f, valid_at(k) > 2u * j + 1 ? hi : 0.f);
+                        }
+                        top = larger2(top, h[k][j]);
+                    }
+                }
+                const uint32_t e = scale_byte(largest_of_16_lanes(magnitude(top)));
                 if (live && valid_at(k)) {
-                    store_values8(to + (k * TPR + t) * 8, valid_at(k), quantize8(h[k], inverse_scale(e)));
+                    const float inverse = inverse_scale(e);
+                    const Pair by = pair_of(inverse, inverse);
+                    store_values8(to + (k * TPR + t) * 8, valid_at(k), make_uint2(e4m3x4(mul2(h[k][0], by), mul2(h[k][1], by)), e4m3x4(mul2(h[k][2], by), mul2(h[k][3], by))));
                     if ((t & 15u) == 0) scales[(k * TPR + t) / 16] = (uint8_t)e;
                 }
             }
@@ -723,14 +812,15 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) k_rms_norm_backward
     const uint64_t units = by_image ? a.period * parts : (a.rows + kNormChunk - 1) / kNormChunk;
     const float per_col = 1.f / (float)a.cols;
     uint32_t cols[V], valid[V];
-    float w[V][8], dw[V][8];
+    Pair w[V][4], dw[V][4] = {};
 #pragma unroll
     for (int k = 0; k < V; ++k) {
+        float v[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
         cols[k] = (k * row_threads + t) * 8;
         valid[k] = cols[k] >= a.cols ? 0u : WHOLE ? 8u : min(8u, a.cols - cols[k]);
+        if (a.weight && valid[k]) load8_any(from_previous(a.weight), cols[k], a.weight_dtype, valid[k], w_whole, v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { w[k][j] = 1.f; dw[k][j] = 0.f; }
-        if (a.weight && valid[k]) load8_any(from_previous(a.weight), cols[k], a.weight_dtype, valid[k], w_whole, w[k]);
+        for (int j = 0; j < 4; ++j) w[k][j] = pair_of(v[2 * j], v[2 * j + 1]);
     }
     uint32_t turn = 0;
     for (uint64_t unit = me; unit < units; unit += workers) {
@@ -745,7 +835,7 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) k_rms_norm_backward
             stride = 1;
             count = min((uint64_t)kNormChunk, a.rows - row0);
         }
-        float dr[V][8] = {};
+        Pair dr[V][4] = {};  // (a pair of zeros is zero)
         Raw8<T> dy[R][V], h[R][V];
         float rstd[R];
         auto fetch = [&](uint64_t i) {
@@ -779,46 +869,54 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) k_rms_norm_backward
             if (i + R < count) fetch(i + R);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                along[r] = 0.f;
+                Pair sums = pair_of(0.f, 0.f);
+                const Pair rstds = pair_of(rstd_now[r], rstd_now[r]);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    float g[8], hat[8];
-                    dy_now[r][k].widen(g);
-                    h_now[r][k].widen(hat);
+                    Pair g[4], hat[4];
+                    pairs_of(dy_now[r][k], g);
+                    pairs_of(h_now[r][k], hat);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        hat[j] *= rstd_now[r];
-                        dw[k][j] = fmaf(g[j], hat[j], dw[k][j]);
-                        along[r] = fmaf(g[j] * w[k][j], hat[j], along[r]);
+                    for (int j = 0; j < 4; ++j) {
+                        const Pair x = mul2(hat[j], rstds), gx = mul2(g[j], x);
+                        dw[k][j] = add2(gx, dw[k][j]);
+                        sums = fma2(gx, w[k][j], sums);
                     }
                 }
+                float even, odd;
+                parts_of(sums, even, odd);
+                along[r] = even + odd;
             }
             sums_across<R>(along, row_threads / 32, t >> 5, worker + 1, row_threads, s_part[turn]);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 if (i + r >= count) break;
                 const uint64_t row = row0 + (i + r) * stride;
-                const float mean = along[r] * per_col;
+                // rstd * (g w - hat mean(g w hat)) = rstd * g w - h * (rstd^2 mean)
+                const float back = -along[r] * per_col * rstd_now[r] * rstd_now[r];
+                const Pair rstds = pair_of(rstd_now[r], rstd_now[r]), backs = pair_of(back, back);
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     if (!valid[k]) continue;
-                    float d[8], hat[8];
-                    dy_now[r][k].widen(d);
-                    h_now[r][k].widen(hat);
+                    Pair d[4], h2[4];
+                    pairs_of(dy_now[r][k], d);
+                    pairs_of(h_now[r][k], h2);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) d[j] = rstd_now[r] * (d[j] * w[k][j] - hat[j] * rstd_now[r] * mean);
+                    for (int j = 0; j < 4; ++j) d[j] = fma2(h2[j], backs, mul2(mul2(d[j], w[k][j]), rstds));
                     if (ps) {
                         float extra[8];
                         load8(ps + row * a.dsum_ld + cols[k], valid[k], WHOLE || s_whole, extra);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) d[j] += extra[j];
+                        for (int j = 0; j < 4; ++j) d[j] = add2(d[j], pair_of(extra[2 * j], extra[2 * j + 1]));
                     }
-                    if (a.dx) store8(reinterpret_cast<T*>(a.dx) + row * a.dx_ld + cols[k], valid[k], WHOLE || x_whole, d);
+                    float v[8];
+                    floats_of(d, v);
+                    if (a.dx) store8(reinterpret_cast<T*>(a.dx) + row * a.dx_ld + cols[k], valid[k], WHOLE || x_whole, v);
                     if (by_image) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) dr[k][j] += d[j];
+                        for (int j = 0; j < 4; ++j) dr[k][j] = add2(dr[k][j], d[j]);
                     } else if (a.dresidual) {
-                        store8(a.dresidual + row * a.cols + cols[k], valid[k], WHOLE && (reinterpret_cast<uintptr_t>(a.dresidual) & 15u) == 0, d);
+                        store8(a.dresidual + row * a.cols + cols[k], valid[k], WHOLE && (reinterpret_cast<uintptr_t>(a.dresidual) & 15u) == 0, v);
                     }
                 }
             }
@@ -827,42 +925,52 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) k_rms_norm_backward
             float* const to = parts > 1 ? r_parts + unit * a.cols : a.dresidual + unit * a.cols;
 #pragma unroll
             for (int k = 0; k < V; ++k)
-                if (valid[k]) store8(to + cols[k], valid[k], WHOLE && (reinterpret_cast<uintptr_t>(to) & 15u) == 0, dr[k]);
+                if (valid[k]) {
+                    float v[8];
+                    floats_of(dr[k], v);
+                    store8(to + cols[k], valid[k], WHOLE && (reinterpret_cast<uintptr_t>(to) & 15u) == 0, v);
+                }
         }
     }
     if (!a.dweight) return;
     float* const to = w_parts + (uint64_t)me * a.cols;
 #pragma unroll
     for (int k = 0; k < V; ++k)
-        if (valid[k]) store8(to + cols[k], valid[k], WHOLE, dw[k]);  // the workspace is aligned, and so are its rows if they are whole vectors
+        if (valid[k]) {  // the workspace is aligned, and so are its rows if they are whole vectors
+            float v[8];
+            floats_of(dw[k], v);
+            store8(to + cols[k], valid[k], WHOLE, v);
+        }
 }
 
-// out[i] = the sum of parts[p][i] in a fixed order: sixteen threads a column, each every sixteenth part
-constexpr uint32_t kSumThreads = 512;
+// out[i] = the sum of parts[p][i] in a fixed order: eight columns a CTA, sixty-four threads a column, each every sixty-fourth part
+constexpr uint32_t kSumThreads = 512, kSumCols = 8, kSumLanes = kSumThreads / kSumCols;
 __global__ void __launch_bounds__(kSumThreads) k_sum_parts(const float* parts, uint32_t count, uint64_t n, float* out) {
-    constexpr uint32_t kLanes = kSumThreads / 32;
-    __shared__ float s_sum[kLanes][33];
+    __shared__ float s_sum[kSumThreads / 32][kSumCols];
     let_next_start();
     wait_for_previous();
     parts = from_previous(parts);
-    const uint32_t lane = threadIdx.x & 31u, part = threadIdx.x >> 5;
-    for (uint64_t i0 = (uint64_t)blockIdx.x * 32; i0 < n; i0 += (uint64_t)gridDim.x * 32) {
-        const uint64_t i = i0 + lane;
+    const uint32_t col = threadIdx.x % kSumCols, part = threadIdx.x / kSumCols;
+    for (uint64_t i0 = (uint64_t)blockIdx.x * kSumCols; i0 < n; i0 += (uint64_t)gridDim.x * kSumCols) {
+        const uint64_t i = i0 + col;
         float sum = 0.f;
         if (i < n) {
             uint32_t p = part;
-            for (; p + 3 * kLanes < count; p += 4 * kLanes) {
-                const float a = parts[p * n + i], b = parts[(p + kLanes) * n + i], c = parts[(p + 2 * kLanes) * n + i], d = parts[(p + 3 * kLanes) * n + i];
+            for (; p + 3 * kSumLanes < count; p += 4 * kSumLanes) {
+                const float a = parts[p * n + i], b = parts[(p + kSumLanes) * n + i], c = parts[(p + 2 * kSumLanes) * n + i], d = parts[(p + 3 * kSumLanes) * n + i];
                 sum += (a + b) + (c + d);
             }
-            for (; p < count; p += kLanes) sum += parts[p * n + i];
+            for (; p < count; p += kSumLanes) sum += parts[p * n + i];
         }
-        s_sum[part][lane] = sum;
+        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 8);
+        sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 16);
+        if ((threadIdx.x & 31u) < kSumCols) s_sum[threadIdx.x >> 5][col] = sum;
         __syncthreads();
-        if (part == 0 && i < n) {
+        if (threadIdx.x < kSumCols && i < n) {
+            float all = 0.f;
 #pragma unroll
-            for (uint32_t p = 1; p < kLanes; ++p) sum += s_sum[p][lane];
-            out[i] = sum;
+            for (uint32_t w = 0; w < kSumThreads / 32; ++w) all += s_sum[w][col];
+            out[i] = all;
         }
         __syncthreads();
     }
@@ -892,7 +1000,7 @@ void rms_norm_backward(const NormBackwardJob& j, float* workspace, cudaStream_t 
     else if (vecs <= 1024) whole ? go(k_rms_norm_backward<T, 2, 1, 512, true>) : go(k_rms_norm_backward<T, 2, 1, 512, false>);
     else whole ? go(k_rms_norm_backward<T, 2, 1, 1024, true>) : go(k_rms_norm_backward<T, 2, 1, 1024, false>);
     auto add_up = [&](const float* parts, uint32_t count, uint64_t n, float* out) {
-        launch_after(k_sum_parts, grid_for(n, 32, 4), kSumThreads, 0, s, parts, count, n, out);
+        launch_after(k_sum_parts, grid_for(n, kSumCols, 4), kSumThreads, 0, s, parts, count, n, out);
     };
     if (j.dweight) add_up(workspace, (uint32_t)workers, j.cols, j.dweight);
     if (d.by_image && d.parts > 1) add_up(r_parts, d.parts, j.period * j.cols, j.dresidual);
