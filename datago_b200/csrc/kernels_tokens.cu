@@ -291,26 +291,37 @@ template <class Out> struct PatchOut {
     bool whole;
 };
 
-// pixel bytes (four to a word) to values; the first is of channel `phase`.  2^23 + pixel, as a float, has the pixel in its low byte.
-template <int C>
-__device__ __forceinline__ void normalise16(const PatchView<C>& in, const uint32_t w[4], uint32_t phase, Pair v[8]) {
-    float g[C], b[C];
+// Gains and shifts of neighbouring features, two at a time, the first of them of channel `phase`.
+template <int C> struct Coefficients {
+    static constexpr int kPairs = C % 2 ? C : C / 2;  // after so many pairs they repeat
+    Pair gain[kPairs], shift[kPairs];
+    __device__ __forceinline__ Coefficients(const PatchView<C>& in, uint32_t phase) {
+        float g[C], b[C];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        g[c] = in.gain[c];
-        b[c] = in.shift[c];
+        for (int c = 0; c < C; ++c) {
+            g[c] = in.gain[c];
+            b[c] = in.shift[c];
 #pragma unroll
-        for (int k = 1; k < C; ++k)
-            if (phase == (uint32_t)k) { g[c] = in.gain[(c + k) % C]; b[c] = in.shift[(c + k) % C]; }
+            for (int k = 1; k < C; ++k)
+                if (phase == (uint32_t)k) { g[c] = in.gain[(c + k) % C]; b[c] = in.shift[(c + k) % C]; }
+        }
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+            gain[j] = pair_of(g[2 * j % C], g[(2 * j + 1) % C]);
+            shift[j] = pair_of(b[2 * j % C], b[(2 * j + 1) % C]);
+        }
     }
-    const Pair less = pair_of(-8388608.f, -8388608.f);
+    // pixel bytes, four to a word, to values.  2^23 + pixel, as a float, has the pixel in its low byte.
+    __device__ __forceinline__ void normalise(const uint32_t w[4], Pair v[8]) const {
+        const Pair less = pair_of(-8388608.f, -8388608.f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t word = w[j >> 1], at = 2 * (j & 1);
-        const Pair u = pair_of(__uint_as_float(__byte_perm(word, 0x4B000000u, 0x7650 + at)), __uint_as_float(__byte_perm(word, 0x4B000000u, 0x7651 + at)));
-        v[j] = fma2(add2(u, less), pair_of(g[(2 * j) % C], g[(2 * j + 1) % C]), pair_of(b[(2 * j) % C], b[(2 * j + 1) % C]));
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t word = w[j >> 1], at = 2 * (j & 1);
+            const Pair u = pair_of(__uint_as_float(__byte_perm(word, 0x4B000000u, 0x7650 + at)), __uint_as_float(__byte_perm(word, 0x4B000000u, 0x7651 + at)));
+            v[j] = fma2(add2(u, less), gain[j % kPairs], shift[j % kPairs]);
+        }
     }
-}
+};
 
 // Sixteen features of a row from `col` on, `valid` of them; all lanes of a warp are here.
 template <class Out>
@@ -354,31 +365,30 @@ __device__ __forceinline__ void store16(const PatchOut<Out>& out, uint64_t row, 
     }
 }
 
+constexpr uint32_t kAcross = 4;  // neighbouring patches whose features from `col` on a thread makes: their places and coefficients are found once
 template <int C, class Out>
-__global__ void __launch_bounds__(kRowThreads) k_patches(const PatchView<C> in, const PatchOut<Out> out, uint32_t items, Divisor per_row, Divisor grid_w, Divisor grid_h, Divisor segment) {
+__global__ void __launch_bounds__(kRowThreads) k_patches(const PatchView<C> in, const PatchOut<Out> out, uint32_t items, Divisor per_row, Divisor sets, Divisor grid_h, Divisor segment) {
     let_next_start();
     wait_for_previous();
     const uint8_t* const pixels = from_previous(in.pixels);
-    constexpr uint32_t kPieces = 2;  // of a thread under way
-    for (uint32_t i0 = blockIdx.x * kRowThreads * kPieces + threadIdx.x; (i0 & ~31u) < items; i0 += gridDim.x * kRowThreads * kPieces) {
-        uint32_t row[kPieces], col[kPieces], valid[kPieces];
-        uint4 w[kPieces];
+    for (uint32_t i0 = blockIdx.x * kRowThreads + threadIdx.x; (i0 & ~31u) < items; i0 += gridDim.x * kRowThreads) {
+        uint32_t col, set, Y, b;
+        const uint32_t band = sets.of(per_row.of(i0, col), set), i = grid_h.of(band, Y), x0 = set * kAcross;
+        col *= 16;
+        const uint32_t y = segment.of(col, b);
+        const uint32_t count = i0 < items && col < in.cols ? min(kAcross, in.grid_w - x0) : 0;
+        const uint8_t* const from = pixels + i * in.image + ((uint64_t)Y * in.patch + y) * in.pitch + (uint64_t)x0 * in.segment + b;
+        uint4 w[kAcross];
 #pragma unroll
-        for (uint32_t k = 0; k < kPieces; ++k) {
-            uint32_t X, Y, b;
-            row[k] = per_row.of(i0 + k * kRowThreads, col[k]);
-            const uint32_t i = grid_h.of(grid_w.of(row[k], X), Y);
-            col[k] *= 16;
-            const uint32_t y = segment.of(col[k], b);
-            valid[k] = i0 + k * kRowThreads < items && col[k] < in.cols ? 16 : 0;
-            w[k] = valid[k] ? *reinterpret_cast<const uint4*>(pixels + i * in.image + ((uint64_t)Y * in.patch + y) * in.pitch + (uint64_t)X * in.segment + b) : make_uint4(0, 0, 0, 0);
-        }
+        for (uint32_t k = 0; k < kAcross; ++k) w[k] = k < count ? *reinterpret_cast<const uint4*>(from + k * in.segment) : make_uint4(0, 0, 0, 0);
+        const Coefficients<C> by(in, C == 3 ? col % 3 : 0);  // 16 is a multiple of 1, 2 and 4
+        const uint64_t row = (uint64_t)band * in.grid_w + x0;
 #pragma unroll
-        for (uint32_t k = 0; k < kPieces; ++k) {
+        for (uint32_t k = 0; k < kAcross; ++k) {
             const uint32_t words[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
             Pair v[8];
-            normalise16<C>(in, words, C == 3 ? col[k] % 3 : 0, v);  // 16 is a multiple of 1, 2 and 4
-            store16(out, row[k], col[k], valid[k], v);
+            by.normalise(words, v);
+            store16(out, row + k, col, k < count ? 16 : 0, v);
         }
     }
 }
@@ -423,7 +433,7 @@ __global__ void __launch_bounds__(kRowThreads) k_patches_staged(const PatchView<
                 }
             }
             Pair v[8];
-            normalise16<C>(in, w, col % C, v);
+            Coefficients<C>(in, col % C).normalise(w, v);
             store16(out, (uint64_t)band * in.grid_w + x0 + x, col, valid, v);
         }
     }
@@ -451,8 +461,8 @@ void patches(const PatchJob& j, PatchOut<Out> out, cudaStream_t s) {
         to.data += i * per_image * out.ld;
         if (sizeof(Out) == 1) to.scales += i * per_image * out.scale_ld;
         if (straight) {
-            const uint32_t items = (uint32_t)(n * per_image * per_row);
-            launch_after(k_patches<C, Out>, grid_for(items, kRowThreads * 2, 32), kRowThreads, 0, s, in, to, items, Divisor(per_row), Divisor(in.grid_w), Divisor(grid_h), Divisor(in.segment));
+            const uint32_t sets = (in.grid_w + kAcross - 1) / kAcross, items = n * grid_h * sets * per_row;
+            launch_after(k_patches<C, Out>, grid_for(items, kRowThreads, 32), kRowThreads, 0, s, in, to, items, Divisor(per_row), Divisor(sets), Divisor(grid_h), Divisor(in.segment));
         } else {
             // patches of a strip: what the shared memory holds, but no more than spreads the work over the chip
             const uint32_t bands = n * grid_h, wanted = (uint32_t)std::max<uint64_t>(1, (uint64_t)bands * in.grid_w / (kSms * 8));
