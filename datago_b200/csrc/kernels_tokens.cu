@@ -7,6 +7,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 
 #include "kernels.h"
@@ -733,10 +734,200 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) k_rms_norm(co
     }
 }
 
+// ---- rows through shared memory -------------------------------------------------------------------------------------------
+// Rows of 16-bit elements that start at multiples of 16 bytes, up to 1280 of them: a warp per row, whose next row is copied into shared memory while it
+// works on this one (cp.async, sixteen bytes a lane; a lane reads what it has copied itself, so nothing but its own copies is waited for).  What is
+// under way then costs no registers, and half as many warps again fit as with rows waiting in registers.
+constexpr uint32_t kStagedCols = 1280;
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void end_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void await_all_copies_but_last() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+template <class T> __device__ __forceinline__ void staged_pairs(const T* at, Pair p[4]) {
+    Raw8<T> x;
+    x.w[0] = *reinterpret_cast<const uint4*>(at);
+    pairs_of(x, p);
+}
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// the weight as floats at the start of the dynamic shared memory
+__device__ __forceinline__ void stage_weight(float* to, const void* weight, int32_t dtype, uint32_t cols) {
+    for (uint32_t c = threadIdx.x; c < cols; c += blockDim.x)
+        to[c] = dtype == DG_F32 ? reinterpret_cast<const float*>(weight)[c] : dtype == DG_BF16 ? widen(reinterpret_cast<const bf16*>(weight)[c]) : widen(reinterpret_cast<const __half*>(weight)[c]);
+    __syncthreads();
+}
+__device__ __forceinline__ void scale_pairs(Pair p[4], const float* w) {
+    const ulonglong2 lo = reinterpret_cast<const ulonglong2*>(w)[0], hi = reinterpret_cast<const ulonglong2*>(w)[1];
+    p[0] = mul2(p[0], lo.x);
+    p[1] = mul2(p[1], lo.y);
+    p[2] = mul2(p[2], hi.x);
+    p[3] = mul2(p[3], hi.y);
+}
+
+constexpr uint32_t kStagedNormThreads = 384;
+// The last of a lane's V vectors may lie behind the row.
+template <class T, int V, bool RESIDUAL, bool WEIGHT>
+__global__ void __launch_bounds__(kStagedNormThreads, 2) k_rms_norm_staged(const NormJob a) {
+    extern __shared__ __align__(16) float s_staged[];
+    let_next_start();
+    wait_for_previous();
+    if (WEIGHT) stage_weight(s_staged, from_previous(a.weight), a.weight_dtype, a.cols);
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, vecs = a.cols / 8, warps = blockDim.x / 32;
+    const T *const px = from_previous(reinterpret_cast<const T*>(a.x)) + 8 * lane, *const pr = from_previous(reinterpret_cast<const T*>(a.residual)) + 8 * lane;
+    constexpr uint32_t kRows = RESIDUAL ? 2 : 1;  // rows of a stage
+    T* const ring = reinterpret_cast<T*>(s_staged + (WEIGHT ? a.cols : 0)) + (size_t)warp * 2 * kRows * a.cols + 8 * lane;
+    const float* const weight = s_staged + 8 * lane;
+    const bool last = lane + 32 * (V - 1) < vecs;
+    const float per_col = 1.f / (float)a.cols;
+    const uint64_t stride = (uint64_t)gridDim.x * warps;
+    uint64_t row = (uint64_t)blockIdx.x * warps + warp, rr = RESIDUAL ? row % a.residual_rows : 0;
+    const uint64_t rr_step = RESIDUAL ? stride % a.residual_rows : 0;
+    auto fetch = [&](uint64_t at, uint32_t stage) {
+        if (at < a.rows) {
+            const uint32_t to = shared_address(ring + stage * kRows * a.cols);
+            const T *const x = px + at * a.x_ld, *const r = pr + rr * a.residual_ld;
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (k + 1 < V || last) {
+                    copy16(to + 512 * k, x + 256 * k);
+                    if (RESIDUAL) copy16(to + 2 * a.cols + 512 * k, r + 256 * k);
+                }
+        }
+        end_copies();
+        if (RESIDUAL) {
+            rr += rr_step;
+            if (rr >= a.residual_rows) rr -= a.residual_rows;
+        }
+    };
+    fetch(row, 0);
+    for (uint32_t stage = 0; row < a.rows; row += stride, stage ^= 1u) {
+        fetch(row + stride, stage ^ 1u);
+        await_all_copies_but_last();
+        const T* const from = ring + stage * kRows * a.cols;
+        Pair h[V][4], sums = pair_of(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            if (k + 1 < V || last) {
+                staged_pairs(from + 256 * k, h[k]);
+                if (RESIDUAL) {
+                    Pair r[4];
+                    staged_pairs(from + a.cols + 256 * k, r);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) h[k][j] = add2(h[k][j], r[j]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[k][j] = pair_of(0.f, 0.f);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sums = fma2(h[k][j], h[k][j], sums);
+        float even, odd;
+        parts_of(sums, even, odd);
+        float sum = even + odd;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+        if (a.sum) {
+            T* const to = reinterpret_cast<T*>(a.sum) + row * a.sum_ld + 8 * lane;
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (k + 1 < V || last) {
+                    float f[8];
+                    floats_of(h[k], f);
+                    store8(to + 256 * k, 8, true, f);
+                }
+        }
+        const float rstd = 1.f / sqrtf(sum * per_col + a.eps);
+        if (lane == 0 && a.rstd) a.rstd[row] = rstd;
+        const Pair rstds = pair_of(rstd, rstd);
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (k + 1 < V || last) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[k][j] = mul2(h[k][j], rstds);
+                if (WEIGHT) scale_pairs(h[k], weight + 256 * k);
+            }
+        if (a.y) {
+            T* const to = reinterpret_cast<T*>(a.y) + row * a.y_ld + 8 * lane;
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (k + 1 < V || last) {
+                    float f[8];
+                    floats_of(h[k], f);
+                    store8(to + 256 * k, 8, true, f);
+                }
+        }
+        if (a.y8.values) {
+            uint32_t top[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                float largest = 0.f;
+                if (k + 1 < V || last) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) largest = larger2(largest, h[k][j]);
+                }
+                top[k] = magnitude(largest);
+            }
+#pragma unroll
+            for (int d = 8; d; d >>= 1)
+#pragma unroll
+                for (int k = 0; k < V; ++k) top[k] = max(top[k], __shfl_xor_sync(0xFFFFFFFFu, top[k], d));
+            uint8_t *const to = a.y8.values + row * a.y8.ld + 8 * lane, *const scales = a.y8.scales + row * a.y8.scale_ld + (lane >> 4);
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (k + 1 < V || last) {
+                    const uint32_t e = scale_byte(top[k]);
+                    const float inverse = inverse_scale(e);
+                    const Pair by = pair_of(inverse, inverse);
+                    *reinterpret_cast<uint2*>(to + 256 * k) = make_uint2(e4m3x4(mul2(h[k][0], by), mul2(h[k][1], by)), e4m3x4(mul2(h[k][2], by), mul2(h[k][3], by)));
+                    if ((lane & 15u) == 0) scales[2 * k] = (uint8_t)e;
+                }
+        }
+    }
+}
+
+// A kernel's dynamic shared memory beyond 48 KB, allowed once on every device.
+template <class K>
+cudaError_t allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t>& done) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = device >= 0 && device < 64 ? 1ull << device : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+constexpr uint32_t kStagedBytes = 115200;  // of a CTA, two to an SM
+
+template <class T, int V, bool RESIDUAL, bool WEIGHT>
+void rms_norm_staged(const NormJob& j, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    allow_smem(k_rms_norm_staged<T, V, RESIDUAL, WEIGHT>, kStagedBytes, done);
+    const uint32_t weight = WEIGHT ? j.cols * 4 : 0, each = (RESIDUAL ? 4 : 2) * j.cols * 2, warps = std::min(kStagedNormThreads / 32, (kStagedBytes - weight) / each);
+    launch_after(k_rms_norm_staged<T, V, RESIDUAL, WEIGHT>, grid_for(j.rows, warps, 2), warps * 32, weight + warps * each, s, j);
+}
+template <class T, int V>
+void rms_norm_staged(const NormJob& j, cudaStream_t s) {
+    if (j.residual) j.weight ? rms_norm_staged<T, V, true, true>(j, s) : rms_norm_staged<T, V, true, false>(j, s);
+    else j.weight ? rms_norm_staged<T, V, false, true>(j, s) : rms_norm_staged<T, V, false, false>(j, s);
+}
+
 template <class T>
 void rms_norm(const NormJob& j, cudaStream_t s) {
     const bool x_whole = rows_aligned<T>(j.x, j.x_ld), r_whole = rows_aligned<T>(j.residual, j.residual_ld), s_whole = rows_aligned<T>(j.sum, j.sum_ld),
                y_whole = rows_aligned<T>(j.y, j.y_ld), whole = x_whole && r_whole && s_whole && y_whole && j.cols % 8 == 0;
+    if constexpr (sizeof(T) == 2) {
+        if (whole && j.cols <= kStagedCols) {
+            switch ((j.cols + 255) / 256) {
+                case 1: return rms_norm_staged<T, 1>(j, s);
+                case 2: return rms_norm_staged<T, 2>(j, s);
+                case 3: return rms_norm_staged<T, 3>(j, s);
+                case 4: return rms_norm_staged<T, 4>(j, s);
+                default: return rms_norm_staged<T, 5>(j, s);
+            }
+        }
+    }
     auto go = [&](auto kernel, uint32_t threads, uint32_t rows_per_cta) {
         const size_t smem = j.weight ? (j.cols + 7) / 8 * 32 : 0;
         if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kNormMaxCols * 4));
