@@ -1252,6 +1252,8 @@ __global__ void __launch_bounds__(kRowThreads) k_dropout(const DropoutJob a, uin
     const T* const x = from_previous(reinterpret_cast<const T*>(a.x));
     T* const y = reinterpret_cast<T*>(a.y);
     const uint64_t step = (uint64_t)gridDim.x * kRowThreads * kDropoutVecs;
+    const Pair scales = pair_of(scale, scale);
+    const uint32_t least = a.threshold << 16;
     for (uint64_t i0 = (uint64_t)blockIdx.x * kRowThreads * kDropoutVecs + threadIdx.x; i0 < nvec; i0 += step) {
         uint64_t row[kDropoutVecs], col[kDropoutVecs];
         uint32_t valid[kDropoutVecs];
@@ -1275,12 +1277,15 @@ __global__ void __launch_bounds__(kRowThreads) k_dropout(const DropoutJob a, uin
             } else {
                 bits_of_8(index, a.seed, bits);
             }
+            Pair p[4];
+            pairs_of(raw[k], p);
             float v[8];
-            raw[k].widen(v);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t b = PER_ROW ? bits[0] & 0xFFFFu : j & 1 ? bits[j >> 1] >> 16 : bits[j >> 1] & 0xFFFFu;
-                v[j] = b >= a.threshold ? v[j] * scale : 0.f;
+            for (int j = 0; j < 4; ++j) {  // a half is compared where it is the upper one: what lies below it does not matter
+                const uint32_t lo = PER_ROW ? bits[0] << 16 : bits[j] << 16, hi = PER_ROW ? lo : bits[j];
+                parts_of(mul2(p[j], scales), v[2 * j], v[2 * j + 1]);
+                v[2 * j] = lo >= least ? v[2 * j] : 0.f;
+                v[2 * j + 1] = hi >= least ? v[2 * j + 1] : 0.f;
             }
             store8(y + row[k] * a.y_ld + col[k], valid[k], y_whole, v);
         }

@@ -19,36 +19,38 @@ ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t k, bool b_by_column) {
     constexpr uint32_t kPairs = kTokenSms / 2;
     const uint32_t groups = (uint32_t)scale_groups(k);
     p.tiles_m = (uint32_t)((m + kProductTileM - 1) / kProductTileM);
-    // Column tiles of one width, as wide as can be (with two accumulators while the contraction is short), or narrower so that more SMs have
-    // one; the contraction whole or in parts.  The cheapest by this measure: a pair takes a group of 128 in a time that goes with its tile's
-    // columns, but no less than that of 96, and as long as for four groups before and after a tile; parts are added up by a launch more.
+    // Column tiles of one width, as wide as can be (with two accumulators, or up to 256 columns with one), or narrower so that more SMs have one; the
+    // contraction whole or in parts.  The cheapest in cycles, by what was measured: a group of 128 takes two cycles a column, but no less than
+    // its bytes do at 39 a cycle and SM (that is 10 TB/s, where copies out of L2 end); a tile's sums 700 before and after it, or 150 where the
+    // next tile hides them; parts a launch more, and their bytes twice.
     uint64_t best = ~0ull;
     for (uint64_t want = (n + kProductMaxTileN - 1) / kProductMaxTileN;; want *= 2) {
         for (const uint32_t widest : {kProductMaxTileN, kProductTwoSums}) {
+            ProductPlan q = p;
             const uint64_t count = std::max<uint64_t>(want, (n + widest - 1) / widest);
-            const uint32_t tile_n = (uint32_t)((n + count - 1) / count + 31) / 32 * 32, tiles_n = (uint32_t)((n + tile_n - 1) / tile_n);
-            const uint64_t tiles = (uint64_t)p.tiles_m * tiles_n;
-            for (uint32_t s = 1; s <= 16 && (s == 1 || s * 8 <= groups); ++s) {
-                const uint32_t each = s == 1 ? groups : ((groups + s - 1) / s + 3) / 4 * 4;  // parts begin at multiples of four groups: the scales come in words
-                const uint64_t parts = (groups + each - 1) / each, rounds = (tiles * parts + kPairs - 1) / kPairs;
-                const uint64_t around = tile_n <= kProductTwoSums ? 256 + (rounds - 1) * 64 : rounds * 256;  // hidden behind the next tile, or not
-                const uint64_t cost = rounds * each * std::max(tile_n, 96u) + 4 * around + (parts > 1 ? 2048 : 0);
+            q.tile_n = (uint32_t)((n + count - 1) / count + 31) / 32 * 32;
+            q.tiles_n = (uint32_t)((n + q.tile_n - 1) / q.tile_n);
+            q.sums = q.tile_n <= kProductTwoSums ? 2 : 1;
+            const uint64_t tiles = (uint64_t)q.tiles_m * q.tiles_n;
+            const uint32_t b_bytes = (b_by_column ? 128 : q.tile_n / 2) * 128;
+            // The tensor cores cut what lies below their sums off: over 116 groups 1.4e-6 of a gradient of random terms was lost, over 44 3e-7.  Where
+            // there are few tiles, and parts are cheap, none is longer than 64.
+            for (uint32_t s = tiles <= kPairs ? std::min(16u, (groups + 63) / 64) : 1; s <= 16 && (s == 1 || s * 8 <= groups); ++s) {
+                q.split_groups = s == 1 ? groups : ((groups + s - 1) / s + 3) / 4 * 4;  // parts begin at multiples of four groups: the scales come in words
+                q.splits = (groups + q.split_groups - 1) / q.split_groups;
+                // a stays where its rows leave room for three slots of b and most pairs walk tiles of the same rows
+                q.a_stays = q.splits == 1 && groups <= 2 * kProductSlots && groups * kProductABytes + 3 * 2 * b_bytes <= kProductRingBytes && tiles >= 2 * kPairs && q.tiles_n > 1;
+                q.slots = std::min(kProductSlots, (kProductRingBytes - (q.a_stays ? groups * kProductABytes : 0)) / (2 * (b_bytes + (q.a_stays ? 0 : kProductABytes))));
+                const uint64_t rounds = (tiles * q.splits + kPairs - 1) / kPairs, group = std::max(2 * q.tile_n, (b_bytes + (q.a_stays ? 0 : kProductABytes)) / 39);
+                const uint64_t cost = rounds * q.split_groups * group + (q.sums == 2 ? 700 + (rounds - 1) * 150 : rounds * 700) + (q.splits > 1 ? 4000 + q.splits * m * n / 400 : 0);
                 if (cost < best) {
                     best = cost;
-                    p.tile_n = tile_n;
-                    p.tiles_n = tiles_n;
-                    p.splits = (uint32_t)parts;
-                    p.split_groups = each;
+                    p = q;
                 }
             }
         }
         if (p.tiles_m * want * 2 > kPairs || n / want <= 32) break;
     }
-    p.sums = p.tile_n <= kProductTwoSums ? 2 : 1;
-    // a stays where its rows leave room for three slots of b and most pairs walk tiles of the same rows
-    const uint32_t b_bytes = (b_by_column ? 128 : p.tile_n / 2) * 128;
-    p.a_stays = p.splits == 1 && groups <= 2 * kProductSlots && groups * kProductABytes + 3 * 2 * b_bytes <= kProductRingBytes && (uint64_t)p.tiles_m * p.tiles_n >= 2 * kPairs && p.tiles_n > 1;
-    p.slots = std::min(kProductSlots, (kProductRingBytes - (p.a_stays ? groups * kProductABytes : 0)) / (2 * (b_bytes + (p.a_stays ? 0 : kProductABytes))));
     return p;
 }
 
@@ -202,7 +204,7 @@ extern "C" int dg_quantize_rows(dg_ctx* ctx, void* stream, const dg_matrix* src,
 
 extern "C" uint64_t dg_product_workspace(dg_ctx* ctx, uint64_t m, uint64_t n, uint64_t k) {
     if (!ctx || m > kMostCols || n > kMostCols || k > kMostCols) return 0;
-    return product_workspace(plan_product(m, n, k), m, n);
+    return std::max(product_workspace(plan_product(m, n, k, false), m, n), product_workspace(plan_product(m, n, k, true), m, n));
 }
 
 extern "C" int dg_product(dg_ctx* ctx, void* stream, const dg_rows8* a, const dg_rows8* b, const dg_matrix* out, void* workspace,
@@ -218,7 +220,7 @@ extern "C" int dg_product(dg_ctx* ctx, void* stream, const dg_rows8* a, const dg
     ProductJob j{};
     j.plan = plan_product(a->rows, b->rows, a->cols, b->by_column != 0);
     if ((uint64_t)j.plan.tiles_m * j.plan.tiles_n * j.plan.splits > kMostCols) return fail(DG_E_TOO_LARGE, "more tiles than a launch can count");
-    if (int rc = check_workspace(workspace, workspace_bytes, product_workspace(j.plan, a->rows, b->rows))) return rc;
+    if (int rc = check_workspace(workspace, workspace_bytes, dg_product_workspace(ctx, a->rows, b->rows, a->cols))) return rc;
     const auto encode = (CUresult(*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                      const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill))encode_tiled_entry();
     if (!encode) return fail(DG_E_CUDA, "the driver has no cuTensorMapEncodeTiled");

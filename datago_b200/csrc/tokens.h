@@ -83,7 +83,7 @@ struct ProductPlan {
     uint32_t slots;                 // of 256 columns each, of the ring of b, and of a unless it stays
     bool a_stays;                   // all groups of a row of tiles have room
 };
-ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t k, bool b_by_column = false);
+ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t k, bool b_by_column);
 inline uint64_t product_part_ld(uint64_t n) { return (n + 3) / 4 * 4; }
 inline uint64_t product_workspace(const ProductPlan& p, uint64_t m, uint64_t n) {
     return p.splits > 1 ? (uint64_t)p.splits * m * product_part_ld(n) * 4 : 0;

@@ -7,10 +7,10 @@ static unsigned int gave_up = 0;
 extern "C" {
 int fake_launches() { int n = launches; launches = 0; return n; }
 void fake_gave_up(unsigned int n) { gave_up = n; }
-void fake_product_plan(uint64_t m, uint64_t n, uint64_t k, uint32_t out[6]) {
-    const dg::ProductPlan p = dg::plan_product(m, n, k);
-    const uint32_t v[6] = {p.tile_n, p.tiles_m, p.tiles_n, p.splits, p.split_groups, p.sums};
-    for (int i = 0; i < 6; ++i) out[i] = v[i];
+void fake_product_plan(uint64_t m, uint64_t n, uint64_t k, int b_by_column, uint32_t out[8]) {
+    const dg::ProductPlan p = dg::plan_product(m, n, k, b_by_column != 0);
+    const uint32_t v[8] = {p.tile_n, p.tiles_m, p.tiles_n, p.splits, p.split_groups, p.sums, p.slots, p.a_stays};
+    for (int i = 0; i < 8; ++i) out[i] = v[i];
 }
 void fake_backward_split(uint64_t rows, uint64_t cols, uint64_t period, int residual, uint32_t out[2]) {
     const dg::NormBackwardSplit d = dg::norm_backward_split(rows, cols, period, residual != 0);

@@ -210,15 +210,22 @@ def test_dropout_refuses(L, ctx):
 
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 48, 64), (7, 1024, 768), (128, 240, 128), (129, 241, 129), (200, 4801, 512), (1152, 768, 57600), (131072, 1152, 768),
                                    (37, 65, 1 << 20), (1 << 20, 16, 16), (5, 1 << 17, 640)])
-def test_product_plans_cover_the_output_and_the_contraction(L, m, n, k):
-    v = (C.c_uint32 * 6)()
-    L.fake_product_plan(C.c_uint64(m), C.c_uint64(n), C.c_uint64(k), v)
-    tile_n, tiles_m, tiles_n, splits, per_split, sums = v
+@pytest.mark.parametrize("b_by_column", [0, 1])
+def test_product_plans_cover_the_output_and_the_contraction(L, ctx, m, n, k, b_by_column):
+    v = (C.c_uint32 * 8)()
+    L.fake_product_plan(C.c_uint64(m), C.c_uint64(n), C.c_uint64(k), b_by_column, v)
+    tile_n, tiles_m, tiles_n, splits, per_split, sums, slots, a_stays = v
     groups = -(-k // 128)
     assert tile_n % 32 == 0 and 32 <= tile_n <= (256 if sums == 1 else 224)
     assert (tiles_m - 1) * 256 < m <= tiles_m * 256 and (tiles_n - 1) * tile_n < n <= tiles_n * tile_n
     assert splits == 1 or k > 1920  # what the binding counts on
     assert (splits == 1 or per_split % 4 == 0) and (splits - 1) * per_split < groups <= splits * per_split
+    # the rings fit what the kernel has for them, and work while something is under way
+    b_bytes = (128 if b_by_column else tile_n // 2) * 128
+    assert slots >= 2 and (groups * 16384 if a_stays else slots * 2 * 16384) + slots * 2 * b_bytes <= 192 * 1024
+    assert not a_stays or (splits == 1 and groups <= 12)
+    if splits > 1:
+        assert L.dg_product_workspace(ctx._h, m, n, k) >= splits * m * -(-n // 4) * 16
 
 
 @pytest.mark.parametrize("rows,cols,period,residual", [(1, 8, 1, 0), (1, 8, 1, 1), (100000, 1152, 1, 1), (55056, 1152, 2294, 1), (55056, 1152, 55056, 0), (64, 16384, 4, 1), (12, 300, 12, 1)])
