@@ -413,15 +413,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_produ
             const uint64_t row0 = (uint64_t)t.m0 + rows;
             const uint32_t live = row0 < j.m ? (uint32_t)min((uint64_t)32, j.m - row0) : 0;  // rows of this warp that the matrix has
             const uint32_t width = (uint32_t)min((uint64_t)tile_n, j.n - t.n0);
-            for (uint32_t c = 0; c < width; c += kPiece) {
-                uint32_t v[kPiece], w[16];
+            uint32_t v[kPiece], w[16];
+            auto read = [&](uint32_t c) {
 #pragma unroll
                 for (uint32_t k = 0; k < kPiece; k += 16) read_16(from + c + k, v + k);
+            };
+            read(0);
+            for (uint32_t c = 0; c < width; c += kPiece) {
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
                     if constexpr (sizeof(T) == 4) w[k] = v[k];
                     else w[k] = pair(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]), T());
+                }
+                // the next sums are on their way while these leave; after the last ones the accumulator is free
+                if (c + kPiece < width) read(c + kPiece);
+                else {
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(in_first_cta(sums_empty(sum.slot)));
                 }
                 const uint32_t piece = mine + room.slot * kOutBytes;
                 room.next(kPieces);
@@ -455,9 +465,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_produ
                     }
                 }
             }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) bar_arrive(in_first_cta(sums_empty(sum.slot)));
             sum.next(sums);
         }
         if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
