@@ -433,6 +433,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_produ
                     __syncwarp();
                     if (lane == 0) bar_arrive(in_first_cta(sums_empty(sum.slot)));
                 }
+                if (!live) continue;  // nothing leaves: what is still being read of the pieces stays as it is
                 const uint32_t piece = mine + room.slot * kOutBytes;
                 room.next(kPieces);
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kPieces - 1) : "memory");  // the piece that was here has left
@@ -444,7 +445,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_produ
                 if (by_map) {  // rows and columns outside the matrix are not written
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0 && live) store_box(&j.out_map, (int32_t)(t.n0 + c), (int32_t)row0, (int32_t)t.split, piece);
+                    if (lane == 0) store_box(&j.out_map, (int32_t)(t.n0 + c), (int32_t)row0, (int32_t)t.split, piece);
                 } else {  // two rows at a time, neighbouring lanes neighbouring words (or elements, of rows that do not begin at words)
                     __syncwarp();
                     T* const to = out + t.split * part_elements + row0 * ld + t.n0 + c;

@@ -54,36 +54,65 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
     return *reinterpret_cast<const uint32_t*>(&p);
 }
 
+// Eight 16-bit elements that start at an element: by words where they start at one, else by the half word before and behind three words.
+template <class T> __device__ __forceinline__ uint4 load_any(const T* p) {
+    if ((reinterpret_cast<uintptr_t>(p) & 2u) == 0) {
+        const uint32_t* const w = reinterpret_cast<const uint32_t*>(p);
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    const uint16_t* const h = reinterpret_cast<const uint16_t*>(p);
+    const uint32_t* const w = reinterpret_cast<const uint32_t*>(h + 1);
+    const uint32_t first = h[0], a = w[0], b = w[1], c = w[2], last = h[7];
+    return make_uint4(first | a << 16, a >> 16 | b << 16, b >> 16 | c << 16, c >> 16 | last << 16);
+}
+template <class T> __device__ __forceinline__ void store_any(T* p, const uint4& v) {
+    if ((reinterpret_cast<uintptr_t>(p) & 2u) == 0) {
+        uint32_t* const w = reinterpret_cast<uint32_t*>(p);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        return;
+    }
+    uint16_t* const h = reinterpret_cast<uint16_t*>(p);
+    uint32_t* const w = reinterpret_cast<uint32_t*>(h + 1);
+    h[0] = (uint16_t)v.x;
+    w[0] = v.x >> 16 | v.y << 16;
+    w[1] = v.y >> 16 | v.z << 16;
+    w[2] = v.z >> 16 | v.w << 16;
+    h[7] = (uint16_t)(v.w >> 16);
+}
 // Up to eight elements from p on (`valid` of them; the others are 0).  whole: p is 16-byte aligned.  Plain loads: what an earlier
 // kernel wrote is read.
 template <class T>
 __device__ __forceinline__ void load8(const T* p, uint32_t valid, bool whole, float v[8]) {
-    if (whole && valid >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            unpack8(*reinterpret_cast<const uint4*>(p), v, T());
+    if constexpr (sizeof(T) == 2) {
+        if (valid >= 8) {
+            unpack8(whole ? *reinterpret_cast<const uint4*>(p) : load_any(p), v, T());
+            return;
         }
-    } else {
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) v[j] = j < valid ? widen(p[j]) : 0.f;
+    } else if (whole && valid >= 8) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        return;
     }
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) v[j] = j < valid ? widen(p[j]) : 0.f;
 }
 template <class T>
 __device__ __forceinline__ void store8(T* p, uint32_t valid, bool whole, const float v[8]) {
-    if (whole && valid >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
+    if constexpr (sizeof(T) == 2) {
+        if (valid >= 8) {
+            const uint4 q = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
+            if (whole) *reinterpret_cast<uint4*>(p) = q;
+            else store_any(p, q);
+            return;
         }
-    } else {
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j)
-            if (j < valid) p[j] = narrow<T>(v[j]);
+    } else if (whole && valid >= 8) {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        return;
     }
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j)
+        if (j < valid) p[j] = narrow<T>(v[j]);
 }
 __device__ __forceinline__ void load8_any(const void* p, uint64_t at, int32_t dtype, uint32_t valid, bool whole, float v[8]) {
     if (dtype == DG_F32) load8(reinterpret_cast<const float*>(p) + at, valid, whole, v);
@@ -110,6 +139,8 @@ template <class T> struct Raw8 {  // eight neighbouring elements as they are in 
         if (whole && valid >= 8) {
 #pragma unroll
             for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else if (sizeof(T) == 2 && valid >= 8) {
+            w[0] = load_any(p);
         } else {
             T e[8];
 #pragma unroll

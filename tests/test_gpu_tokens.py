@@ -198,6 +198,15 @@ def test_product_of_more_tiles_than_the_chip_holds(ctx):
     check_product(ctx, operand(ctx, 20001, 200, 1, 5), operand(ctx, 1000, 200, 128, 6), BF16)
 
 
+def test_product_whose_last_tiles_are_partly_outside(ctx):
+    # a warp without rows in a tile follows, in the same CTA, one that has just sent its rows out
+    for m, n, k in ((20001, 1000, 200), (20033, 104, 300), (19000, 1000, 128)):
+        a, b = operand(ctx, m, k, 1, 15), operand(ctx, n, k, 128, 16)
+        first = check_product(ctx, a, b, BF16)
+        for _ in range(20):
+            assert torch.equal(tk.product(ctx, a, b, BF16), first)
+
+
 @pytest.mark.parametrize("dtype,lead,gap", [(BF16, 1, 3), (F32, 4, 4), (F16, 8, 16), (F32, 1, 0)])
 def test_product_into_rows_of_any_distance(ctx, dtype, lead, gap):
     for m, n, k in ((200, 250, 384), (70, 33, 9000)):
