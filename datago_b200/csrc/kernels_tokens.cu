@@ -428,10 +428,19 @@ __global__ void __launch_bounds__(kRowThreads) k_patches(const PatchView<C> in, 
 // Segments that are no multiple of sixteen bytes, or do not start at one: a CTA brings its patches' rows of pixels (up to `across` patches of a row of
 // patches) into shared memory first, word by word where the bytes begin at words, and gathers the features from there.
 constexpr uint32_t kStripBytes = 40 * 1024;
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// from any place in shared memory; up to three bytes on either side are read too
+__device__ __forceinline__ void sixteen_bytes(uint32_t at, uint32_t w[4]) {
+    uint32_t v[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[i]) : "r"((at & ~3u) + 4 * i));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(v[i], v[i + 1], 8 * (at & 3u));
+}
 
 template <int C, class Out>
 __global__ void __launch_bounds__(kRowThreads) k_patches_staged(const PatchView<C> in, const PatchOut<Out> out, uint32_t across, Divisor strips_x, Divisor grid_h, uint32_t strips,
-                                                                uint32_t strip_pitch) {
+                                                                uint32_t strip_pitch, Divisor per_patch, Divisor segment) {
     extern __shared__ __align__(16) uint8_t s_strip[];
     let_next_start();
     wait_for_previous();
@@ -451,12 +460,30 @@ __global__ void __launch_bounds__(kRowThreads) k_patches_staged(const PatchView<
             if (lane < bytes - head - 4 * words) to[head + 4 * words + lane] = p[head + 4 * words + lane];
         }
         __syncthreads();
-        const uint32_t per_patch = (in.cols + kScaleGroup - 1) / kScaleGroup * 8, items = count * per_patch;
+        const uint32_t items = count * per_patch.d;
         for (uint32_t k = threadIdx.x; (k & ~31u) < items; k += kRowThreads) {
-            const uint32_t x = k / per_patch, col = (k - x * per_patch) * 16, valid = k < items && col < in.cols ? min(16u, in.cols - col) : 0;
-            uint32_t y = col / in.segment, b = col - y * in.segment, w[4] = {};
+            uint32_t col, b, w[4] = {};
+            const uint32_t x = per_patch.of(k, col);
+            col *= 16;
+            const uint32_t valid = k < items && col < in.cols ? min(16u, in.cols - col) : 0;
+            uint32_t y = segment.of(col, b);
             auto line = [&] { return s_strip + y * strip_pitch + (uint32_t)((reinterpret_cast<uintptr_t>(from) + y * in.pitch) & 3u) + x * in.segment; };
-            if (valid) {
+            if (valid && in.segment >= 16) {
+                // sixteen bytes cross into the next row of pixels once at most: `here` of them are of this one, and the next one's are read from
+                // as far before its start as puts them behind those
+                const uint32_t here = min(16u, in.segment - b);
+                sixteen_bytes(shared_address(line() + b), w);
+                if (here < valid) {
+                    uint32_t next[4];
+                    ++y;
+                    sixteen_bytes(shared_address(line()) - here, next);
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const uint32_t mine = here >= 4 * j + 4 ? ~0u : here <= 4 * j ? 0u : (1u << (8 * (here - 4 * j))) - 1;
+                        w[j] = (w[j] & mine) | (next[j] & ~mine);
+                    }
+                }
+            } else if (valid) {
                 const uint8_t* q = line();
 #pragma unroll
                 for (uint32_t j = 0; j < 16; ++j) {
@@ -498,10 +525,11 @@ void patches(const PatchJob& j, PatchOut<Out> out, cudaStream_t s) {
         } else {
             // patches of a strip: what the shared memory holds, but no more than spreads the work over the chip
             const uint32_t bands = n * grid_h, wanted = (uint32_t)std::max<uint64_t>(1, (uint64_t)bands * in.grid_w / (kSms * 8));
-            const uint32_t across = std::max(1u, std::min({in.grid_w, (kStripBytes / j.patch - 8) / in.segment, std::max(wanted, 8u)}));
-            const uint32_t pitch = (across * in.segment + 3 + 7) / 4 * 4, strips_x = (in.grid_w + across - 1) / across;
-            launch_after(k_patches_staged<C, Out>, grid_for((uint64_t)bands * strips_x, 1, 16), kRowThreads, (size_t)pitch * j.patch, s, in, to, across, Divisor(strips_x), Divisor(grid_h),
-                         bands * strips_x, pitch);
+            const uint32_t most_across = std::max(1u, std::min({in.grid_w, (kStripBytes / j.patch - 8) / in.segment, std::max(wanted, 8u)}));
+            const uint32_t strips_x = (in.grid_w + most_across - 1) / most_across, across = (in.grid_w + strips_x - 1) / strips_x;
+            const uint32_t pitch = (across * in.segment + 3 + 7) / 4 * 4;
+            launch_after(k_patches_staged<C, Out>, grid_for((uint64_t)bands * strips_x, 1, 16), kRowThreads, (size_t)pitch * j.patch + 24, s, in, to, across, Divisor(strips_x), Divisor(grid_h),
+                         bands * strips_x, pitch, Divisor(per_row), Divisor(in.segment));
         }
     }
 }
@@ -778,7 +806,6 @@ template <class T> __device__ __forceinline__ void staged_pairs(const T* at, Pai
     x.w[0] = *reinterpret_cast<const uint4*>(at);
     pairs_of(x, p);
 }
-__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // the weight as floats at the start of the dynamic shared memory
 __device__ __forceinline__ void stage_weight(float* to, const void* weight, int32_t dtype, uint32_t cols) {
     for (uint32_t c = threadIdx.x; c < cols; c += blockDim.x)

@@ -171,7 +171,7 @@ extern "C" int dg_patch_rows(dg_ctx* ctx, void* stream, const uint8_t* pixels, u
     if (channels < 1 || channels > 4) return fail(DG_E_INVALID, "%u channels: 1 to 4 are wanted", channels);
     if (patch == 0 || patch > 4096 || h == 0 || w == 0 || h % patch || w % patch) return fail(DG_E_INVALID, "%u x %u pixels are no whole number of %u x %u patches", h, w, patch, patch);
     const uint64_t per_image = (uint64_t)(h / patch) * (w / patch), rows = n * per_image, cols = (uint64_t)patch * patch * channels;
-    if ((uint64_t)patch * (patch * channels + 11) > 48 * 1024) return fail(DG_E_TOO_LARGE, "patches of %u x %u x %u: at most 48 KB", patch, patch, channels);
+    if ((uint64_t)patch * (patch * channels + 11) > 48 * 1024 - 24) return fail(DG_E_TOO_LARGE, "patches of %u x %u x %u: at most 48 KB", patch, patch, channels);
     if (per_image > (1ull << 27) / scale_groups(cols)) return fail(DG_E_TOO_LARGE, "%u x %u pixels are too many for one image", h, w);
     if (n && !pixels) return fail(DG_E_INVALID, "pixels is NULL");
     if (out) {
