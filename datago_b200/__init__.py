@@ -558,10 +558,14 @@ class Batch:
         import torch
         from . import tokens
         bucket = self.buckets()[k]
-        own, current = torch.cuda.ExternalStream(self.ctx.stream, self.ctx.device), torch.cuda.current_stream(self.ctx.device)
-        current.wait_stream(own)
+        current = torch.cuda.current_stream(self.ctx.device)
+        own = torch.cuda.ExternalStream(self.ctx.stream, self.ctx.device) if self.ctx.stream else torch.cuda.default_stream(self.ctx.device)
+        apart = own.cuda_stream != current.cuda_stream
+        if apart:
+            current.wait_stream(own)
         rows = tokens.patch_rows(self.ctx, bucket["array"], patch, mean, std, dtype)
-        own.wait_stream(current)  # the batch's memory is handed on in the order of its own stream
+        if apart:
+            own.wait_stream(current)  # the batch's memory is handed on in the order of its own stream
         return rows
 
     def stage_ms(self):

@@ -151,6 +151,29 @@ int check_workspace(const void* p, uint64_t bytes, uint64_t needed) {
     return DG_OK;
 }
 
+// Where a matrix lies.  Two of them share memory unless their ranges are apart, or they are other columns of rows that are equally far apart.
+struct Lies {
+    uintptr_t at;
+    uint64_t rows, width, pitch;  // bytes
+};
+Lies lies(const dg_matrix* m) { return {(uintptr_t)m->data, m->rows, m->cols * element(m->dtype), m->ld * element(m->dtype)}; }
+Lies lies(const dg_rows8* r) { return r->by_column ? Lies{(uintptr_t)r->values, r->cols, r->rows, r->ld} : Lies{(uintptr_t)r->values, r->rows, r->cols, r->ld}; }
+bool share(const Lies& a, const Lies& b) {
+    if (!a.rows || !b.rows || !a.at || !b.at) return false;
+    if (a.at + (a.rows - 1) * a.pitch + a.width <= b.at || b.at + (b.rows - 1) * b.pitch + b.width <= a.at) return false;
+    if (a.pitch != b.pitch) return true;
+    const uint64_t apart = (b.at % a.pitch + a.pitch - a.at % a.pitch) % a.pitch;  // from the columns of a to those of b
+    return !(apart >= a.width && apart + b.width <= a.pitch);
+}
+// out may be in, where that is said of them, but not reach into it otherwise
+template <class A, class B>
+int check_apart(const A* out, const char* out_name, const B* in, const char* in_name, bool in_place = false) {
+    if (!out || !in) return DG_OK;
+    const Lies a = lies(out), b = lies(in);
+    if (in_place && a.at == b.at && (a.pitch == b.pitch || a.rows <= 1)) return DG_OK;
+    return share(a, b) ? fail(DG_E_INVALID, "%s overlaps %s", out_name, in_name) : DG_OK;
+}
+
 cudaStream_t stream_of(dg_ctx* ctx, void* stream) { return stream ? (cudaStream_t)stream : (cudaStream_t)dg_ctx_stream(ctx); }
 // Runs `launch` (which returns a cudaError_t or nothing) on the context's device.
 template <class F>
@@ -198,6 +221,7 @@ extern "C" int dg_quantize_rows(dg_ctx* ctx, void* stream, const dg_matrix* src,
     if (!out) return fail(DG_E_INVALID, "out is NULL");
     if (out->by_column && src->rows == 0) return fail(DG_E_INVALID, "the transpose of a matrix without rows has no columns");
     if (int rc = check_rows8_like(out, "out", out->by_column ? src->cols : src->rows, out->by_column ? src->rows : src->cols)) return rc;
+    if (int rc = check_apart(out, "out", src, "src")) return rc;
     if (src->rows == 0) return DG_OK;
     return launched(ctx, [&] { launch_quantize_rows(*src, *out, stream_of(ctx, stream)); });
 }
@@ -216,6 +240,8 @@ extern "C" int dg_product(dg_ctx* ctx, void* stream, const dg_rows8* a, const dg
     if (a->rows > kMostCols || b->rows == 0 || b->rows > kMostCols) return fail(DG_E_INVALID, "a has %llu rows, b %llu", (unsigned long long)a->rows, (unsigned long long)b->rows);
     if (int rc = check_matrix(out, "out")) return rc;
     if (out->rows != a->rows || out->cols != b->rows) return fail(DG_E_INVALID, "out: %llu x %llu elements wanted", (unsigned long long)a->rows, (unsigned long long)b->rows);
+    for (const dg_rows8* in : {a, b})
+        if (int rc = check_apart(out, "out", in, "an operand")) return rc;
     if (a->rows == 0) return DG_OK;
     ProductJob j{};
     j.plan = plan_product(a->rows, b->rows, a->cols, b->by_column != 0);
@@ -265,6 +291,9 @@ extern "C" int dg_product_status(dg_ctx* ctx, void* stream) {
     if (int rc = check_ctx(ctx)) return rc;
     OnDevice on(ctx_device(ctx));
     unsigned int count = 0;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (on.error == cudaSuccess && cudaStreamIsCapturing(stream_of(ctx, stream), &capture) == cudaSuccess && capture != cudaStreamCaptureStatusNone)
+        return fail(DG_E_INVALID, "the stream is being captured");
     const cudaError_t e = on.error != cudaSuccess ? on.error : product_gave_up(&count, stream_of(ctx, stream));
     if (e != cudaSuccess) return fail(DG_E_CUDA, "%s", cudaGetErrorString(e));
     return count ? fail(DG_E_SYNC_LIMIT, "%u CTAs of products gave up waiting for a copy", count) : DG_OK;
@@ -284,7 +313,6 @@ extern "C" int dg_rms_norm(dg_ctx* ctx, void* stream, const dg_matrix* x, const 
     if (!(eps >= 0) || !std::isfinite(eps)) return fail(DG_E_INVALID, "eps is finite and not below 0");
     if (sum) {
         if (int rc = check_like(sum, "sum", x->rows, x->cols, x->dtype)) return rc;
-        if (sum->data == x->data && sum->ld != x->ld) return fail(DG_E_INVALID, "sum: in place of x its rows are as far apart");
     }
     if (y) if (int rc = check_like(y, "y", x->rows, x->cols, x->dtype)) return rc;
     if (y8) {
@@ -293,6 +321,14 @@ extern "C" int dg_rms_norm(dg_ctx* ctx, void* stream, const dg_matrix* x, const 
     }
     if (int rc = check_floats(rstd, "rstd")) return rc;
     if (!sum && !y && !y8 && !rstd) return fail(DG_E_INVALID, "no output is wanted");
+    if (int rc = check_apart(sum, "sum", x, "x", true)) return rc;
+    if (int rc = check_apart(y, "y", sum, "sum")) return rc;
+    if (int rc = check_apart(y8, "y8", sum, "sum")) return rc;
+    for (const dg_matrix* in : {x, residual, weight}) {
+        if (int rc = in == x ? DG_OK : check_apart(sum, "sum", in, "an input")) return rc;
+        if (int rc = check_apart(y, "y", in, "an input")) return rc;
+        if (int rc = check_apart(y8, "y8", in, "an input")) return rc;
+    }
     if (x->rows == 0) return DG_OK;
     NormJob j{};
     j.rows = x->rows; j.cols = (uint32_t)x->cols; j.dtype = x->dtype; j.eps = eps;
@@ -323,8 +359,10 @@ extern "C" int dg_rms_norm_backward(dg_ctx* ctx, void* stream, const dg_matrix* 
     if (dsum) if (int rc = check_like(dsum, "dsum", dy->rows, dy->cols, dy->dtype)) return rc;
     if (dx) {
         if (int rc = check_like(dx, "dx", dy->rows, dy->cols, dy->dtype)) return rc;
-        if ((dx->data == dy->data && dx->ld != dy->ld) || (dsum && dx->data == dsum->data && dx->ld != dsum->ld))
-            return fail(DG_E_INVALID, "dx: in place of a gradient its rows are as far apart");
+        for (const dg_matrix* in : {dy, dsum})
+            if (int rc = check_apart(dx, "dx", in, "a gradient", true)) return rc;
+        for (const dg_matrix* in : {h, weight})
+            if (int rc = check_apart(dx, "dx", in, "h or weight")) return rc;
     }
     if (dy->rows && !rstd) return fail(DG_E_INVALID, "rstd is NULL");
     if (!dx && !dresidual && !dweight) return fail(DG_E_INVALID, "no output is wanted");
@@ -351,7 +389,7 @@ extern "C" int dg_dropout(dg_ctx* ctx, void* stream, const dg_matrix* x, double 
     if (int rc = check_ctx(ctx)) return rc;
     if (int rc = check_matrix(x, "x")) return rc;
     if (int rc = check_like(y, "y", x->rows, x->cols, x->dtype)) return rc;
-    if (x->data == y->data && x->rows > 1 && x->ld != y->ld) return fail(DG_E_INVALID, "y: in place of x its rows are as far apart");
+    if (int rc = check_apart(y, "y", x, "x", true)) return rc;
     const double t = p >= 0 && p < 1 ? std::floor(p * 65536 + 0.5) : 65536;
     if (t > 65535) return fail(DG_E_INVALID, "p is in [0, 1) and at most 65535 / 65536");
     if (offset + x->rows * (per_row ? 1 : x->cols) < offset) return fail(DG_E_INVALID, "offset: the indices pass 2^64");

@@ -344,7 +344,7 @@ DG_API void dg_host_release(void* block);
  * stream is cudaStreamLegacy), without allocating, waiting or copying, so they can be captured into a graph.  What they
  * read has to be complete on that stream, and their results are complete in its order.  Buffers are the caller's, workspaces too: two
  * calls (or captured graphs) that may run at the same time need workspaces of their own.  The calling thread's current device
- * is the same after the call.  Outputs may not overlap inputs unless an entry point says so.  With rows == 0 a call does
+ * is the same after the call.  Outputs may not overlap inputs or each other unless an entry point says so (matrices that do are refused).  With rows == 0 a call does
  * nothing (gradients of weights become zero). */
 enum { DG_F32 = 0, DG_BF16 = 1, DG_F16 = 2 };
 

@@ -488,6 +488,58 @@ def test_stem_reads_the_buckets_of_a_batch():
         b.patch_rows(0, 16, MEAN[:3], STD[:3])
 
 
+def test_a_batch_on_the_current_stream_hands_its_buckets_over():
+    rng = np.random.default_rng(9)
+    img = rng.integers(0, 256, (300, 400, 3), dtype=np.uint8)
+    for stream in (torch.cuda.Stream(), torch.cuda.default_stream()):
+        tfm = dg.Context(0, CFG, stream=stream.cuda_stream)
+        with torch.cuda.stream(stream):
+            with tfm.batch([img, img], flags=dg.BATCH_COLLATE) as b:
+                b.upload()
+                b.run()
+                rows = b.patch_rows(0, 16, MEAN[:3], STD[:3])
+                outs = b.download()
+                b.sync()
+            want = tk.patch_rows(tfm, torch.from_numpy(np.stack(outs)).cuda(), 16, MEAN[:3], STD[:3])
+            assert torch.equal(rows.values.view(torch.uint8), want.values.view(torch.uint8))
+
+
+def test_the_status_of_products_is_not_asked_for_inside_a_capture(ctx):
+    a, b = operand(ctx, 40, 256, 1, 97), operand(ctx, 30, 256, 1, 98)
+    want = tk.product(ctx, a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = tk.product(ctx, a, b)
+        with pytest.raises(dg.DatagoB200Error):
+            tk.product_status(ctx)
+    graph.replay()
+    assert torch.equal(got, want)
+    tk.product_status(ctx)
+
+
+def test_indices_beyond_32_bits(ctx):
+    # 4.6 G elements, 9.2 GB: the last rows of a large matrix are those of the rows alone
+    rows, cols, tail = 70001, 65536, 5
+    x = torch.full((rows, cols), 1.5, dtype=BF16, device="cuda")
+    x[-tail:] = rand((tail, cols), BF16, 99)
+    whole = tk.dropout(ctx, x, 0.25, 3, 7)
+    assert torch.equal(whole[-tail:], tk.dropout(ctx, x[-tail:], 0.25, 3, 7 + (rows - tail) * cols))
+    q = tk.quantize_rows(ctx, x)
+    same_rows8(tk.Rows8(q.values[-tail:], q.scales[-tail:]), x[-tail:].double(), 1)
+    del whole, q
+    narrow = x.view(-1, 1024)  # 4.48 M rows
+    last = tk.rms_norm(ctx, narrow, residual=narrow[:1])
+    alone = tk.rms_norm(ctx, narrow[-200:], residual=narrow[:1])
+    assert torch.equal(last.y[-200:], alone.y) and torch.equal(last.sum[-200:], alone.sum) and torch.equal(last.rstd[-200:], alone.rstd)
+    a = tk.quantize_rows(ctx, narrow[:, :128])
+    del last, x, narrow
+    b = operand(ctx, 640, 128, 128, 3)
+    out = tk.product(ctx, a, b)  # 2.87 G elements
+    part = tk.Rows8(a.values[-300:], a.scales[-300:])
+    assert torch.equal(out[-300:], tk.product(ctx, part, b))
+    tk.product_status(ctx)
+
+
 def test_a_captured_stem_replays_on_new_inputs(ctx):
     stem, weight, norm_weight = make_stem(ctx, BF16, width=200)
     pixels = torch.randint(0, 256, (2, 42, 28, 3), device="cuda", dtype=torch.uint8)

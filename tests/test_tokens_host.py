@@ -83,16 +83,21 @@ def test_a_planning_context_and_no_context_have_no_token_rows(L):
 def test_quantize_rows_refuses(L, ctx):
     call = lambda m, r: L.dg_quantize_rows(ctx._h, None, m, r)  # noqa: E731
     for m in BAD_MATRICES:
-        refused(L, call(m, rows8()))
+        refused(L, call(m, rows8(values=2 * AT)))
     for r in BAD_ROWS8:
-        refused(L, call(matrix(), r))
+        refused(L, call(matrix(data=3 * AT), r))
     refused(L, call(matrix(), rows8(by_column=1)))               # the transpose has 256 rows
     refused(L, call(matrix(), rows8(256, 4, by_column=1, ld=240)))
     refused(L, call(matrix(), rows8(256, 4, by_column=2)))
     refused(L, call(matrix(rows=0), rows8(256, 16, by_column=1)))
-    launched(L, call(matrix(), rows8()))
-    launched(L, call(matrix(), rows8(block=128)))
-    launched(L, call(matrix(ld=300), rows8(256, 4, by_column=1)))
+    far = 2 * AT
+    for r in (rows8(), rows8(values=AT + 512 * 3), rows8(values=AT - 512), rows8(256, 4, by_column=1, ld=512)):
+        refused(L, call(matrix(), r))                            # over the source
+    launched(L, call(matrix(), rows8(values=far)))
+    launched(L, call(matrix(), rows8(values=far, block=128)))
+    launched(L, call(matrix(ld=1024), rows8(values=AT + 512, ld=2048)))  # other columns of the same rows
+    refused(L, call(matrix(ld=1024), rows8(values=AT + 496, ld=2048)))
+    launched(L, call(matrix(ld=300), rows8(256, 4, by_column=1, values=far)))
     launched(L, call(matrix(rows=0, data=None), rows8(0, values=None, scales=None)), 0)
 
 
@@ -113,12 +118,14 @@ def test_patch_rows_refuses(L, ctx):
 
 
 def test_product_refuses(L, ctx):
-    def call(a=rows8(), b=rows8(8), out=matrix(4, 8), work=None, nbytes=0):
+    def call(a=rows8(), b=rows8(8), out=matrix(4, 8, data=3 * AT), work=None, nbytes=0):
         return L.dg_product(ctx._h, None, (a), (b), (out), work, nbytes)
     launched(L, call())
     launched(L, call(a=rows8(block=128), b=rows8(8, block=128)))
     launched(L, call(a=rows8(by_column=1), b=rows8(8, by_column=1)))
     launched(L, call(a=rows8(0, values=None, scales=None), out=matrix(0, 8, data=None)), 0)
+    refused(L, call(out=matrix(4, 8)))
+    refused(L, call(b=rows8(8, values=3 * AT + 16)))
     for r in BAD_ROWS8:
         refused(L, call(a=r))
         refused(L, call(b=r))
@@ -129,7 +136,7 @@ def test_product_refuses(L, ctx):
     refused(L, call(out=matrix(5, 8)))
     refused(L, call(out=matrix(4, 9)))
     # a long contraction of few rows is split, and its parts need room
-    a, b, out = rows8(64, 8192), rows8(64, 8192), matrix(64, 64)
+    a, b, out = rows8(64, 8192), rows8(64, 8192), matrix(64, 64, data=3 * AT)
     need = L.dg_product_workspace(ctx._h, 64, 64, 8192)
     assert need >= 2 * 64 * 64 * 4
     refused(L, call(a, b, out))
@@ -151,7 +158,10 @@ def test_rms_norm_refuses(L, ctx):
     def call(x=matrix(), residual=None, weight=None, eps=1e-6, sum=None, y=out, y8=None, rstd=None):
         return L.dg_rms_norm(ctx._h, None, (x), (residual), (weight), eps, (sum), (y), (y8), rstd)
     launched(L, call())
-    launched(L, call(residual=matrix(2), weight=matrix(1, dtype=0), sum=matrix(), y=None, y8=rows8(), rstd=AT))
+    launched(L, call(residual=matrix(2, data=3 * AT), weight=matrix(1, dtype=0, data=4 * AT), sum=matrix(), y=None, y8=rows8(values=5 * AT), rstd=AT))
+    for bad in (dict(sum=matrix(data=AT + 512)), dict(y=matrix()), dict(y8=rows8()), dict(sum=matrix(data=3 * AT), y8=rows8(values=3 * AT)), dict(sum=matrix(), residual=matrix(2, data=AT + 512)),
+                dict(y=matrix(data=3 * AT), sum=matrix(data=3 * AT))):
+        refused(L, call(**bad))
     launched(L, call(x=matrix(0, data=None), y=matrix(0, data=None)), 0)
     for m in BAD_MATRICES:
         refused(L, call(x=m))
@@ -173,7 +183,7 @@ def test_rms_norm_backward_refuses(L, ctx):
     need = L.dg_rms_norm_backward_workspace(ctx._h, 4, 256, 2)
     assert need > 0
 
-    def call(dy=matrix(), h=matrix(), rstd=AT, weight=None, dsum=None, dx=matrix(), dr=AT, period=2, dw=AT, work=AT, nbytes=need):
+    def call(dy=matrix(), h=matrix(data=4 * AT), rstd=AT, weight=None, dsum=None, dx=matrix(), dr=AT, period=2, dw=AT, work=AT, nbytes=need):
         return L.dg_rms_norm_backward(ctx._h, None, (dy), (h), rstd, (weight), (dsum), (dx), dr, period, dw, work, nbytes)
     launched(L, call())
     launched(L, call(dx=None, dr=None, period=7))
@@ -186,7 +196,7 @@ def test_rms_norm_backward_refuses(L, ctx):
             refused(L, call(dsum=m))
             refused(L, call(dx=m))
     for bad in (dict(rstd=None), dict(rstd=AT + 2), dict(dr=AT + 2), dict(dw=AT + 2), dict(period=0), dict(period=3), dict(weight=matrix(2)), dict(h=matrix(dtype=0)),
-                dict(dx=matrix(ld=512)), dict(dsum=matrix(data=3 * AT, ld=512), dx=matrix(data=3 * AT)), dict(dx=None, dr=None, dw=None), dict(work=None), dict(nbytes=need - 1), dict(work=AT + 4)):
+                dict(dx=matrix(ld=512)), dict(dsum=matrix(data=3 * AT, ld=512), dx=matrix(data=3 * AT)), dict(dx=matrix(data=4 * AT)), dict(dx=matrix(data=AT + 512)), dict(dx=None, dr=None, dw=None), dict(work=None), dict(nbytes=need - 1), dict(work=AT + 4)):
         refused(L, call(**bad))
     wide = matrix(cols=16392, ld=16392)
     refused(L, call(wide, wide, dx=wide), TOO_LARGE)
