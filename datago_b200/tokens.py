@@ -24,6 +24,8 @@ GROUP = 128         # columns that share a scale
 _matrix_desc = struct.Struct("QQQQiI").pack  # data, rows, cols, ld, dtype
 _rows8_desc = struct.Struct("QQQQQQII").pack  # values, scales, rows, cols, ld, scale_ld, block
 
+_floats = [struct.Struct(f"{n}f").pack for n in range(1, 5)]
+
 _lib = None
 
 
@@ -101,11 +103,6 @@ def _on_device(ctx, t, name):
         raise _invalid(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
 
 
-def _new(shape, dtype, like):
-    """torch.empty, in two thirds of its time"""
-    return torch.empty_strided(shape, (shape[1], 1) if len(shape) == 2 else (1,), dtype=dtype, device=like.device)
-
-
 def _matrix(ctx, t, name):
     _on_device(ctx, t, name)
     dtype, shape = _DTYPES.get(t.dtype), t.shape
@@ -160,12 +157,23 @@ def _rows8(ctx, r, name, transposed=None):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _out(out, shape, dtype, like, name):
+def _out(ctx, out, rows, cols, dtype, like, name):
+    """A result and its descriptor: a new matrix, or the caller's"""
     if out is None:
-        return _new(shape, dtype, like)
-    if not isinstance(out, torch.Tensor) or tuple(out.shape) != tuple(shape) or out.dtype != dtype:
-        raise _invalid(f"{name}: a tensor {tuple(shape)} of {dtype} is wanted")
-    return out
+        out = torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=like.device)
+        return out, _matrix_desc(out.data_ptr(), rows, cols, cols, _DTYPES[dtype], 0)
+    if not isinstance(out, torch.Tensor) or out.shape != (rows, cols) or out.dtype != dtype:
+        raise _invalid(f"{name}: a tensor ({rows}, {cols}) of {dtype} is wanted")
+    return out, _matrix(ctx, out, name)
+
+
+def _new_rows8(rows, cols, like):
+    """Rows8.empty and its descriptor"""
+    groups = -(-cols // GROUP)
+    ld, scale_ld, device = -(-cols // 16) * 16, -(-groups // 4) * 4, like.device
+    values = torch.empty_strided((rows, cols), (ld, 1), dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty_strided((rows, groups), (scale_ld, 1), dtype=torch.float8_e8m0fnu, device=device)
+    return Rows8(values, scales), _rows8_desc(values.data_ptr(), scales.data_ptr(), rows, cols, ld, scale_ld, 1, 0)
 
 
 def _workspace(nbytes, like):
@@ -190,16 +198,18 @@ def patch_rows(ctx, pixels, patch, mean, std, dtype=None, out=None):
     patch = int(patch)
     if patch < 1 or h % patch or w % patch or h == 0 or w == 0:
         raise _invalid(f"{h} x {w} pixels are no whole number of {patch} x {patch} patches")
-    shape = (n * (h // patch) * (w // patch), patch * patch * c)
+    rows, cols = n * (h // patch) * (w // patch), patch * patch * c
+    desc8 = desc = None
     if dtype is None:
-        out = Rows8.empty(*shape, pixels.device) if out is None else out
-        desc8, desc = _rows8(ctx, out, "out"), None
+        if out is None:
+            out, desc8 = _new_rows8(rows, cols, pixels)
+        else:
+            desc8 = _rows8(ctx, out, "out")
     else:
         if dtype not in _DTYPES:
             raise _invalid("dtype: float32, bfloat16 or float16 is wanted")
-        out = _out(out, shape, dtype, pixels, "out")
-        desc8, desc = None, _matrix(ctx, out, "out")
-    floats = C.c_float * c
+        out, desc = _out(ctx, out, rows, cols, dtype, pixels, "out")
+    floats = _floats[c - 1] if c <= 4 else struct.Struct(f"{c}f").pack
     _check(lib().dg_patch_rows(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, pixels.data_ptr(), n, h, w, c, patch, floats(*mean), floats(*std),
                                desc8, desc))
     return out
@@ -224,11 +234,11 @@ def product(ctx, a, b, dtype=torch.bfloat16, out=None):
     if dtype not in _DTYPES:
         raise _invalid("dtype: float32, bfloat16 or float16 is wanted")
     (m, k), n = a.values.shape, b.values.shape[0]
-    out = _out(out, (m, n), dtype, a.values, "out")
+    out, desc = _out(ctx, out, m, n, dtype, a.values, "out")
     L = lib()
     nbytes = L.dg_product_workspace(ctx._h, m, n, k) if k > 1920 else 0
     work, at = _workspace(nbytes, out)
-    _check(L.dg_product(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, da, db, _matrix(ctx, out, "out"), at, nbytes))
+    _check(L.dg_product(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, da, db, desc, at, nbytes))
     return out
 
 
@@ -244,16 +254,14 @@ def rms_norm(ctx, x, weight=None, residual=None, eps=1e-6, eight_bit=False, sum_
     rows, cols = x.shape
     w = _vector(ctx, weight, "weight", cols)
     r = None if residual is None else _matrix(ctx, residual, "residual")
-    total = _out(sum_out, (rows, cols), x.dtype, x, "sum_out")
-    rstd = _new((rows,), torch.float32, x)
+    total, total_desc = _out(ctx, sum_out, rows, cols, x.dtype, x, "sum_out")
+    rstd = torch.empty_strided((rows,), (1,), dtype=torch.float32, device=x.device)
     y16 = y8 = None
     if eight_bit:
-        y = Rows8.empty(rows, cols, x.device)
-        y8 = _rows8(ctx, y, "y")
+        y, y8 = _new_rows8(rows, cols, x)
     else:
-        y = _new((rows, cols), x.dtype, x)
-        y16 = _matrix(ctx, y, "y")
-    _check(lib().dg_rms_norm(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, src, r, w, eps, _matrix(ctx, total, "sum_out"), y16, y8, rstd.data_ptr()))
+        y, y16 = _out(ctx, None, rows, cols, x.dtype, x, "y")
+    _check(lib().dg_rms_norm(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, src, r, w, eps, total_desc, y16, y8, rstd.data_ptr()))
     return Norm(y, total, rstd)
 
 
@@ -267,16 +275,16 @@ def rms_norm_backward(ctx, dy, h, rstd, weight=None, dsum=None, residual_rows=No
     _on_device(ctx, rstd, "rstd")
     if rstd.dtype != torch.float32 or rstd.numel() != rows or not rstd.is_contiguous():
         raise _invalid(f"rstd: {rows} neighbouring float32 are wanted")
-    dx = _out(dx_out, (rows, cols), dy.dtype, dy, "dx_out")
+    dx, dx_desc = _out(ctx, dx_out, rows, cols, dy.dtype, dy, "dx_out")
     period = int(residual_rows or 0)
     if residual_rows is not None and (period < 1 or rows % period):
         raise _invalid(f"{residual_rows} residual rows do not divide {rows}")
-    dweight = _new((cols,), torch.float32, dy)
-    dresidual = _new((period, cols), torch.float32, dy) if period else None
+    dweight = torch.empty_strided((cols,), (1,), dtype=torch.float32, device=dy.device)
+    dresidual = torch.empty_strided((period, cols), (cols, 1), dtype=torch.float32, device=dy.device) if period else None
     L = lib()
     nbytes = L.dg_rms_norm_backward_workspace(ctx._h, rows, cols, period)
     work, at = _workspace(nbytes, dy)
-    _check(L.dg_rms_norm_backward(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, g, hm, rstd.data_ptr(), w, s, _matrix(ctx, dx, "dx_out"),
+    _check(L.dg_rms_norm_backward(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, g, hm, rstd.data_ptr(), w, s, dx_desc,
                                   dresidual.data_ptr() if period else None, period, dweight.data_ptr(), at, nbytes))
     return dx, dresidual, dweight
 
@@ -285,11 +293,11 @@ def dropout(ctx, x, p, seed, offset=0, per_row=False, out=None):
     """x with elements (or, per_row, rows) dropped with probability p and the others scaled up.  The mask is a function of (seed, offset + index):
     the same call on the gradient is the backward pass.  out may be x."""
     src = _matrix(ctx, x, "x")
-    out = _out(out, x.shape, x.dtype, x, "out")
+    out, desc = _out(ctx, out, *x.shape, x.dtype, x, "out")
     seed, offset = int(seed), int(offset)
     if not 0 <= seed < 1 << 64 or not 0 <= offset < 1 << 64:
         raise _invalid("seed and offset are in [0, 2^64)")
-    _check(lib().dg_dropout(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, src, p, seed, offset, per_row, _matrix(ctx, out, "out")))
+    _check(lib().dg_dropout(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, src, p, seed, offset, per_row, desc))
     return out
 
 
@@ -310,7 +318,7 @@ class PatchStem:
         self.weight8 = quantize_rows(self.ctx, weight, block=GROUP)
 
     def forward(self, pixels, positions, offset=0):
-        """(Norm with Rows8 for the first layer, what backward wants).  positions: [tokens of an image, width].  offset: where this batch's
+        """(Norm with Rows8 for the first layer, what backward wants).  positions: [tokens of an image, width] of the stem's dtype.  offset: where this batch's
         elements begin in the run's count (see dropout)."""
         if isinstance(pixels, DeviceArray):
             pixels = torch.as_tensor(pixels, device=f"cuda:{self.ctx.device}")
