@@ -547,13 +547,12 @@ void patch_rows(const PatchJob& j, const dg_rows8* out8, const dg_matrix* out, c
 }
 
 // ---- scales along the rows of the source, and of 128 x 128 blocks -------------------------------------------------------------
-// The transpose of a matrix stays in the order of the matrix (dg_rows8.by_column): only its scales run along the rows.  A warp holds 256 columns
-// of ROWS rows as they were loaded; the warps of a CTA have 128 rows, the group of a scale, and meet twice over its 256 columns' maxima.
+// The transpose of a matrix stays in the order of the matrix (dg_rows8.by_column): only its scales run along the rows.  A CTA holds 128 x 128 elements
+// as they were loaded, a thread eight rows of eight columns, and meets twice over its columns' maxima.
 // 37003 x 1000 bf16: 26 us, 4.3 TB/s; two CTAs of 128 registers a thread fit an SM, and each waits for its loads once (transposing the values
 // through shared memory as well took 46).
-template <class T> constexpr int kColumnRows = sizeof(T) == 4 ? 8 : 16;  // what fits the registers
-template <class T> constexpr uint32_t kColumnThreads = 128 / kColumnRows<T> * 32;
-constexpr uint32_t kColumnTile = 256;
+constexpr uint32_t kColumnThreads = 256, kColumnTile = 128;
+constexpr int kColumnRows = 8;  // of a thread
 
 // Magnitudes of two 16-bit elements compared at once: like those of 32 bits, they order as whole numbers.
 __device__ __forceinline__ uint32_t larger(uint32_t top, uint32_t v, bf16) { return __vmaxu2(top, v & 0x7FFF7FFFu); }
@@ -566,17 +565,18 @@ __device__ __forceinline__ uint32_t magnitude_of(uint32_t half, __half) { return
 // BLOCK: one scale for 128 columns too.  scale_row / scale_col: how far apart the scales of neighbouring groups of rows and of neighbouring
 // columns (blocks of 128 columns) are.
 template <class T, bool BLOCK>
-__global__ void __launch_bounds__(kColumnThreads<T>, 2) k_columns8(const T* src, uint64_t rows, uint64_t cols, uint64_t ld, bool whole, uint32_t tiles_x, uint64_t tiles,
-                                                                   uint8_t* values, uint64_t out_ld, uint8_t* scales, uint64_t scale_row, uint64_t scale_col) {
-    constexpr int R = kColumnRows<T>, kWarps = 128 / R, kWords = sizeof(T) * 2;
-    __shared__ __align__(16) uint32_t s_top[kWarps][32][kWords];
+__global__ void __launch_bounds__(kColumnThreads, sizeof(T) == 4 ? 2 : 4) k_columns8(const T* src, uint64_t rows, uint64_t cols, uint64_t ld, bool whole, uint32_t tiles_x, uint64_t tiles,
+                                                                                     uint8_t* values, uint64_t out_ld, uint8_t* scales, uint64_t scale_row, uint64_t scale_col) {
+    constexpr int R = kColumnRows, kWarps = kColumnThreads / 32, kWords = sizeof(T) * 2;
+    __shared__ __align__(16) uint32_t s_top[kWarps][16][kWords];
     __shared__ __align__(16) float s_inverse[kColumnTile];
+    __shared__ uint32_t s_warp[kColumnTile / 32];
     let_next_start();
     wait_for_previous();
     src = from_previous(src);
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t cv = threadIdx.x & 15u, warp = threadIdx.x >> 5, first = (threadIdx.x >> 4) * R;  // eight columns from 8 cv, R rows from `first`
     for (uint64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const uint64_t ty = tile / tiles_x, c0 = (tile - ty * tiles_x) * kColumnTile, col = c0 + 8 * lane, r0 = ty * 128 + warp * R;
+        const uint64_t ty = tile / tiles_x, c0 = (tile - ty * tiles_x) * kColumnTile, col = c0 + 8 * cv, r0 = ty * 128 + first;
         const uint32_t valid = col < cols ? (uint32_t)min((uint64_t)8, cols - col) : 0;
         Raw8<T> x[R];
 #pragma unroll
@@ -592,9 +592,13 @@ __global__ void __launch_bounds__(kColumnThreads<T>, 2) k_columns8(const T* src,
                 top[4 * k + 3] = larger(top[4 * k + 3], x[i].w[k].w, T());
             }
 #pragma unroll
-        for (int k = 0; k < kWords / 4; ++k) *reinterpret_cast<uint4*>(&s_top[warp][lane][4 * k]) = make_uint4(top[4 * k], top[4 * k + 1], top[4 * k + 2], top[4 * k + 3]);
+        for (int k = 0; k < kWords; ++k) top[k] = larger(top[k], __shfl_xor_sync(0xFFFFFFFFu, top[k], 16), T());  // the warp's other rows
+        if ((threadIdx.x & 16u) == 0)
+#pragma unroll
+            for (int k = 0; k < kWords / 4; ++k) *reinterpret_cast<uint4*>(&s_top[warp][cv][4 * k]) = make_uint4(top[4 * k], top[4 * k + 1], top[4 * k + 2], top[4 * k + 3]);
         __syncthreads();
-        for (uint32_t c = threadIdx.x; c < kColumnTile; c += kColumnThreads<T>) {  // a thread per column
+        if (threadIdx.x < kColumnTile) {  // a thread per column
+            const uint32_t c = threadIdx.x;
             uint32_t m = 0;
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -604,31 +608,30 @@ __global__ void __launch_bounds__(kColumnThreads<T>, 2) k_columns8(const T* src,
                 for (int w = 0; w < kWarps; ++w) m = max(m, s_top[w][c >> 3][(c & 7u) >> 1] >> (16 * (c & 1u)) & 0xFFFFu);
                 m = magnitude_of(m, T());
             }
-            if constexpr (BLOCK) {  // 128 columns are four whole warps
+            if constexpr (BLOCK) {
                 m = __reduce_max_sync(0xFFFFFFFFu, m);
-                __shared__ uint32_t s_warp[kColumnTile / 32];
-                if (lane == 0) s_warp[c >> 5] = m;
-                asm volatile("bar.sync 1, 256;" ::: "memory");  // the 256 threads that are here
-                const uint32_t first = c >> 7 << 2;
-                m = max(max(s_warp[first], s_warp[first + 1]), max(s_warp[first + 2], s_warp[first + 3]));
-                if ((c & 127u) == 0 && c0 + c < cols) scales[ty * scale_row + (c0 + c) / 128 * scale_col] = (uint8_t)scale_byte(m);
+                if ((c & 31u) == 0) s_warp[warp] = m;
+                asm volatile("bar.sync 1, 128;" ::: "memory");  // the threads that are here
+                m = max(max(s_warp[0], s_warp[1]), max(s_warp[2], s_warp[3]));
+                if (c == 0) scales[ty * scale_row + c0 / 128 * scale_col] = (uint8_t)scale_byte(m);
             } else if (c0 + c < cols) {
                 scales[ty * scale_row + (c0 + c) * scale_col] = (uint8_t)scale_byte(m);
             }
             s_inverse[c] = inverse_scale(scale_byte(m));
         }
         __syncthreads();
-        float inverse[8];
-        *reinterpret_cast<float4*>(inverse) = *reinterpret_cast<const float4*>(&s_inverse[8 * lane]);
-        *reinterpret_cast<float4*>(inverse + 4) = *reinterpret_cast<const float4*>(&s_inverse[8 * lane + 4]);
+        Pair inverse[4];
+        {
+            const ulonglong2 *const p = reinterpret_cast<const ulonglong2*>(&s_inverse[8 * cv]), lo = p[0], hi = p[1];
+            inverse[0] = lo.x; inverse[1] = lo.y; inverse[2] = hi.x; inverse[3] = hi.y;
+        }
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             if (!valid || r0 + i >= rows) continue;
-            float v[8];
-            x[i].widen(v);
+            Pair v[4];
+            pairs_of(x[i], v);
             store_values8(values + (r0 + i) * out_ld + col, valid,
-                          make_uint2(e4m3x4(v[0] * inverse[0], v[1] * inverse[1], v[2] * inverse[2], v[3] * inverse[3]),
-                                     e4m3x4(v[4] * inverse[4], v[5] * inverse[5], v[6] * inverse[6], v[7] * inverse[7])));
+                          make_uint2(e4m3x4(mul2(v[0], inverse[0]), mul2(v[1], inverse[1])), e4m3x4(mul2(v[2], inverse[2]), mul2(v[3], inverse[3]))));
         }
     }
 }
@@ -643,7 +646,7 @@ void quantize_rows(const dg_matrix& m, const dg_rows8& out, cudaStream_t s) {
     const uint32_t tiles_x = (uint32_t)((m.cols + kColumnTile - 1) / kColumnTile);
     const uint64_t tiles = scale_groups(m.rows) * tiles_x;
     auto go = [&](auto kernel) {
-        launch_after(kernel, grid_for(tiles, 1, 32), kColumnThreads<T>, 0, s, (const T*)m.data, m.rows, m.cols, m.ld, whole, tiles_x, tiles, out.values, out.ld,
+        launch_after(kernel, grid_for(tiles, 1, 32), kColumnThreads, 0, s, (const T*)m.data, m.rows, m.cols, m.ld, whole, tiles_x, tiles, out.values, out.ld,
                      out.scales, out.by_column ? 1 : out.scale_ld, out.by_column ? out.scale_ld : 1);
     };
     if (out.block == 1) go(k_columns8<T, false>);
