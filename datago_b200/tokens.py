@@ -2,8 +2,10 @@
 include/datago_b200.h), on torch tensors.
 
 Every function takes the Context of the tensors' device first, launches on torch's current stream of that device and returns
-without waiting; nothing is kept between calls, so calls can be captured into CUDA graphs.  Results are new tensors unless `out` is given.
-Matrices are 2-d tensors of float32, bfloat16 or float16 whose columns are neighbours in memory; rows may be any distance apart.
+without waiting; nothing is kept between calls, so calls can be captured into CUDA graphs.  Results are new tensors unless `out` is given; the
+rows of new ones (dropout's apart) begin at multiples of 16 bytes, so those whose rows are no multiple of that long are not contiguous (a product of
+124515 x 685 in bfloat16 then takes 71 us, into contiguous rows 171).  Matrices are 2-d tensors of float32, bfloat16 or float16 whose columns
+are neighbours in memory; their rows, those of `out` too, may be any distance apart.
 Gradients are calls of their own (rms_norm_backward, dropout on the gradient, product on operands quantised along the contraction);
 PatchStem puts them together for the stem of a model.
 """
@@ -160,8 +162,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda de
 def _out(ctx, out, rows, cols, dtype, like, name):
     """A result and its descriptor: a new matrix, or the caller's"""
     if out is None:
-        out = torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=like.device)
-        return out, _matrix_desc(out.data_ptr(), rows, cols, cols, _DTYPES[dtype], 0)
+        ld = (cols + 3) // 4 * 4 if dtype is torch.float32 else (cols + 7) // 8 * 8
+        out = torch.empty_strided((rows, cols), (ld, 1), dtype=dtype, device=like.device)
+        return out, _matrix_desc(out.data_ptr(), rows, cols, ld, _DTYPES[dtype], 0)
     if not isinstance(out, torch.Tensor) or out.shape != (rows, cols) or out.dtype != dtype:
         raise _invalid(f"{name}: a tensor ({rows}, {cols}) of {dtype} is wanted")
     return out, _matrix(ctx, out, name)
@@ -293,6 +296,8 @@ def dropout(ctx, x, p, seed, offset=0, per_row=False, out=None):
     """x with elements (or, per_row, rows) dropped with probability p and the others scaled up.  The mask is a function of (seed, offset + index):
     the same call on the gradient is the backward pass.  out may be x."""
     src = _matrix(ctx, x, "x")
+    if out is None:
+        out = torch.empty_strided(x.shape, (x.shape[1], 1), dtype=x.dtype, device=x.device)  # one long row, if x is
     out, desc = _out(ctx, out, *x.shape, x.dtype, x, "out")
     seed, offset = int(seed), int(offset)
     if not 0 <= seed < 1 << 64 or not 0 <= offset < 1 << 64:

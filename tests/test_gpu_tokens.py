@@ -216,6 +216,19 @@ def test_product_into_rows_of_any_distance(ctx, dtype, lead, gap):
         assert untouched(view, big)
 
 
+def test_new_matrices_have_rows_that_begin_at_16_bytes(ctx):
+    a, b = operand(ctx, 50, 200, 1, 17), operand(ctx, 33, 200, 1, 18)
+    for dtype in (F32, BF16, F16):
+        got = tk.product(ctx, a, b, dtype)
+        n = tk.rms_norm(ctx, got)
+        dx = tk.rms_norm_backward(ctx, n.y, n.sum, n.rstd)[0]
+        assert all(x.stride(0) * x.element_size() % 16 == 0 and x.shape == (50, 33) for x in (n.y, n.sum, dx))
+        assert tk.dropout(ctx, got.contiguous(), 0.5, 1).is_contiguous()
+        assert got.shape == (50, 33) and got.stride(1) == 1 and got.stride(0) * got.element_size() % 16 == 0 and got.data_ptr() % 16 == 0
+        dense = tk.product(ctx, a, b, dtype, out=torch.empty(50, 33, dtype=dtype, device="cuda"))
+        assert dense.is_contiguous() and torch.equal(dense, got)
+
+
 def test_product_ignores_what_lies_behind_the_columns(ctx):
     x = operand(ctx, 40, 200, 1, 9)
     b = operand(ctx, 30, 200, 1, 10)
