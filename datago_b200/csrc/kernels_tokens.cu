@@ -549,8 +549,8 @@ void patch_rows(const PatchJob& j, const dg_rows8* out8, const dg_matrix* out, c
 // ---- scales along the rows of the source, and of 128 x 128 blocks -------------------------------------------------------------
 // The transpose of a matrix stays in the order of the matrix (dg_rows8.by_column): only its scales run along the rows.  A CTA holds 128 x 128 elements
 // as they were loaded, a thread eight rows of eight columns, and meets twice over its columns' maxima.
-// 37003 x 1000 bf16: 26 us, 4.3 TB/s; two CTAs of 128 registers a thread fit an SM, and each waits for its loads once (transposing the values
-// through shared memory as well took 46).
+// 37003 x 1000 bf16: 23.5 us, 4.7 TB/s; each CTA waits for its loads once, and four of 64 registers a thread to an SM hide more of that than two of 128
+// did (26).  Transposing the values through shared memory as well took 46.
 constexpr uint32_t kColumnThreads = 256, kColumnTile = 128;
 constexpr int kColumnRows = 8;  // of a thread
 
@@ -1025,7 +1025,8 @@ void rms_norm(const NormJob& j, cudaStream_t s) {
 }
 
 // Backward.  24 images of 2294 x 1152 bf16 with all gradients: 92 us, 4.2 TB/s, 6 of them in the last sums; what bounds it is the chain of a row: its loads,
-// the sum along it across five warps, the stores (a warp per row has no barrier, but 160 registers of sums: 100 us and more).
+// the sum along it across five warps, the stores (a warp per row has no barrier, but 160 registers of sums: 100 us and more, and 97
+// with rows by cp.async and the sums for dweight in shared memory).
 // A worker (a.split.row_threads threads, whole warps) takes units one after the other, and a unit's rows R at a time, so that the loads of R
 // rows are under way at once and the R sums along them cross the worker's warps together.  A thread owns V vectors of eight columns of every row; it
 // keeps the elements as they were loaded and widens them twice, before and after those sums.
