@@ -196,6 +196,8 @@ def patch_rows(ctx, pixels, patch, mean, std, dtype=None, out=None):
     if pixels.dtype != torch.uint8 or pixels.dim() != 4 or not pixels.is_contiguous():
         raise _invalid("pixels: a contiguous uint8 [n, height, width, channels] tensor is wanted")
     n, h, w, c = pixels.shape
+    if not 1 <= c <= 4:
+        raise _invalid(f"{c} channels: 1 to 4 are wanted")
     if len(mean) != c or len(std) != c:
         raise _invalid(f"mean and std: {c} numbers are wanted")
     patch = int(patch)
@@ -212,7 +214,7 @@ def patch_rows(ctx, pixels, patch, mean, std, dtype=None, out=None):
         if dtype not in _DTYPES:
             raise _invalid("dtype: float32, bfloat16 or float16 is wanted")
         out, desc = _out(ctx, out, rows, cols, dtype, pixels, "out")
-    floats = _floats[c - 1] if c <= 4 else struct.Struct(f"{c}f").pack
+    floats = _floats[c - 1]
     _check(lib().dg_patch_rows(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, pixels.data_ptr(), n, h, w, c, patch, floats(*mean), floats(*std),
                                desc8, desc))
     return out

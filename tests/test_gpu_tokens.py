@@ -608,3 +608,10 @@ def test_refusals_leave_the_device_usable(ctx):
         with pytest.raises(dg.DatagoB200Error):
             call()
     assert torch.equal(tk.dropout(ctx, x, 0.0, 1), x)
+
+
+@pytest.mark.parametrize("channels", [0, 5])
+def test_pixels_of_other_channels_are_refused(ctx, channels):
+    pixels = torch.zeros(1, 16, 16, channels, dtype=torch.uint8, device="cuda")
+    with pytest.raises(dg.DatagoB200Error):
+        tk.patch_rows(ctx, pixels, 16, (0.5,) * channels, (0.5,) * channels)
