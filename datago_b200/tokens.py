@@ -333,15 +333,17 @@ class PatchStem:
         if self.p:
             dropout(self.ctx, x, self.p, self.seed, offset, out=x)
         norm = rms_norm(self.ctx, x, self.norm_weight, residual=positions, eps=self.eps, eight_bit=True, sum_out=x)
-        return norm, (pixels, norm.sum, norm.rstd, len(positions), offset)
+        # what later changes of the stem's attributes must not change: the same draws and the same weight go into the gradients
+        return norm, (pixels, norm.sum, norm.rstd, len(positions), offset, self.p, self.seed, self.norm_weight)
 
     def backward(self, saved, dy, dsum=None):
-        """Gradients (weight, positions, norm_weight), float32, from those of the norm's output and, in dsum, of its sum.  The pixels of
-        the bucket still have to be there."""
-        pixels, h, rstd, tokens, offset = saved
-        dx, dpositions, dnorm = rms_norm_backward(self.ctx, dy, h, rstd, self.norm_weight, dsum, tokens)
-        if self.p:
-            dropout(self.ctx, dx, self.p, self.seed, offset, out=dx)
+        """Gradients (weight, positions, norm_weight), float32, from those of the norm's output and, in dsum, of its sum, with the p, seed and
+        norm_weight of that forward pass, whatever the stem has now (an evaluation between the two may set p to 0).  The pixels of the bucket still
+        have to be there."""
+        pixels, h, rstd, tokens, offset, p, seed, norm_weight = saved
+        dx, dpositions, dnorm = rms_norm_backward(self.ctx, dy, h, rstd, norm_weight, dsum, tokens)
+        if p:
+            dropout(self.ctx, dx, p, seed, offset, out=dx)
         x = patch_rows(self.ctx, pixels, self.patch, self.mean, self.std, self.dtype)
         dweight = product(self.ctx, quantize_rows(self.ctx, dx, transpose=True), quantize_rows(self.ctx, x, transpose=True), torch.float32)
         return dweight, dpositions, dnorm
