@@ -318,11 +318,14 @@ class PatchStem:
     def __init__(self, ctx, patch, mean, std, weight, norm_weight=None, p=0.0, seed=0, eps=1e-6, dtype=torch.bfloat16):
         self.ctx, self.patch, self.mean, self.std = ctx, int(patch), tuple(mean), tuple(std)
         self.norm_weight, self.p, self.seed, self.eps, self.dtype = norm_weight, float(p), int(seed), float(eps), dtype
+        self.weight8 = None
         self.set_weight(weight)
 
     def set_weight(self, weight):
-        """After an optimizer step: the new weight in 8 bits."""
-        self.weight8 = quantize_rows(self.ctx, weight, block=GROUP)
+        """After an optimizer step: the new weight in 8 bits, on torch's current stream.  One of the same shape takes the old one's place in memory, so that
+        captured forward passes read it too."""
+        kept = self.weight8 if self.weight8 is not None and self.weight8.shape == weight.shape else None
+        self.weight8 = quantize_rows(self.ctx, weight, block=GROUP, out=kept)
 
     def forward(self, pixels, positions, offset=0):
         """(Norm with Rows8 for the first layer, what backward wants).  positions: [tokens of an image, width] of the stem's dtype.  offset: where this batch's

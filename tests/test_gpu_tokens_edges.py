@@ -58,3 +58,22 @@ def test_a_backward_pass_goes_by_its_forward_pass(ctx):
     want = stem.backward(saved, dy)
     stem.p = 0.5
     assert same(stem.backward(saved, dy), want)
+
+
+def test_a_captured_stem_reads_the_weight_that_was_set(ctx):
+    stem, pixels, positions = stem_of(ctx), some_pixels((2, 28, 42, 3), 13), rand((6, 96), F32, 14)
+    stem.forward(pixels, positions)
+    places = stem.weight8.values.data_ptr(), stem.weight8.scales.data_ptr()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = stem.forward(pixels, positions)[0]
+    new = rand((96, 588), F32, 15, 0.05)
+    stem.set_weight(new)
+    assert (stem.weight8.values.data_ptr(), stem.weight8.scales.data_ptr()) == places
+    graph.replay()
+    other = tk.PatchStem(ctx, 14, MEAN, STD, new, stem.norm_weight, p=0.25, seed=5, dtype=F32)
+    want = other.forward(pixels, positions)[0]
+    assert torch.equal(norm.sum, want.sum) and torch.equal(norm.y.values.float(), want.y.values.float())
+    stem.set_weight(rand((100, 588), F32, 16))  # of another shape: elsewhere
+    assert stem.weight8.shape == (100, 588)
