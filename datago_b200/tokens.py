@@ -7,7 +7,8 @@ rows of new ones (dropout's apart) begin at multiples of 16 bytes, so those whos
 124515 x 685 in bfloat16 then takes 71 us, into contiguous rows 171).  Matrices are 2-d tensors of float32, bfloat16 or float16 whose columns
 are neighbours in memory; their rows, those of `out` too, may be any distance apart.
 Gradients are calls of their own (rms_norm_backward, dropout on the gradient, product on operands quantised along the contraction);
-PatchStem puts them together for the stem of a model.
+PatchStem puts them together for the stem of a model.  Autograd knows nothing of these calls: while it records, tensors that require a gradient are
+refused (detach() them, or call under no_grad()).
 """
 import ctypes as C
 import struct
@@ -103,6 +104,8 @@ def _on_device(ctx, t, name):
         raise _invalid(f"{name}: a torch tensor is wanted")
     if t.get_device() != ctx.device or not t.is_cuda:  # (-1 for tensors of the host)
         raise _invalid(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise _invalid(f"{name} requires a gradient, which would be lost here: detach() it, or call under no_grad()")
 
 
 def _matrix(ctx, t, name):
@@ -313,7 +316,7 @@ class PatchStem:
     the images of a bucket), norm, 8-bit rows for the first layer.
 
     weight: [width, patch * patch * channels]; norm_weight: [width] or None.  The weight is laid out in 8 bits (scales of 128 x 128 blocks)
-    here and by set_weight, not with every call."""
+    here and by set_weight, not with every call.  weight, norm_weight and positions may require gradients: backward returns them."""
 
     def __init__(self, ctx, patch, mean, std, weight, norm_weight=None, p=0.0, seed=0, eps=1e-6, dtype=torch.bfloat16):
         self.ctx, self.patch, self.mean, self.std = ctx, int(patch), tuple(mean), tuple(std)
@@ -325,19 +328,20 @@ class PatchStem:
         """After an optimizer step: the new weight in 8 bits, on torch's current stream.  One of the same shape takes the old one's place in memory, so that
         captured forward passes read it too."""
         kept = self.weight8 if self.weight8 is not None and self.weight8.shape == weight.shape else None
-        self.weight8 = quantize_rows(self.ctx, weight, block=GROUP, out=kept)
+        self.weight8 = quantize_rows(self.ctx, weight.detach(), block=GROUP, out=kept)
 
     def forward(self, pixels, positions, offset=0):
         """(Norm with Rows8 for the first layer, what backward wants).  positions: [tokens of an image, width] of the stem's dtype.  offset: where this batch's
         elements begin in the run's count (see dropout)."""
         if isinstance(pixels, DeviceArray):
             pixels = torch.as_tensor(pixels, device=f"cuda:{self.ctx.device}")
+        norm_weight = None if self.norm_weight is None else self.norm_weight.detach()
         x = product(self.ctx, patch_rows(self.ctx, pixels, self.patch, self.mean, self.std), self.weight8, self.dtype)
         if self.p:
             dropout(self.ctx, x, self.p, self.seed, offset, out=x)
-        norm = rms_norm(self.ctx, x, self.norm_weight, residual=positions, eps=self.eps, eight_bit=True, sum_out=x)
+        norm = rms_norm(self.ctx, x, norm_weight, residual=positions.detach(), eps=self.eps, eight_bit=True, sum_out=x)
         # what later changes of the stem's attributes must not change: the same draws and the same weight go into the gradients
-        return norm, (pixels, norm.sum, norm.rstd, len(positions), offset, self.p, self.seed, self.norm_weight)
+        return norm, (pixels, norm.sum, norm.rstd, len(positions), offset, self.p, self.seed, norm_weight)
 
     def backward(self, saved, dy, dsum=None):
         """Gradients (weight, positions, norm_weight), float32, from those of the norm's output and, in dsum, of its sum, with the p, seed and

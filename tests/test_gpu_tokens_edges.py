@@ -77,3 +77,34 @@ def test_a_captured_stem_reads_the_weight_that_was_set(ctx):
     assert torch.equal(norm.sum, want.sum) and torch.equal(norm.y.values.float(), want.y.values.float())
     stem.set_weight(rand((100, 588), F32, 16))  # of another shape: elsewhere
     assert stem.weight8.shape == (100, 588)
+
+
+# ---- autograd --------------------------------------------------------------------------------------------------------------
+def calls_on(ctx, t, plain):
+    """Every function on `t` (64 x 256) where `plain` does as well."""
+    rstd = torch.ones(64, device="cuda")
+    return (lambda: tk.quantize_rows(ctx, t), lambda: tk.rms_norm(ctx, t), lambda: tk.rms_norm(ctx, plain, residual=t), lambda: tk.rms_norm(ctx, plain, weight=t[0]),
+            lambda: tk.rms_norm_backward(ctx, t, plain, rstd), lambda: tk.rms_norm_backward(ctx, plain, t, rstd), lambda: tk.rms_norm_backward(ctx, plain, plain, rstd, dsum=t),
+            lambda: tk.dropout(ctx, t, 0.5, 1), lambda: tk.dropout(ctx, plain, 0.5, 1, out=t))
+
+
+def test_tensors_whose_gradient_would_be_lost_are_refused(ctx):
+    leaf, plain = rand((64, 256), F32, 20).requires_grad_(), rand((64, 256), F32, 21)
+    for t in (leaf, leaf * 2):
+        for call in calls_on(ctx, t, plain):
+            with pytest.raises(dg.DatagoB200Error, match="grad"):
+                call()
+        with torch.no_grad():
+            for call in calls_on(ctx, t.detach().clone().requires_grad_(), plain):
+                call()
+
+
+def test_a_stem_takes_parameters(ctx):
+    weight, norm_weight, positions = (torch.nn.Parameter(rand(s, F32, 22 + i, 0.1)) for i, s in enumerate(((96, 588), (96,), (6, 96))))
+    pixels, dy = some_pixels((2, 28, 42, 3), 25), rand((12, 96), F32, 26)
+    stem = tk.PatchStem(ctx, 14, MEAN, STD, weight, norm_weight, p=0.1, dtype=F32)
+    norm, saved = stem.forward(pixels, positions)
+    got = stem.backward(saved, dy)
+    assert not norm.sum.requires_grad
+    other = tk.PatchStem(ctx, 14, MEAN, STD, weight.detach(), norm_weight.detach(), p=0.1, dtype=F32)
+    assert same(got, other.backward(other.forward(pixels, positions.detach())[1], dy))
