@@ -8,7 +8,7 @@ rows of new ones (dropout's apart) begin at multiples of 16 bytes, so those whos
 are neighbours in memory; their rows, those of `out` too, may be any distance apart.
 Gradients are calls of their own (rms_norm_backward, dropout on the gradient, product on operands quantised along the contraction);
 PatchStem puts them together for the stem of a model.  Autograd knows nothing of these calls: while it records, tensors that require a gradient are
-refused (detach() them, or call under no_grad()).
+refused (detach() them, or call under no_grad()), and what is written into a caller's tensor counts as a change in place.
 """
 import ctypes as C
 import struct
@@ -106,6 +106,13 @@ def _on_device(ctx, t, name):
         raise _invalid(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise _invalid(f"{name} requires a gradient, which would be lost here: detach() it, or call under no_grad()")
+
+
+def _changed(out):
+    """Tells autograd that a caller's tensor, or Rows8, has been written to."""
+    for t in (out.values, out.scales) if isinstance(out, Rows8) else (out,):
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 def _matrix(ctx, t, name):
@@ -207,7 +214,7 @@ def patch_rows(ctx, pixels, patch, mean, std, dtype=None, out=None):
     if patch < 1 or h % patch or w % patch or h == 0 or w == 0:
         raise _invalid(f"{h} x {w} pixels are no whole number of {patch} x {patch} patches")
     rows, cols = n * (h // patch) * (w // patch), patch * patch * c
-    desc8 = desc = None
+    desc8, desc, given = None, None, out is not None
     if dtype is None:
         if out is None:
             out, desc8 = _new_rows8(rows, cols, pixels)
@@ -220,6 +227,8 @@ def patch_rows(ctx, pixels, patch, mean, std, dtype=None, out=None):
     floats = _floats[c - 1]
     _check(lib().dg_patch_rows(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, pixels.data_ptr(), n, h, w, c, patch, floats(*mean), floats(*std),
                                desc8, desc))
+    if given:
+        _changed(out)
     return out
 
 
@@ -228,11 +237,14 @@ def quantize_rows(ctx, x, transpose=False, block=1, out=None):
     keeps the matrix's order in memory."""
     src = _matrix(ctx, x, "x")
     rows, cols = x.shape
-    if out is None:
+    given = out is not None
+    if not given:
         if block not in (1, GROUP):
             raise _invalid("block is 1 or 128")
         out = Rows8.empty(cols, rows, x.device, block, True) if transpose else Rows8.empty(rows, cols, x.device, block)
     _check(lib().dg_quantize_rows(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, src, _rows8(ctx, out, "out", transpose)))
+    if given:
+        _changed(out)
     return out
 
 
@@ -241,12 +253,14 @@ def product(ctx, a, b, dtype=torch.bfloat16, out=None):
     da, db = _rows8(ctx, a, "a"), _rows8(ctx, b, "b")
     if dtype not in _DTYPES:
         raise _invalid("dtype: float32, bfloat16 or float16 is wanted")
-    (m, k), n = a.values.shape, b.values.shape[0]
+    (m, k), n, given = a.values.shape, b.values.shape[0], out is not None
     out, desc = _out(ctx, out, m, n, dtype, a.values, "out")
     L = lib()
     nbytes = L.dg_product_workspace(ctx._h, m, n, k) if k > 1920 else 0
     work, at = _workspace(nbytes, out)
     _check(L.dg_product(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, da, db, desc, at, nbytes))
+    if given:
+        _changed(out)
     return out
 
 
@@ -270,6 +284,8 @@ def rms_norm(ctx, x, weight=None, residual=None, eps=1e-6, eight_bit=False, sum_
     else:
         y, y16 = _out(ctx, None, rows, cols, x.dtype, x, "y")
     _check(lib().dg_rms_norm(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, src, r, w, eps, total_desc, y16, y8, rstd.data_ptr()))
+    if sum_out is not None:
+        _changed(total)
     return Norm(y, total, rstd)
 
 
@@ -294,6 +310,8 @@ def rms_norm_backward(ctx, dy, h, rstd, weight=None, dsum=None, residual_rows=No
     work, at = _workspace(nbytes, dy)
     _check(L.dg_rms_norm_backward(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, g, hm, rstd.data_ptr(), w, s, dx_desc,
                                   dresidual.data_ptr() if period else None, period, dweight.data_ptr(), at, nbytes))
+    if dx_out is not None:
+        _changed(dx)
     return dx, dresidual, dweight
 
 
@@ -301,13 +319,16 @@ def dropout(ctx, x, p, seed, offset=0, per_row=False, out=None):
     """x with elements (or, per_row, rows) dropped with probability p and the others scaled up.  The mask is a function of (seed, offset + index):
     the same call on the gradient is the backward pass.  out may be x."""
     src = _matrix(ctx, x, "x")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_strided(x.shape, (x.shape[1], 1), dtype=x.dtype, device=x.device)  # one long row, if x is
     out, desc = _out(ctx, out, *x.shape, x.dtype, x, "out")
     seed, offset = int(seed), int(offset)
     if not 0 <= seed < 1 << 64 or not 0 <= offset < 1 << 64:
         raise _invalid("seed and offset are in [0, 2^64)")
     _check(lib().dg_dropout(ctx._h, _raw_stream(ctx.device) or _LEGACY_STREAM, src, p, seed, offset, per_row, desc))
+    if given:
+        _changed(out)
     return out
 
 

@@ -108,3 +108,19 @@ def test_a_stem_takes_parameters(ctx):
     assert not norm.sum.requires_grad
     other = tk.PatchStem(ctx, 14, MEAN, STD, weight.detach(), norm_weight.detach(), p=0.1, dtype=F32)
     assert same(got, other.backward(other.forward(pixels, positions.detach())[1], dy))
+
+
+def test_autograd_notices_results_that_are_written_into_its_tensors(ctx):
+    w = torch.ones(64, 256, device="cuda", requires_grad=True)
+    plain, rstd, pixels = rand((64, 256), F32, 27), torch.ones(64, device="cuda"), some_pixels((64, 8, 8, 4), 28)
+    a8, b8 = tk.quantize_rows(ctx, rand((64, 100), F32, 29)), tk.quantize_rows(ctx, rand((256, 100), F32, 30))
+    for write in (lambda x: tk.dropout(ctx, x, 0.5, 1, out=x), lambda x: tk.rms_norm(ctx, x, sum_out=x), lambda x: tk.rms_norm_backward(ctx, x, plain, rstd, dx_out=x),
+                  lambda x: tk.product(ctx, a8, b8, F32, out=x), lambda x: tk.patch_rows(ctx, pixels, 8, MEAN + (0.5,), STD + (0.5,), F32, out=x)):
+        x = rand((64, 256), F32, 31)
+        loss = (x * w).sum()
+        write(x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        x = rand((64, 256), F32, 32)
+        tk.dropout(ctx, x, 0.5, 1, out=x)
