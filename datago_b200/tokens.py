@@ -153,7 +153,8 @@ def _rows8(ctx, r, name, transposed=None):
     (ld, one), (scale_ld, sone) = v.stride(), s.stride()
     if sone != 1 and groups > 1:
         raise _invalid(f"{name}: scales have to be neighbours in memory")
-    by_row, by_column = one == 1 or cols <= 1, ld == 1 or rows <= 1
+    # A single column, or row, fits both orders.  Rows of a single column that are neighbours are its line: the transpose of one row.
+    by_row, by_column = (one == 1 or cols <= 1) and not (cols <= 1 < rows and ld == 1), ld == 1 or rows <= 1
     if transposed is not None:
         by_row, by_column = by_row and not transposed, by_column and transposed
     if by_row:

@@ -124,3 +124,28 @@ def test_autograd_notices_results_that_are_written_into_its_tensors(ctx):
     with torch.inference_mode():
         x = rand((64, 256), F32, 32)
         tk.dropout(ctx, x, 0.5, 1, out=x)
+
+
+# ---- single rows and none --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("m,n", [(768, 33), (33, 47), (16, 1), (1, 768), (1, 1), (1000, 300)])
+def test_product_over_a_single_row_of_transposed_operands(ctx, m, n, block):
+    a, b = tk.quantize_rows(ctx, rand((1, m), F32, 40), transpose=True, block=block), tk.quantize_rows(ctx, rand((1, n), F32, 41), transpose=True, block=block)
+    want = a.to_float().double() @ b.to_float().double().t()  # one product each
+    assert torch.equal(tk.product(ctx, a, b, F32).double(), want.float().double())
+    by_row = tk.Rows8.empty(n, 1, "cuda", block)
+    by_row.values.copy_(b.values)
+    by_row.scales.view(torch.uint8).copy_(b.scales.view(torch.uint8))
+    assert torch.equal(tk.product(ctx, a, by_row, F32).double(), want.float().double())
+
+
+def test_stem_of_a_single_patch(ctx):
+    stem, pixels, positions, dy = stem_of(ctx, p=0.0), some_pixels((1, 14, 14, 3), 42), rand((1, 96), F32, 43), rand((1, 96), F32, 44)
+    norm, saved = stem.forward(pixels, positions)
+    dweight, dpositions, dnorm = stem.backward(saved, dy)
+    dx = tk.rms_norm_backward(ctx, dy, norm.sum, norm.rstd, stem.norm_weight)[0]
+    x = tk.patch_rows(ctx, pixels, 14, MEAN, STD, F32)
+    # every group is one number, which its scale brings to [224, 448]: half a step of e4m3 is 2^-4 of it, each
+    want = dx.double().t() @ x.double()
+    assert bool(((dweight - want).abs() <= (2 * 2.0 ** -4 + 2.0 ** -7) * want.abs()).all())
+    assert torch.equal(dpositions, dx) and dnorm.shape == (96,)

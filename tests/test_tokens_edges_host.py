@@ -1,0 +1,48 @@
+"""The entry points of the token rows at their edges, without a GPU: csrc/tokens.cpp against stand-ins for the CUDA runtime and for the kernels (see
+test_tokens_host.py, whose helpers are used here)."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+import torch
+
+import datago_b200 as dg
+from datago_b200 import tokens as tk
+from test_tokens_host import AT, CSRC, INVALID, OK, ROOT, SYNC_LIMIT, TOO_LARGE, launched, matrix, refused, rows8
+
+
+@pytest.fixture(scope="module")
+def library(tmp_path_factory):
+    out = str(tmp_path_factory.mktemp("fake") / "libtokens_edges.so")
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    sources = [os.path.join(ROOT, "tests", f) for f in ("fake_device.cpp", "fake_tokens_edges.cpp")]
+    sources += [os.path.join(CSRC, f) for f in ("tokens.cpp", "api.cu", "feeder.cpp", "host_blocks.cpp", "host_logic.cpp", "jpeg_header.cpp")]
+    subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-pthread", "-Wl,-Bsymbolic", "-I", os.path.join(cuda, "include"), "-x", "c++", *sources, "-o", out], check=True)
+    return out
+
+
+@pytest.fixture
+def L(library, monkeypatch):
+    monkeypatch.setattr(dg, "library_path", lambda: library)
+    monkeypatch.setattr(dg, "_lib", None)
+    monkeypatch.delenv("DATAGO_B200_REBUILD", raising=False)
+    lib = tk.lib()
+    lib.fake_launches()
+    yield lib
+    monkeypatch.setattr(tk, "_lib", None)
+
+
+@pytest.fixture
+def ctx(L):
+    return dg.Context(0)
+
+
+@pytest.mark.parametrize("rows,cols,by_column,column", [(768, 1, True, 1), (16, 1, True, 1), (768, 1, False, 0), (1, 768, True, 1), (1, 768, False, 0), (768, 2, True, 1), (1, 1, True, 0), (1, 1, False, 0)])
+def test_rows8_of_a_single_row_or_column_keep_their_order(L, ctx, monkeypatch, rows, cols, by_column, column):
+    monkeypatch.setattr(tk, "_on_device", lambda ctx, t, name: None)
+    r = tk.Rows8.empty(rows, cols, "cpu", by_column=by_column)
+    desc = tk._rows8(ctx, r, "a")
+    assert int.from_bytes(desc[-4:], "little") == column  # dg_rows8.by_column
+    launched(L, L.dg_product(ctx._h, None, desc, rows8(5, cols), matrix(rows, 5, data=3 * AT), None, 0))
+    assert tk._rows8(ctx, r, "out", by_column) == desc or (rows == 1 and cols == 1)
