@@ -374,5 +374,7 @@ class PatchStem:
         if p:
             dropout(self.ctx, dx, p, seed, offset, out=dx)
         x = patch_rows(self.ctx, pixels, self.patch, self.mean, self.std, self.dtype)
+        if not len(x):  # a sum over no rows; the transposes would have no columns
+            return torch.zeros(dx.shape[1], x.shape[1], dtype=torch.float32, device=dx.device), dpositions, dnorm
         dweight = product(self.ctx, quantize_rows(self.ctx, dx, transpose=True), quantize_rows(self.ctx, x, transpose=True), torch.float32)
         return dweight, dpositions, dnorm

@@ -149,3 +149,12 @@ def test_stem_of_a_single_patch(ctx):
     want = dx.double().t() @ x.double()
     assert bool(((dweight - want).abs() <= (2 * 2.0 ** -4 + 2.0 ** -7) * want.abs()).all())
     assert torch.equal(dpositions, dx) and dnorm.shape == (96,)
+
+
+def test_stem_of_no_images(ctx):
+    stem = stem_of(ctx)
+    norm, saved = stem.forward(some_pixels((0, 28, 42, 3), 45), rand((6, 96), F32, 46))
+    assert norm.y.shape == (0, 96) and norm.sum.shape == (0, 96)
+    dweight, dpositions, dnorm = stem.backward(saved, torch.empty(0, 96, device="cuda"))
+    assert dweight.shape == (96, 588) and dpositions.shape == (6, 96) and dnorm.shape == (96,)
+    assert not bool(dweight.any()) and not bool(dpositions.any()) and not bool(dnorm.any())
