@@ -343,9 +343,11 @@ extern "C" int dg_rms_norm(dg_ctx* ctx, void* stream, const dg_matrix* x, const 
 }
 
 extern "C" uint64_t dg_rms_norm_backward_workspace(dg_ctx* ctx, uint64_t rows, uint64_t cols, uint64_t residual_rows) {
-    if (!ctx || rows == 0 || cols == 0 || cols > kNormMaxCols || rows > kMostRows || (residual_rows && rows % residual_rows)) return 0;
-    const uint64_t period = residual_rows ? residual_rows : rows;
-    return norm_backward_workspace(norm_backward_split(rows, cols, period, residual_rows != 0), cols, period);
+    if (!ctx || rows == 0 || cols == 0 || cols > kNormMaxCols || rows > kMostRows) return 0;
+    // a call without dresidual ignores residual_rows and deals the rows out otherwise
+    const uint64_t without = norm_backward_workspace(norm_backward_split(rows, cols, rows, false), cols, rows);
+    if (!residual_rows || rows % residual_rows) return without;
+    return std::max(without, norm_backward_workspace(norm_backward_split(rows, cols, residual_rows, true), cols, residual_rows));
 }
 
 extern "C" int dg_rms_norm_backward(dg_ctx* ctx, void* stream, const dg_matrix* dy, const dg_matrix* h, const float* rstd, const dg_matrix* weight,

@@ -404,7 +404,7 @@ DG_API int dg_rms_norm(dg_ctx* ctx, void* stream, const dg_matrix* x, const dg_m
  *   dresidual[t] = sum of dx over the rows r with r % residual_rows == t     (before dx is rounded; residual_rows x cols floats, may be NULL)
  *   dweight = sum over the rows of dy * hat                                  (cols floats, may be NULL)
  * dx may be NULL, dy or dsum.  Sums have a fixed order.  residual_rows is ignored without dresidual.  workspace:
- * dg_rms_norm_backward_workspace bytes, 16-byte aligned. */
+ * dg_rms_norm_backward_workspace bytes (enough with and without dresidual), 16-byte aligned. */
 DG_API uint64_t dg_rms_norm_backward_workspace(dg_ctx* ctx, uint64_t rows, uint64_t cols, uint64_t residual_rows);
 DG_API int dg_rms_norm_backward(dg_ctx* ctx, void* stream, const dg_matrix* dy, const dg_matrix* h, const float* rstd, const dg_matrix* weight,
                                 const dg_matrix* dsum, const dg_matrix* dx, float* dresidual, uint64_t residual_rows, float* dweight,

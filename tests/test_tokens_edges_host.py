@@ -46,3 +46,15 @@ def test_rows8_of_a_single_row_or_column_keep_their_order(L, ctx, monkeypatch, r
     assert int.from_bytes(desc[-4:], "little") == column  # dg_rows8.by_column
     launched(L, L.dg_product(ctx._h, None, desc, rows8(5, cols), matrix(rows, 5, data=3 * AT), None, 0))
     assert tk._rows8(ctx, r, "out", by_column) == desc or (rows == 1 and cols == 1)
+
+
+@pytest.mark.parametrize("rows,cols,period", [(6144, 1152, 256), (90000, 1152, 300), (100000, 512, 500), (4, 256, 2), (7, 33, 3), (24, 16384, 24), (1, 8, 1), (55056, 1152, 2294)])
+def test_a_norms_backward_pass_needs_what_was_asked_for(L, ctx, rows, cols, period):
+    need = L.dg_rms_norm_backward_workspace(ctx._h, rows, cols, period)
+    assert need > 0
+    x, h = matrix(rows, cols), matrix(rows, cols, data=1 << 40)
+    for dresidual in (AT, None):  # residual_rows is ignored without dresidual
+        if dresidual and rows % period:
+            continue
+        launched(L, L.dg_rms_norm_backward(ctx._h, None, x, h, AT, None, None, None, dresidual, period, AT, AT, need))
+    assert L.dg_rms_norm_backward_workspace(ctx._h, rows, cols, 0) <= need
