@@ -324,6 +324,7 @@ extern "C" int dg_rms_norm(dg_ctx* ctx, void* stream, const dg_matrix* x, const 
     if (int rc = check_apart(sum, "sum", x, "x", true)) return rc;
     if (int rc = check_apart(y, "y", sum, "sum")) return rc;
     if (int rc = check_apart(y8, "y8", sum, "sum")) return rc;
+    if (int rc = check_apart(y, "y", y8, "y8")) return rc;
     for (const dg_matrix* in : {x, residual, weight}) {
         if (int rc = in == x ? DG_OK : check_apart(sum, "sum", in, "an input")) return rc;
         if (int rc = check_apart(y, "y", in, "an input")) return rc;

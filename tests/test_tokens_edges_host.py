@@ -58,3 +58,12 @@ def test_a_norms_backward_pass_needs_what_was_asked_for(L, ctx, rows, cols, peri
             continue
         launched(L, L.dg_rms_norm_backward(ctx._h, None, x, h, AT, None, None, None, dresidual, period, AT, AT, need))
     assert L.dg_rms_norm_backward_workspace(ctx._h, rows, cols, 0) <= need
+
+
+def test_the_norms_two_outputs_are_apart(L, ctx):
+    def call(y, y8):
+        return L.dg_rms_norm(ctx._h, None, matrix(), None, None, 1e-6, None, y, y8, None)
+    launched(L, call(matrix(data=2 * AT), rows8(values=3 * AT)))
+    refused(L, call(matrix(data=2 * AT), rows8(values=2 * AT)))
+    refused(L, call(matrix(data=2 * AT), rows8(values=2 * AT + 4 * 512 - 16)))
+    launched(L, call(matrix(data=2 * AT), rows8(values=2 * AT + 4 * 512)))
