@@ -151,7 +151,8 @@ int check_workspace(const void* p, uint64_t bytes, uint64_t needed) {
     return DG_OK;
 }
 
-// Where a matrix lies.  Two of them share memory unless their ranges are apart, or they are other columns of rows that are equally far apart.
+// Where a matrix lies.  Two of them share memory unless their ranges are apart, or they are other columns of rows that are equally far apart (as a
+// single row is from any).
 struct Lies {
     uintptr_t at;
     uint64_t rows, width, pitch;  // bytes
@@ -161,9 +162,9 @@ Lies lies(const dg_rows8* r) { return r->by_column ? Lies{(uintptr_t)r->values, 
 bool share(const Lies& a, const Lies& b) {
     if (!a.rows || !b.rows || !a.at || !b.at) return false;
     if (a.at + (a.rows - 1) * a.pitch + a.width <= b.at || b.at + (b.rows - 1) * b.pitch + b.width <= a.at) return false;
-    if (a.pitch != b.pitch) return true;
-    const uint64_t apart = (b.at % a.pitch + a.pitch - a.at % a.pitch) % a.pitch;  // from the columns of a to those of b
-    return !(apart >= a.width && apart + b.width <= a.pitch);
+    if (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) return true;
+    const uint64_t pitch = a.rows > 1 ? a.pitch : b.pitch, apart = (b.at % pitch + pitch - a.at % pitch) % pitch;  // from the columns of a to those of b
+    return !(apart >= a.width && apart + b.width <= pitch);
 }
 // out may be in, where that is said of them, but not reach into it otherwise
 template <class A, class B>

@@ -158,3 +158,13 @@ def test_stem_of_no_images(ctx):
     dweight, dpositions, dnorm = stem.backward(saved, torch.empty(0, 96, device="cuda"))
     assert dweight.shape == (96, 588) and dpositions.shape == (6, 96) and dnorm.shape == (96,)
     assert not bool(dweight.any()) and not bool(dpositions.any()) and not bool(dnorm.any())
+
+
+def test_a_row_beside_other_rows_is_apart_from_them(ctx):
+    big = rand((12, 512), F32, 55)
+    x, weight, position = big[:, 256:], big[0, :256], big[3:4, :256]
+    want = tk.rms_norm(ctx, x.clone(), weight.clone(), residual=position.clone())
+    got = tk.rms_norm(ctx, x, weight, residual=position, sum_out=x)
+    assert torch.equal(got.y, want.y) and torch.equal(x, want.sum)
+    with pytest.raises(dg.DatagoB200Error):
+        tk.rms_norm(ctx, x, big[0, 128:384], sum_out=x)

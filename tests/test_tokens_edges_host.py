@@ -67,3 +67,17 @@ def test_the_norms_two_outputs_are_apart(L, ctx):
     refused(L, call(matrix(data=2 * AT), rows8(values=2 * AT)))
     refused(L, call(matrix(data=2 * AT), rows8(values=2 * AT + 4 * 512 - 16)))
     launched(L, call(matrix(data=2 * AT), rows8(values=2 * AT + 4 * 512)))
+
+
+def test_a_single_row_is_apart_from_rows_beside_it(L, ctx):
+    # rows of 256 elements of 2 bytes, 512 elements apart; one row beside them, whatever distance it names
+    def call(at, cols=256, ld=None, rows=1):
+        return L.dg_rms_norm(ctx._h, None, matrix(ld=512, data=AT), matrix(rows, cols, ld, data=at), None, 1e-6, matrix(ld=512, data=AT), None, None, None)
+    launched(L, call(AT + 512))
+    launched(L, call(AT + 512 + 3 * 1024))
+    launched(L, call(AT + 512, ld=300))
+    launched(L, call(AT - 512))
+    for at in (AT, AT + 2, AT + 510, AT + 514, AT + 1024, AT + 3 * 1024, AT - 510):
+        refused(L, call(at))
+    launched(L, call(AT + 512, ld=512, rows=2))
+    refused(L, call(AT + 512, ld=600, rows=2))  # the second one is in the first columns of the rows
