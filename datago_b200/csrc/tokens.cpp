@@ -197,6 +197,7 @@ extern "C" int dg_patch_rows(dg_ctx* ctx, void* stream, const uint8_t* pixels, u
     const uint64_t per_image = (uint64_t)(h / patch) * (w / patch), rows = n * per_image, cols = (uint64_t)patch * patch * channels;
     if ((uint64_t)patch * (patch * channels + 11) > 48 * 1024 - 24) return fail(DG_E_TOO_LARGE, "patches of %u x %u x %u: at most 48 KB", patch, patch, channels);
     if (per_image > (1ull << 27) / scale_groups(cols)) return fail(DG_E_TOO_LARGE, "%u x %u pixels are too many for one image", h, w);
+    if (n > kMostCols) return fail(DG_E_TOO_LARGE, "%u images: at most %llu", n, (unsigned long long)kMostCols);  // launches add up to 2^30 images to a count of 32 bits
     if (n && !pixels) return fail(DG_E_INVALID, "pixels is NULL");
     if (out) {
         if (int rc = check_matrix(out, "out")) return rc;

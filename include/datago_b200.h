@@ -371,8 +371,8 @@ typedef struct dg_rows8 {
 
 /* Patches of a bucket as rows.  Row (i * h/patch + Y) * w/patch + X, feature (y * patch + x) * channels + c is
  * (pixels[i][Y * patch + y][X * patch + x][c] / 255 - mean[c]) / std[c].  Exactly one of out8 (block 1) and out (f32, bf16, f16) is
- * not NULL.  h and w have to be multiples of patch; channels 1 to 4; a patch at most 48 KB (126 x 126 x 3); mean and std hold
- * `channels` host floats, std > 0. */
+ * not NULL.  h and w have to be multiples of patch; channels 1 to 4; a patch at most 48 KB (126 x 126 x 3); n at most 2^31 - 1024;
+ * mean and std hold `channels` host floats, std > 0. */
 DG_API int dg_patch_rows(dg_ctx* ctx, void* stream, const uint8_t* pixels, uint32_t n, uint32_t h, uint32_t w, uint32_t channels,
                          uint32_t patch, const float* mean, const float* std, const dg_rows8* out8, const dg_matrix* out);
 

@@ -81,3 +81,13 @@ def test_a_single_row_is_apart_from_rows_beside_it(L, ctx):
         refused(L, call(at))
     launched(L, call(AT + 512, ld=512, rows=2))
     refused(L, call(AT + 512, ld=600, rows=2))  # the second one is in the first columns of the rows
+
+
+def test_images_are_counted_in_32_bits(L, ctx):
+    one = (C.c_float * 4)(1, 1, 1, 1)
+
+    def call(n):
+        return L.dg_patch_rows(ctx._h, None, AT, n, 1, 1, 1, 1, one, one, rows8(n, 1, values=1 << 50, scales=1 << 52), None)
+    launched(L, call((1 << 31) - 1024))
+    for n in ((1 << 31) - 1023, 1 << 31, (1 << 32) - 1):
+        refused(L, call(n), TOO_LARGE)
