@@ -397,7 +397,8 @@ extern "C" int dg_dropout(dg_ctx* ctx, void* stream, const dg_matrix* x, double 
     if (int rc = check_apart(y, "y", x, "x", true)) return rc;
     const double t = p >= 0 && p < 1 ? std::floor(p * 65536 + 0.5) : 65536;
     if (t > 65535) return fail(DG_E_INVALID, "p is in [0, 1) and at most 65535 / 65536");
-    if (offset + x->rows * (per_row ? 1 : x->cols) < offset) return fail(DG_E_INVALID, "offset: the indices pass 2^64");
+    const uint64_t indices = x->rows * (per_row ? 1 : x->cols);
+    if (indices && offset + (indices - 1) < offset) return fail(DG_E_INVALID, "offset: the indices pass 2^64");
     if (x->rows == 0) return DG_OK;
     const DropoutJob j{x->data, y->data, x->rows, x->cols, x->ld, y->ld, seed, offset, (uint32_t)t, x->dtype, per_row != 0};
     return launched(ctx, [&] { launch_dropout(j, stream_of(ctx, stream)); });

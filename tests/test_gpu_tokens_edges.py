@@ -168,3 +168,15 @@ def test_a_row_beside_other_rows_is_apart_from_them(ctx):
     assert torch.equal(got.y, want.y) and torch.equal(x, want.sum)
     with pytest.raises(dg.DatagoB200Error):
         tk.rms_norm(ctx, x, big[0, 128:384], sum_out=x)
+
+
+def test_dropout_of_the_last_indices_there_are(ctx):
+    x = torch.ones(4, 24, device="cuda")
+    first = (1 << 64) - 96
+    whole = tk.dropout(ctx, x, 0.5, 3, first)
+    for r in range(4):  # row by row, the last one alone
+        assert torch.equal(tk.dropout(ctx, x[r:r + 1], 0.5, 3, first + 24 * r), whole[r:r + 1])
+    assert torch.equal(tk.dropout(ctx, x[:, :1], 0.5, 3, (1 << 64) - 4, per_row=True)[3], tk.dropout(ctx, x[:1, :1], 0.5, 3, (1 << 64) - 1)[0])
+    for call in (lambda: tk.dropout(ctx, x, 0.5, 3, first + 1), lambda: tk.dropout(ctx, x, 0.5, 3, (1 << 64) - 3, per_row=True)):
+        with pytest.raises(dg.DatagoB200Error):
+            call()

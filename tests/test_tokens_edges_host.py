@@ -91,3 +91,12 @@ def test_images_are_counted_in_32_bits(L, ctx):
     launched(L, call((1 << 31) - 1024))
     for n in ((1 << 31) - 1023, 1 << 31, (1 << 32) - 1):
         refused(L, call(n), TOO_LARGE)
+
+
+def test_dropout_takes_the_last_index_there_is(L, ctx):
+    def call(offset, per_row, rows=4):
+        return L.dg_dropout(ctx._h, None, matrix(rows), 0.1, 1, offset, per_row, matrix(rows, data=2 * AT))
+    for per_row, count in ((0, 1024), (1, 4)):
+        launched(L, call((1 << 64) - count, per_row))
+        refused(L, call((1 << 64) - count + 1, per_row))
+        refused(L, call((1 << 64) - 1, per_row))
