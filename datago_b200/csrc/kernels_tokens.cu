@@ -999,7 +999,8 @@ void rms_norm(const NormJob& j, cudaStream_t s) {
     }
     auto go = [&](auto kernel, uint32_t threads, uint32_t rows_per_cta) {
         const size_t smem = j.weight ? (j.cols + 7) / 8 * 32 : 0;
-        if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kNormMaxCols * 4));
+        // 48 KB, the kernel's own s_part among them, need no allowance
+        if (smem + threads / 32 * sizeof(float) > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kNormMaxCols * 4));
         launch_after(kernel, grid_for(j.rows, rows_per_cta, 1024 / threads), threads, smem, s, j, x_whole, r_whole, s_whole, y_whole);
     };
 #define DG_NORM(V, TPR, THREADS) (whole ? go(k_rms_norm<T, V, TPR, THREADS, true>, THREADS, THREADS / TPR) : go(k_rms_norm<T, V, TPR, THREADS, false>, THREADS, THREADS / TPR))

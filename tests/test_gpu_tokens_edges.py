@@ -180,3 +180,33 @@ def test_dropout_of_the_last_indices_there_are(ctx):
     for call in (lambda: tk.dropout(ctx, x, 0.5, 3, first + 1), lambda: tk.dropout(ctx, x, 0.5, 3, (1 << 64) - 3, per_row=True)):
         with pytest.raises(dg.DatagoB200Error):
             call()
+
+
+# ---- borders ---------------------------------------------------------------------------------------------------------------
+def norms_of_wide_rows():
+    own = dg.Context(0)
+    for dtype in (F32, BF16):
+        for cols in (12288, 12280, 12273, 12264, 12289, 16384):  # the weight as floats: 48 KB and a little less or more
+            x, w = rand((3, cols), dtype, cols), rand((cols,), F32, 50)
+            got = tk.rms_norm(own, x, w)
+            want = x.double() / torch.sqrt(x.double().square().mean(1, keepdim=True) + 1e-6) * w.double()
+            # a sum of 64 + 14 additions, a handful of products, the rounding to the type
+            assert bool(((got.y.double() - want).abs() <= (50 * 2.0 ** -24 + (2.0 ** -8 if dtype is BF16 else 2.0 ** -24)) * want.abs() + 1e-30).all()), (dtype, cols)
+
+
+def test_norm_of_weights_that_need_more_shared_memory_than_a_launch_has_unasked():
+    # in a process of its own: what a kernel has been allowed once it may have from then on
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = "import sys; sys.path[:0] = [%r, %r]; import test_gpu_tokens_edges as t; t.norms_of_wide_rows()" % (here, os.path.dirname(here))
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
+
+
+def test_norm_has_16384_columns_at_most(ctx):
+    for cols in (16384, 16385):
+        x, rstd = rand((2, cols), BF16, 51), torch.ones(2, device="cuda")
+        for call in (lambda: tk.rms_norm(ctx, x), lambda: tk.rms_norm_backward(ctx, x, x.clone(), rstd)):
+            if cols == 16384:
+                call()
+            else:
+                with pytest.raises(dg.DatagoB200Error, match="16384"):
+                    call()
