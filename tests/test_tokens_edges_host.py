@@ -100,3 +100,15 @@ def test_dropout_takes_the_last_index_there_is(L, ctx):
         launched(L, call((1 << 64) - count, per_row))
         refused(L, call((1 << 64) - count + 1, per_row))
         refused(L, call((1 << 64) - 1, per_row))
+
+
+@pytest.mark.parametrize("cols,status", [(16384, OK), (16385, TOO_LARGE), (32768, TOO_LARGE)])
+def test_a_norm_has_as_many_columns_as_the_header_says(L, ctx, cols, status):
+    with open(os.path.join(ROOT, "include", "datago_b200.h")) as f:
+        text = f.read()
+    assert "cols at most 16384" in text and "at most 32768" not in text
+    x, h = matrix(4, cols), matrix(4, cols, data=2 * AT)
+    need = L.dg_rms_norm_backward_workspace(ctx._h, 4, cols, 0)
+    check = launched if status == OK else lambda L, rc: refused(L, rc, status)
+    check(L, L.dg_rms_norm(ctx._h, None, x, None, None, 1e-6, None, h, None, None))
+    check(L, L.dg_rms_norm_backward(ctx._h, None, x, h, AT, None, None, None, None, 0, AT, AT, need))
