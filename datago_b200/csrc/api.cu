@@ -98,6 +98,10 @@ inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 }  // namespace
 
+// Products that have given up on each device, as far as some context has been told: what a new context need not report.
+constexpr int kDevices = 64;
+static std::atomic<uint32_t> products_known[kDevices];
+
 struct dg_ctx {
     int device = 0;
     cudaStream_t stream = nullptr;   // kernels and downloads are ordered on this stream, and dg_batch_run orders it behind the inputs
@@ -130,6 +134,7 @@ struct dg_ctx {
     // dp2a kernel (measurements, and the test-suite's coverage of that kernel).
     bool hmma = true;
     dg_ctx_counters counters{};  // guarded by mu
+    std::atomic<uint32_t> products_seen{0};  // of those that gave up on the device: the ones this context has reported (see dg_product_status)
     // Largest decoded image accepted (width * height * channels bytes); the `image` crate's default allocation limit is 512 MiB.
     uint64_t max_image_bytes = (uint64_t)512 << 20;
 };
@@ -160,6 +165,7 @@ static int ctx_create(int device, const dg_image_config* cfg, void* stream, bool
     }
     dg_ctx* c = new dg_ctx();
     c->device = device;
+    if (device != DG_DEVICE_NONE && device < kDevices) c->products_seen = products_known[device].load();
     if (cfg && cfg->crop_and_resize) {
         if (!config_valid(*cfg)) { delete c; return fail(DG_E_INVALID, "image_config: size, ratio and aspect-ratio bounds must be positive and ordered"); }
         c->cfg = *cfg;
@@ -227,6 +233,16 @@ extern "C" void dg_ctx_destroy(dg_ctx* c) {
 }
 
 int dg::ctx_device(const dg_ctx* c) { return c->device; }
+static uint32_t raise_to(std::atomic<uint32_t>& most, uint32_t v) {  // returns what it was
+    uint32_t before = most.load();
+    while (before < v && !most.compare_exchange_weak(before, v)) {}
+    return before;
+}
+uint32_t dg::ctx_products_unreported(dg_ctx* c, uint32_t count) {
+    if (c->device < kDevices) raise_to(products_known[c->device], count);
+    const uint32_t seen = raise_to(c->products_seen, count);
+    return count > seen ? count - seen : 0;
+}
 void* dg::encode_tiled_entry() { return (void*)encode_tiled_fn(); }
 
 extern "C" void* dg_ctx_stream(dg_ctx* c) { return c ? (void*)c->stream : nullptr; }

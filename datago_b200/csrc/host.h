@@ -61,6 +61,7 @@ int dg_set_error(int code, const char* msg);
 
 // ---- contexts ---------------------------------------------------------------------------------------------------------
 int ctx_device(const dg_ctx* ctx);    // DG_DEVICE_NONE for planning-only ones
+uint32_t ctx_products_unreported(dg_ctx* ctx, uint32_t count);  // of `count` products that have given up on its device, those that the context has not reported; now it has
 void* encode_tiled_entry();           // cuTensorMapEncodeTiled, or NULL where the driver does not have it
 
 // ---- batches --------------------------------------------------------------------------------------------------------

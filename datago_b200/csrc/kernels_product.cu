@@ -49,7 +49,7 @@ constexpr uint32_t kSecond = kProductTwoSums, kScaleColumns = 2 * kProductTwoSum
 static_assert(kScaleColumns + 2 * 24 <= 512 && kScaleColumns >= kProductMaxTileN, "the scales fit behind the sums");
 constexpr uint32_t kWaitLimit = 1u << 20;  // waits of up to 2 us each
 
-__device__ unsigned int g_gave_up;
+__device__ unsigned int g_gave_up;  // never set back: each context remembers what it has reported
 
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
@@ -550,10 +550,6 @@ cudaError_t product_gave_up(unsigned int* count, cudaStream_t s) {
     *count = 0;
     if (e == cudaSuccess) e = cudaMemcpyAsync(count, at, sizeof *count, cudaMemcpyDeviceToHost, s);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-    if (e == cudaSuccess && *count) {
-        e = cudaMemsetAsync(at, 0, sizeof *count, s);
-        if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-    }
     return e;
 }
 

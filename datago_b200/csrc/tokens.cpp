@@ -1,5 +1,5 @@
 // C entry points of the token rows (declared in include/datago_b200.h): checks of the arguments, tensor maps, launches.  None of them
-// allocates, waits (dg_product_status apart) or keeps anything, so calls need no lock and can be captured.
+// allocates, waits or keeps anything (dg_product_status apart), so calls need no lock and can be captured.
 #include <algorithm>
 #include <cmath>
 #include <cstdarg>
@@ -298,6 +298,7 @@ extern "C" int dg_product_status(dg_ctx* ctx, void* stream) {
         return fail(DG_E_INVALID, "the stream is being captured");
     const cudaError_t e = on.error != cudaSuccess ? on.error : product_gave_up(&count, stream_of(ctx, stream));
     if (e != cudaSuccess) return fail(DG_E_CUDA, "%s", cudaGetErrorString(e));
+    count = ctx_products_unreported(ctx, count);
     return count ? fail(DG_E_SYNC_LIMIT, "%u CTAs of products gave up waiting for a copy", count) : DG_OK;
 }
 

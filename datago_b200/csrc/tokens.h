@@ -101,6 +101,6 @@ struct ProductJob {
     ProductPlan plan;
 };
 cudaError_t launch_product(const ProductJob& job, cudaStream_t s);
-cudaError_t product_gave_up(unsigned int* count, cudaStream_t s);  // waits for the stream; the count starts anew
+cudaError_t product_gave_up(unsigned int* count, cudaStream_t s);  // waits for the stream; CTAs on the current device since the process began
 
 }  // namespace dg

@@ -389,8 +389,9 @@ DG_API int dg_quantize_rows(dg_ctx* ctx, void* stream, const dg_matrix* src, con
 DG_API uint64_t dg_product_workspace(dg_ctx* ctx, uint64_t m, uint64_t n, uint64_t k);
 DG_API int dg_product(dg_ctx* ctx, void* stream, const dg_rows8* a, const dg_rows8* b, const dg_matrix* out, void* workspace,
                       uint64_t workspace_bytes);
-/* Waits for the stream.  DG_E_SYNC_LIMIT when a product on the device has given up waiting for a copy since the last call (its output is
- * then undefined): the counterpart of what dg_batch_sync reports for resize passes.  Not inside a stream capture. */
+/* Waits for the stream.  DG_E_SYNC_LIMIT when a product on the device, whichever context's, has given up waiting for a copy since the last call with
+ * this ctx (its output is then undefined): the counterpart of what dg_batch_sync reports for resize passes.  Every context gets its own report; a new
+ * one none of what others had got before.  Not inside a stream capture. */
 DG_API int dg_product_status(dg_ctx* ctx, void* stream);
 
 /* h = x + residual (row r takes residual row r % residual->rows, so positions can be shared by all images of a bucket; residual may be

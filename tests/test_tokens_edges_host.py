@@ -112,3 +112,22 @@ def test_a_norm_has_as_many_columns_as_the_header_says(L, ctx, cols, status):
     check = launched if status == OK else lambda L, rc: refused(L, rc, status)
     check(L, L.dg_rms_norm(ctx._h, None, x, None, None, 1e-6, None, h, None, None))
     check(L, L.dg_rms_norm_backward(ctx._h, None, x, h, AT, None, None, None, None, 0, AT, AT, need))
+
+
+def test_every_context_learns_of_products_that_gave_up(L):
+    first, second = dg.Context(0), dg.Context(0)
+    for c in (first, second):
+        assert L.dg_product_status(c._h, None) == OK
+    L.fake_gave_up(3)
+    refused(L, L.dg_product_status(first._h, None), SYNC_LIMIT)
+    assert L.dg_product_status(first._h, None) == OK  # once
+    later = dg.Context(0)
+    assert L.dg_product_status(later._h, None) == OK  # reported before there was this one
+    refused(L, L.dg_product_status(second._h, None), SYNC_LIMIT)  # its own report, which the other one's call has not taken
+    assert b"3 CTAs" in L.dg_last_error()
+    assert L.dg_product_status(second._h, None) == OK
+    L.fake_gave_up(1)
+    for c in (later, second, first):
+        refused(L, L.dg_product_status(c._h, None), SYNC_LIMIT)
+        assert b"1 CTAs" in L.dg_last_error()
+        assert L.dg_product_status(c._h, None) == OK
