@@ -18,7 +18,8 @@
 // An operand whose rows are neighbours in memory (dg_rows8.by_column) is copied as 128 rows x 128 columns too, and the instruction told.
 // Measured: 8192 x 8192 x 8192 432 us, 2.5 PFLOP/s; 131072 x 1152 x 768 into bf16 126 us, 1.8 (its 302 MB of output alone take 80 at the 3.8 TB/s of a plain
 // fill, its multiplications alone 80, its copies 55: they do not quite hide one another); 1152 x 768 x 57600 61 us, where copies out of L2 end at
-// 10 TB/s; 7 x 1024 x 768 6 us, all latency.  Accuracy: 1.5e-8 of the result over 128 columns, 3e-7 over parts of 8192.
+// 10 TB/s; 7 x 1024 x 768 6 us, all latency.  Accuracy: 1.5e-8 of the result over 128 columns, 3e-7 over 8192,
+// which no part of a contraction exceeds (dg::plan_product).
 // Waits are bounded: a CTA that runs out of patience counts itself (dg_product_status) and leaves.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -225,7 +226,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_produ
         t.n0 = tn * tile_n;
         t.same_before = a_stays && tn != 0 && i != first;
         t.same_after = a_stays && tn + 1 != tiles_n && i + 1 != end;
-        t.g0 = t.split * j.plan.split_groups;
+        t.g0 = j.first_group + t.split * j.plan.split_groups;
         t.g1 = min(groups, t.g0 + j.plan.split_groups);
         return t;
     };
@@ -482,16 +483,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_produ
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// The parts of a split contraction, added up in their order.
+// The parts of a split contraction, added up in their order, behind the sum of those before them (before: NULL where there are none).
 template <class T>
-__global__ void __launch_bounds__(256) k_add_parts(const float* parts, uint32_t splits, uint64_t part_elements, uint64_t m, uint64_t n, uint64_t part_ld, T* out,
-                                                   uint64_t ld) {
+__global__ void __launch_bounds__(256) k_add_parts(const float* before, const float* parts, uint32_t splits, uint64_t part_elements, uint64_t m, uint64_t n, uint64_t part_ld,
+                                                   T* out, uint64_t ld) {
     let_next_start();
     wait_for_previous();
     parts = from_previous(parts);
+    before = from_previous(before);
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < m * (part_ld / 4); i += (uint64_t)gridDim.x * 256) {
         const uint64_t row = i / (part_ld / 4), col = (i - row * (part_ld / 4)) * 4;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 sum = before ? *reinterpret_cast<const float4*>(before + row * part_ld + col) : make_float4(0.f, 0.f, 0.f, 0.f);
         for (uint32_t p = 0; p < splits; ++p) {
             const float4 v = *reinterpret_cast<const float4*>(parts + p * part_elements + row * part_ld + col);
             sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
@@ -529,10 +531,18 @@ template <class T>
 cudaError_t product(const ProductJob& j, cudaStream_t s) {
     if (j.plan.splits == 1) return product_into<T>(j, (T*)j.out, j.ld, 0, s);
     const uint64_t part_ld = product_part_ld(j.n), part = j.m * part_ld;
-    const cudaError_t e = product_into<float>(j, j.parts, part_ld, part, s);
-    if (e != cudaSuccess) return e;
-    const uint32_t ctas = (uint32_t)std::min<uint64_t>((j.m * (part_ld / 4) + 255) / 256, (uint64_t)kSms * 8);
-    launch_after(k_add_parts<T>, ctas, 256, 0, s, j.parts, j.plan.splits, part, j.m, j.n, part_ld, (T*)j.out, j.ld);
+    const uint32_t ctas = (uint32_t)std::min<uint64_t>((j.m * (part_ld / 4) + 255) / 256, (uint64_t)kSms * 8), splits = j.plan.splits;
+    float* const sum = j.parts + j.plan.together * part;  // of the parts so far, where they are not all made together
+    ProductJob some = j;
+    for (uint32_t first = 0; first < splits; first += some.plan.splits) {
+        some.first_group = first * j.plan.split_groups;
+        some.plan.splits = std::min(j.plan.together, splits - first);
+        const cudaError_t e = product_into<float>(some, j.parts, part_ld, part, s);
+        if (e != cudaSuccess) return e;
+        const float* const before = first ? sum : nullptr;
+        if (first + some.plan.splits < splits) launch_after(k_add_parts<float>, ctas, 256, 0, s, before, j.parts, some.plan.splits, part, j.m, j.n, part_ld, sum, part_ld);
+        else launch_after(k_add_parts<T>, ctas, 256, 0, s, before, j.parts, some.plan.splits, part, j.m, j.n, part_ld, (T*)j.out, j.ld);
+    }
     return cudaGetLastError();
 }
 

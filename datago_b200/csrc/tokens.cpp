@@ -33,9 +33,12 @@ ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t k, bool b_by_column) {
             q.sums = q.tile_n <= kProductTwoSums ? 2 : 1;
             const uint64_t tiles = (uint64_t)q.tiles_m * q.tiles_n;
             const uint32_t b_bytes = (b_by_column ? 128 : q.tile_n / 2) * 128;
-            // The tensor cores cut what lies below their sums off: over 116 groups 1.4e-6 of a gradient of random terms was lost, over 44 3e-7.  Where
-            // there are few tiles, and parts are cheap, none is longer than 64.
-            for (uint32_t s = tiles <= kPairs ? std::min(16u, (groups + 63) / 64) : 1; s <= 16 && (s == 1 || s * 8 <= groups); ++s) {
+            // The tensor cores cut off what lies below their sums, and lose the more the longer a sum is (random terms over 116 groups 1.4e-6 of the
+            // result, over 44 3e-7; beside one large term all small ones): no part is longer than kProductPartGroups (4096 x 4096 x
+            // 131072 1.91 ms, in one part 1.52; 4096 x 1152 x 57600 285 us, in three parts 225).  More parts than that asks for, up to 16, where they
+            // spread the work.
+            const uint32_t least = (groups + kProductPartGroups - 1) / kProductPartGroups;
+            for (uint32_t s = least; s == least || (s <= 16 && s * 8 <= groups); ++s) {
                 q.split_groups = s == 1 ? groups : ((groups + s - 1) / s + 3) / 4 * 4;  // parts begin at multiples of four groups: the scales come in words
                 q.splits = (groups + q.split_groups - 1) / q.split_groups;
                 // a stays where its rows leave room for three slots of b and most pairs walk tiles of the same rows
@@ -51,6 +54,7 @@ ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t k, bool b_by_column) {
         }
         if (p.tiles_m * want * 2 > kPairs || n / want <= 32) break;
     }
+    p.together = (uint32_t)std::min<uint64_t>(p.splits, std::max<uint64_t>(1, kProductPartsBytes / (4 * m * product_part_ld(n))));
     return p;
 }
 
@@ -247,7 +251,7 @@ extern "C" int dg_product(dg_ctx* ctx, void* stream, const dg_rows8* a, const dg
     if (a->rows == 0) return DG_OK;
     ProductJob j{};
     j.plan = plan_product(a->rows, b->rows, a->cols, b->by_column != 0);
-    if ((uint64_t)j.plan.tiles_m * j.plan.tiles_n * j.plan.splits > kMostCols) return fail(DG_E_TOO_LARGE, "more tiles than a launch can count");
+    if ((uint64_t)j.plan.tiles_m * j.plan.tiles_n * j.plan.together > kMostCols) return fail(DG_E_TOO_LARGE, "more tiles than a launch can count");
     if (int rc = check_workspace(workspace, workspace_bytes, dg_product_workspace(ctx, a->rows, b->rows, a->cols))) return rc;
     const auto encode = (CUresult(*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                      const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill))encode_tiled_entry();
@@ -265,12 +269,12 @@ extern "C" int dg_product(dg_ctx* ctx, void* stream, const dg_rows8* a, const dg
         return map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, r.values, dim, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B);
     };
     if (!operand(&j.a, *a, kProductTileM / 2) || !operand(&j.b, *b, j.plan.tile_n / 2)) return fail(DG_E_CUDA, "cuTensorMapEncodeTiled rejected an operand");
-    {  // the output, or its parts; rows that do not start at multiples of 16 bytes are stored without a map
+    {  // the output, or the parts of a launch; rows that do not start at multiples of 16 bytes are stored without a map
         const bool split = j.plan.splits > 1;
         void* const at = split ? workspace : out->data;
         const int32_t dtype = split ? (int32_t)DG_F32 : out->dtype;
         const uint64_t ld = (split ? product_part_ld(b->rows) : out->ld) * element(dtype);
-        const cuuint64_t dim[3] = {b->rows, a->rows, j.plan.splits}, pitch[2] = {ld, ld * a->rows};
+        const cuuint64_t dim[3] = {b->rows, a->rows, j.plan.together}, pitch[2] = {ld, ld * a->rows};
         const cuuint32_t box[3] = {(cuuint32_t)(64 / element(dtype)), 32, 1};
         const CUtensorMapDataType types[3] = {CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16};
         j.out_by_map = ((uintptr_t)at | ld) % 16 == 0 && pitch[1] < 1ull << 40 &&

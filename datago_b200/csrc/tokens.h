@@ -74,11 +74,14 @@ void launch_dropout(const DropoutJob& job, cudaStream_t s);
 // ---- product (kernels_product.cu) ------------------------------------------------------------------------------------------
 // Tiles of 256 x at most 256; up to 224 columns a tile's sums leave tensor memory while the next tile's are made.
 constexpr uint32_t kProductTileM = 256, kProductMaxTileN = 256, kProductTwoSums = 224;
+constexpr uint32_t kProductPartGroups = 64;              // of a part of the contraction, at most
+constexpr uint64_t kProductPartsBytes = 512ull << 20;    // of the workspace for parts that are made together (one part may be larger)
 constexpr uint32_t kProductRingBytes = 192 * 1024, kProductABytes = kProductTileM / 2 * 128, kProductSlots = 6;
 struct ProductPlan {
     uint32_t tile_n;           // columns of an output tile, a multiple of 32
     uint32_t tiles_m, tiles_n;
     uint32_t splits, split_groups;  // the contraction is cut into `splits` parts of split_groups groups of 128
+    uint32_t together;              // parts of a launch: all, or as many as the workspace has room for beside the sum of those before them
     uint32_t sums;                  // accumulators
     uint32_t slots;                 // of 256 columns each, of the ring of b, and of a unless it stays
     bool a_stays;                   // all groups of a row of tiles have room
@@ -86,7 +89,7 @@ struct ProductPlan {
 ProductPlan plan_product(uint64_t m, uint64_t n, uint64_t k, bool b_by_column);
 inline uint64_t product_part_ld(uint64_t n) { return (n + 3) / 4 * 4; }
 inline uint64_t product_workspace(const ProductPlan& p, uint64_t m, uint64_t n) {
-    return p.splits > 1 ? (uint64_t)p.splits * m * product_part_ld(n) * 4 : 0;
+    return p.splits > 1 ? (uint64_t)(p.together + (p.together < p.splits)) * m * product_part_ld(n) * 4 : 0;
 }
 struct ProductJob {
     // boxes of 128 bytes x 128 (a), tile_n / 2 (b) or, of an operand by column, 128 lines, 128-byte swizzle; of 64 bytes x 32 rows x 1 part, 64-byte swizzle
@@ -99,6 +102,7 @@ struct ProductJob {
     int32_t dtype;
     float* parts;
     ProductPlan plan;
+    uint32_t first_group;  // of the parts of a launch
 };
 cudaError_t launch_product(const ProductJob& job, cudaStream_t s);
 cudaError_t product_gave_up(unsigned int* count, cudaStream_t s);  // waits for the stream; CTAs on the current device since the process began

@@ -8,6 +8,11 @@ static unsigned int gave_up = 0;
 extern "C" {
 int fake_launches() { int n = launches; launches = 0; return n; }
 void fake_gave_up(unsigned int more) { gave_up += more; }
+void fake_product_plan(uint64_t m, uint64_t n, uint64_t k, int b_by_column, uint64_t out[6]) {
+    const dg::ProductPlan p = dg::plan_product(m, n, k, b_by_column != 0);
+    const uint64_t v[6] = {p.splits, p.split_groups, p.together, (uint64_t)p.tiles_m * p.tiles_n, p.slots, p.a_stays};
+    for (int i = 0; i < 6; ++i) out[i] = v[i];
+}
 }
 
 namespace dg {

@@ -210,3 +210,61 @@ def test_norm_has_16384_columns_at_most(ctx):
             else:
                 with pytest.raises(dg.DatagoB200Error, match="16384"):
                     call()
+
+
+# ---- products ----------------------------------------------------------------------------------------------------------------
+def whole_numbers(rows, cols, most, scales, seed, by_column=False):
+    """Rows8 of whole numbers up to `most` in magnitude, whose groups have scales 2^0 .. 2^scales."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = tk.Rows8.empty(rows, cols, "cuda", by_column=by_column)
+    r.values.copy_(torch.randint(-most, most + 1, (rows, cols), generator=g, device="cuda", dtype=torch.int8).float())
+    r.scales.view(torch.uint8).copy_(torch.randint(127, 128 + scales, r.scales.shape, generator=g, device="cuda", dtype=torch.uint8))
+    return r
+
+
+def sum_of_products(a, b):
+    total = torch.zeros(a.shape[0], b.shape[0], dtype=torch.float64, device="cuda")
+    step = 16384
+    for k in range(0, a.shape[1], step):
+        part = [tk.Rows8(r.values[:, k:k + step], r.scales[:, k // 128:(k + step) // 128]).to_float().double() for r in (a, b)]
+        total += part[0] @ part[1].t()
+    return total
+
+
+@pytest.mark.parametrize("m,n,k,most,scales", [(1, 1, 5, 7, 2), (7, 1024, 768, 7, 2), (129, 241, 513, 7, 2), (300, 96, 1500, 7, 2), (2561, 520, 300, 7, 2), (20001, 200, 640, 7, 2),
+                                               (64, 64, 20000, 2, 1), (1152, 768, 5000, 3, 1), (250, 130, 9000, 3, 1)])
+@pytest.mark.parametrize("a_turned,b_turned", [(False, False), (True, True)])
+def test_products_of_whole_numbers_are_exact(ctx, m, n, k, most, scales, a_turned, b_turned):
+    a, b = whole_numbers(m, k, most, scales, m + k, a_turned), whole_numbers(n, k, most, scales, n + k + 1, b_turned)
+    assert k * (most << scales) ** 2 < 1 << 23
+    assert torch.equal(tk.product(ctx, a, b, F32).double(), sum_of_products(a, b))
+
+
+def one_and_ones(rows, groups):
+    """2^15 in the first column, nothing in the rest of its group, ones elsewhere."""
+    r = tk.Rows8.empty(rows, 128 * groups, "cuda")
+    r.values.copy_(torch.ones(1, device="cuda"))
+    r.values[:, 1:128].copy_(torch.zeros(1, device="cuda"))
+    r.scales.view(torch.uint8).fill_(127)
+    r.scales.view(torch.uint8)[:, 0] = 127 + 15
+    return r
+
+
+@pytest.mark.parametrize("m,n,groups", [(1152, 768, 2048), (2560, 2560, 320), (64, 64, 1 << 13), (4096, 1152, 450)])
+def test_long_sums_lose_what_64_groups_lose(ctx, m, n, groups):
+    # Beside 2^30 the tensor cores' sums have steps of 2^7, and all that 32 ones add is cut off, up to the end of the part.  Other parts are exact; they
+    # are off by 2^6 at most each time when they are added; there are 16, or one for 60 groups.
+    got = tk.product(ctx, one_and_ones(m, groups), one_and_ones(n, groups), F32).double()
+    off = (got - (2.0 ** 30 + 128 * (groups - 1))).abs().max()
+    assert off <= 63 * 128 + 64 * max(17, groups // 60 + 2), off
+
+
+def test_parts_that_do_not_fit_their_workspace_at_once(ctx):
+    m, n, k = 4096, 2048, 163840  # 20 parts of 32 MB
+    assert tk.lib().dg_product_workspace(ctx._h, m, n, k) < 20 * m * n * 4
+    a, b = whole_numbers(m, k, 1, 0, 60), whole_numbers(n, k, 1, 0, 61)
+    want = sum_of_products(a, b)
+    assert torch.equal(tk.product(ctx, a, b, F32).double(), want)
+    got = tk.product(ctx, a, b, BF16)
+    assert torch.equal(got, want.float().to(BF16))  # rounded once
+    tk.product_status(ctx)

@@ -131,3 +131,24 @@ def test_every_context_learns_of_products_that_gave_up(L):
         refused(L, L.dg_product_status(c._h, None), SYNC_LIMIT)
         assert b"1 CTAs" in L.dg_last_error()
         assert L.dg_product_status(c._h, None) == OK
+
+
+@pytest.mark.parametrize("m,n,k", [(1152, 768, 1 << 20), (4096, 1152, 57600), (4096, 4096, 131072), (64, 64, 1 << 24), (1, 1, (1 << 31) - 1024), (65536, 65536, 1 << 20), (8192, 8192, 8192), (8192, 8192, 8193),
+                                   (131072, 1152, 768), (200, 4801, 8320), (1152, 768, 57600)])
+@pytest.mark.parametrize("b_by_column", [0, 1])
+def test_no_part_of_a_contraction_is_longer_than_64_groups(L, ctx, m, n, k, b_by_column):
+    v = (C.c_uint64 * 6)()
+    L.fake_product_plan(C.c_uint64(m), C.c_uint64(n), C.c_uint64(k), b_by_column, v)
+    splits, per_split, together, tiles, slots, a_stays = v
+    groups = -(-k // 128)
+    assert per_split <= 64 and (splits - 1) * per_split < groups <= splits * per_split
+    assert 1 <= together <= splits and tiles * together < 1 << 31 and (splits == 1 or per_split % 4 == 0)
+    part = m * -(-n // 4) * 16
+    if splits == 1:
+        assert together == 1
+        return
+    # all parts at once, or as many as half a GB holds and a place for their sum
+    kept = splits if together == splits else together + 1
+    assert L.dg_product_workspace(ctx._h, m, n, k) >= kept * part
+    assert together == 1 or together * part <= 1 << 29
+    assert together == splits or (together + 1) * part > 1 << 29
