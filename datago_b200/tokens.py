@@ -15,7 +15,7 @@ import struct
 
 import torch
 
-from . import DatagoB200Error, DeviceArray, _check, lib as _library
+from . import Batch, DatagoB200Error, DeviceArray, _check, lib as _library
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _LEGACY_STREAM = 1  # cudaStreamLegacy: torch's default stream, which has no handle of its own
@@ -202,6 +202,8 @@ def patch_rows(ctx, pixels, patch, mean, std, dtype=None, out=None):
     """Patches of a bucket (uint8 [n, height, width, channels]: a tensor, or a DeviceArray of Batch.buckets()) as rows: Rows8, or with `dtype` a
     tensor.  Row (i, Y, X), feature (y, x, c) is (pixel / 255 - mean[c]) / std[c]; height and width are multiples of `patch`."""
     if isinstance(pixels, DeviceArray):
+        if isinstance(pixels._owner, Batch) and not pixels._owner._h:
+            raise _invalid("pixels: the batch is closed")
         pixels = torch.as_tensor(pixels, device=f"cuda:{ctx.device}")
     _on_device(ctx, pixels, "pixels")
     if pixels.dtype != torch.uint8 or pixels.dim() != 4 or not pixels.is_contiguous():
@@ -355,8 +357,6 @@ class PatchStem:
     def forward(self, pixels, positions, offset=0):
         """(Norm with Rows8 for the first layer, what backward wants).  positions: [tokens of an image, width] of the stem's dtype.  offset: where this batch's
         elements begin in the run's count (see dropout)."""
-        if isinstance(pixels, DeviceArray):
-            pixels = torch.as_tensor(pixels, device=f"cuda:{self.ctx.device}")
         norm_weight = None if self.norm_weight is None else self.norm_weight.detach()
         x = product(self.ctx, patch_rows(self.ctx, pixels, self.patch, self.mean, self.std), self.weight8, self.dtype)
         if self.p:

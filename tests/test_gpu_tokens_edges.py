@@ -7,6 +7,7 @@ import os
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 import torch
 
@@ -268,3 +269,34 @@ def test_parts_that_do_not_fit_their_workspace_at_once(ctx):
     got = tk.product(ctx, a, b, BF16)
     assert torch.equal(got, want.float().to(BF16))  # rounded once
     tk.product_status(ctx)
+
+
+# ---- buckets of batches ------------------------------------------------------------------------------------------------------
+CFG = dict(crop_and_resize=True, default_image_size=512, downsampling_ratio=16, min_aspect_ratio=0.5, max_aspect_ratio=2.0)
+
+
+def same_image_batch(tfm, count=2, seed=9):
+    image = np.random.default_rng(seed).integers(0, 256, (300, 400, 3), dtype=np.uint8)
+    b = tfm.batch([image] * count, flags=dg.BATCH_COLLATE)
+    b.upload()
+    b.run()
+    return b
+
+
+def test_a_bucket_of_a_closed_batch_is_refused():
+    tfm = dg.Context(0, CFG)
+    stem = tk.PatchStem(tfm, 16, MEAN, STD, rand((96, 768), F32, 1, 0.02), dtype=F32)
+    b = same_image_batch(tfm)
+    b.sync()
+    array = b.buckets()[0]["array"]
+    tokens = array.shape[1] * array.shape[2] // 256
+    positions, dy = rand((tokens, 96), F32, 2), rand((2 * tokens, 96), F32, 3)
+    saved = stem.forward(array, positions)[1]
+    got = stem.backward(saved, dy)
+    pixels = torch.as_tensor(array, device="cuda")
+    assert same(stem.backward(stem.forward(pixels, positions)[1], dy), got)
+    del pixels
+    b.close()
+    for call in (lambda: tk.patch_rows(tfm, array, 16, MEAN, STD), lambda: stem.forward(array, positions), lambda: stem.backward(saved, dy)):
+        with pytest.raises(dg.DatagoB200Error, match="closed"):
+            call()
