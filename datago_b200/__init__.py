@@ -555,18 +555,8 @@ class Batch:
         and outlive the batch, those of damaged items are undefined (look at the items' status after sync())."""
         if not self._h:
             raise DatagoB200Error(1, "the batch is closed")
-        import torch
         from . import tokens
-        bucket = self.buckets()[k]
-        current = torch.cuda.current_stream(self.ctx.device)
-        own = torch.cuda.ExternalStream(self.ctx.stream, self.ctx.device) if self.ctx.stream else torch.cuda.default_stream(self.ctx.device)
-        apart = own.cuda_stream != current.cuda_stream
-        if apart:
-            current.wait_stream(own)
-        rows = tokens.patch_rows(self.ctx, bucket["array"], patch, mean, std, dtype)
-        if apart:
-            own.wait_stream(current)  # the batch's memory is handed on in the order of its own stream
-        return rows
+        return tokens.patch_rows(self.ctx, self.buckets()[k]["array"], patch, mean, std, dtype)
 
     def stage_ms(self):
         ms = (C.c_float * len(STAGES))()

@@ -198,13 +198,34 @@ def _workspace(nbytes, like):
     return work, work.data_ptr()
 
 
+def _streams_of(batch):
+    """(torch's current stream, the stream of a batch) where they differ, else None.  While the current stream is being captured it cannot wait for what is
+    outside: the batch then has to be complete."""
+    device, handle = batch.ctx.device, batch.ctx.stream
+    current = torch.cuda.current_stream(device)
+    if current.cuda_stream == (handle or 0):
+        return None
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            return None
+    return current, torch.cuda.ExternalStream(handle, device) if handle else torch.cuda.default_stream(device)
+
+
 def patch_rows(ctx, pixels, patch, mean, std, dtype=None, out=None):
     """Patches of a bucket (uint8 [n, height, width, channels]: a tensor, or a DeviceArray of Batch.buckets()) as rows: Rows8, or with `dtype` a
-    tensor.  Row (i, Y, X), feature (y, x, c) is (pixel / 255 - mean[c]) / std[c]; height and width are multiples of `patch`."""
+    tensor.  Row (i, Y, X), feature (y, x, c) is (pixel / 255 - mean[c]) / std[c]; height and width are multiples of `patch`.  A DeviceArray is read behind
+    its batch's run(), and its batch may be closed right after the call (inside a stream capture neither is waited for)."""
     if isinstance(pixels, DeviceArray):
-        if isinstance(pixels._owner, Batch) and not pixels._owner._h:
+        batch = pixels._owner if isinstance(pixels._owner, Batch) else None
+        if batch is not None and not batch._h:
             raise _invalid("pixels: the batch is closed")
-        pixels = torch.as_tensor(pixels, device=f"cuda:{ctx.device}")
+        streams = None if batch is None else _streams_of(batch)
+        if streams:
+            streams[0].wait_stream(streams[1])
+        rows = patch_rows(ctx, torch.as_tensor(pixels, device=f"cuda:{ctx.device}"), patch, mean, std, dtype, out)
+        if streams:
+            streams[1].wait_stream(streams[0])  # the batch's memory is handed on in the order of its own stream
+        return rows
     _on_device(ctx, pixels, "pixels")
     if pixels.dtype != torch.uint8 or pixels.dim() != 4 or not pixels.is_contiguous():
         raise _invalid("pixels: a contiguous uint8 [n, height, width, channels] tensor is wanted")

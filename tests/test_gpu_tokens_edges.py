@@ -300,3 +300,40 @@ def test_a_bucket_of_a_closed_batch_is_refused():
     for call in (lambda: tk.patch_rows(tfm, array, 16, MEAN, STD), lambda: stem.forward(array, positions), lambda: stem.backward(saved, dy)):
         with pytest.raises(dg.DatagoB200Error, match="closed"):
             call()
+
+
+def test_a_buckets_array_is_read_behind_its_batch_and_before_the_batch_goes():
+    tfm, other = dg.Context(0, CFG), dg.Context(0)
+    want = None
+    for stream in (torch.cuda.Stream(), torch.cuda.default_stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(stream):
+            for _ in range(4):
+                b = same_image_batch(tfm)
+                rows = tk.patch_rows(other, b.buckets()[0]["array"], 16, MEAN, STD, F32)  # without waiting for the batch
+                b.close()
+                same_image_batch(tfm, seed=10).close()  # another one in its place
+                want = rows if want is None else want
+                stream.synchronize()
+                assert torch.equal(rows, want)
+    b = same_image_batch(tfm)
+    b.sync()
+    assert torch.equal(tk.patch_rows(tfm, torch.as_tensor(b.buckets()[0]["array"], device="cuda"), 16, MEAN, STD, F32), want)
+    torch.cuda.synchronize()
+    b.close()
+
+
+def test_a_buckets_array_can_be_read_in_a_graph():
+    tfm = dg.Context(0, CFG)
+    b = same_image_batch(tfm)
+    b.sync()
+    want = b.patch_rows(0, 16, MEAN, STD, F32)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first, second = b.patch_rows(0, 16, MEAN, STD, F32), tk.patch_rows(tfm, b.buckets()[0]["array"], 16, MEAN, STD, F32)
+    first.zero_()
+    second.zero_()
+    graph.replay()
+    assert torch.equal(first, want) and torch.equal(second, want)
+    torch.cuda.synchronize()
+    b.close()
