@@ -102,7 +102,8 @@ def _invalid(msg):
 def _on_device(ctx, t, name):
     if not isinstance(t, torch.Tensor):
         raise _invalid(f"{name}: a torch tensor is wanted")
-    if t.get_device() != ctx.device or not t.is_cuda:  # (-1 for tensors of the host)
+    device = t.get_device()  # -1 for tensors of the host
+    if device != ctx.device or device < 0:
         raise _invalid(f"{name} is on {t.device}, the context on cuda:{ctx.device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise _invalid(f"{name} requires a gradient, which would be lost here: detach() it, or call under no_grad()")
@@ -154,7 +155,7 @@ def _rows8(ctx, r, name, transposed=None):
     if sone != 1 and groups > 1:
         raise _invalid(f"{name}: scales have to be neighbours in memory")
     # A single column, or row, fits both orders.  Rows of a single column that are neighbours are its line: the transpose of one row.
-    by_row, by_column = (one == 1 or cols <= 1) and not (cols <= 1 < rows and ld == 1), ld == 1 or rows <= 1
+    by_row, by_column = one == 1 if cols > 1 else ld != 1 or rows <= 1, ld == 1 or rows <= 1
     if transposed is not None:
         by_row, by_column = by_row and not transposed, by_column and transposed
     if by_row:
