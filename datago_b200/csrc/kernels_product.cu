@@ -151,7 +151,8 @@ __device__ __forceinline__ uint32_t scale_word(const uint8_t* p, uint32_t q, uin
     return (left > 1 ? (uint32_t)*reinterpret_cast<const uint16_t*>(p) : p[0]) | (left == 3 ? (uint32_t)p[2] << 16 : 0u);
 }
 
-template <class T>
+// RAGGED: the output's rows begin at multiples of 16 bytes, but end inside one.
+template <class T, bool RAGGED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_product(const __grid_constant__ ProductJob j, T* out, uint64_t ld, uint64_t part_elements) {
     extern __shared__ unsigned char raw_smem[];
     __shared__ __align__(8) unsigned long long s_bar[4 * kSlots + 2 * kScaleStages + 5];
@@ -404,7 +405,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_produ
     } else {  // ---- storers
         constexpr uint32_t kPiece = 64 / sizeof(T);  // columns of a piece
         const uint32_t rows = (warp & 3u) * 32, mine = smem + kOutAt + (warp & 3u) * kPieces * kOutBytes;
-        const bool by_map = j.out_by_map, by_word = sizeof(T) == 4 || ((reinterpret_cast<uintptr_t>(out) | (ld * sizeof(T)) | (part_elements * sizeof(T))) & 3u) == 0;
+        const bool by_map = j.map_cols != 0, by_word = sizeof(T) == 4 || ((reinterpret_cast<uintptr_t>(out) | (ld * sizeof(T)) | (part_elements * sizeof(T))) & 3u) == 0;
         Place room;
         Place sum;
         bool go_on = true;
@@ -417,6 +418,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_produ
             const uint64_t row0 = (uint64_t)t.m0 + rows;
             const uint32_t live = row0 < j.m ? (uint32_t)min((uint64_t)32, j.m - row0) : 0;  // rows of this warp that the matrix has
             const uint32_t width = (uint32_t)min((uint64_t)tile_n, j.n - t.n0);
+            const uint32_t mapped = RAGGED ? min(width, max((uint32_t)j.map_cols, t.n0) - t.n0) : width;  // columns of the tile that the map has
             uint32_t v[kPiece], w[16];
             auto read = [&](uint32_t c) {
 #pragma unroll
@@ -446,10 +448,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_produ
                 for (uint32_t k = 0; k < 4; ++k)  // 64-byte swizzle: 16 bytes k of row r at k ^ (r / 2 % 4)
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(piece + lane * 64 + ((k ^ ((lane >> 1) & 3u)) << 4)), "r"(w[4 * k]), "r"(w[4 * k + 1]),
                                  "r"(w[4 * k + 2]), "r"(w[4 * k + 3]) : "memory");
-                if (by_map) {  // rows and columns outside the matrix are not written
+                if (by_map) {  // rows and columns outside the map are not written
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) store_box(&j.out_map, (int32_t)(t.n0 + c), (int32_t)row0, (int32_t)t.split, piece);
+                    if (lane == 0) {
+                        if (!RAGGED || c < mapped) store_box(&j.out_map, (int32_t)(t.n0 + c), (int32_t)row0, (int32_t)t.split, piece);
+                        else asm volatile("cp.async.bulk.commit_group;" ::: "memory");  // pieces are counted by it
+                    }
+                    // what is left behind the map's last sixteen bytes is one part of sixteen more: by the lane that has put its row there
+                    if (RAGGED && mapped < width && c + kPiece > mapped && lane < live) {
+                        uint32_t q[4];
+                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
+                                     : "r"(piece + lane * 64 + ((((mapped - c) * (uint32_t)sizeof(T) >> 4) ^ ((lane >> 1) & 3u)) << 4)));
+                        T* const to = out + (row0 + lane) * ld + t.n0 + mapped;
+                        const uint32_t bytes = (width - mapped) * sizeof(T);
+                        if (bytes & 8u) *reinterpret_cast<uint2*>(to) = make_uint2(q[0], q[1]);
+                        if (bytes & 4u) reinterpret_cast<uint32_t*>(to)[bytes & 8u ? 2 : 0] = bytes & 8u ? q[2] : q[0];
+                        if (bytes & 2u) reinterpret_cast<uint16_t*>(to)[(bytes >> 1) - 1] = (uint16_t)(bytes & 8u ? bytes & 4u ? q[3] : q[2] : bytes & 4u ? q[1] : q[0]);
+                    }
                 } else {  // two rows at a time, neighbouring lanes neighbouring words (or elements, of rows that do not begin at words)
                     __syncwarp();
                     T* const to = out + t.split * part_elements + row0 * ld + t.n0 + c;
@@ -506,7 +522,7 @@ __global__ void __launch_bounds__(256) k_add_parts(const float* before, const fl
 }
 
 // The kernel's shared memory, allowed once on every device (devices beyond 63: with every call).
-template <class T>
+template <class T, bool RAGGED>
 cudaError_t allow_smem() {
     static std::atomic<uint64_t> done{0};
     int device = 0;
@@ -514,22 +530,23 @@ cudaError_t allow_smem() {
     if (e != cudaSuccess) return e;
     const uint64_t bit = device >= 0 && device < 64 ? 1ull << device : 0;
     if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-    e = cudaFuncSetAttribute(k_product<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+    e = cudaFuncSetAttribute(k_product<T, RAGGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
     if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
     return e;
 }
 
-template <class T>
+template <class T, bool RAGGED>
 cudaError_t product_into(const ProductJob& j, T* out, uint64_t ld, uint64_t part_elements, cudaStream_t s) {
-    const cudaError_t e = allow_smem<T>();
+    const cudaError_t e = allow_smem<T, RAGGED>();
     if (e != cudaSuccess) return e;
     const uint32_t tiles = j.plan.tiles_m * j.plan.tiles_n * j.plan.splits;
-    launch_after(k_product<T>, 2 * std::min<uint32_t>(tiles, kSms / 2), kThreads, kSmemBytes, s, j, out, ld, part_elements);
+    launch_after(k_product<T, RAGGED>, 2 * std::min<uint32_t>(tiles, kSms / 2), kThreads, kSmemBytes, s, j, out, ld, part_elements);
     return cudaGetLastError();
 }
 template <class T>
 cudaError_t product(const ProductJob& j, cudaStream_t s) {
-    if (j.plan.splits == 1) return product_into<T>(j, (T*)j.out, j.ld, 0, s);
+    // What a warp does about a row's end costs the others too (131072 x 1152 x 768 124 us instead of 120): products without one have a kernel without it.
+    if (j.plan.splits == 1) return j.map_cols && j.map_cols < j.n ? product_into<T, true>(j, (T*)j.out, j.ld, 0, s) : product_into<T, false>(j, (T*)j.out, j.ld, 0, s);
     const uint64_t part_ld = product_part_ld(j.n), part = j.m * part_ld;
     const uint32_t ctas = (uint32_t)std::min<uint64_t>((j.m * (part_ld / 4) + 255) / 256, (uint64_t)kSms * 8), splits = j.plan.splits;
     float* const sum = j.parts + j.plan.together * part;  // of the parts so far, where they are not all made together
@@ -537,7 +554,7 @@ cudaError_t product(const ProductJob& j, cudaStream_t s) {
     for (uint32_t first = 0; first < splits; first += some.plan.splits) {
         some.first_group = first * j.plan.split_groups;
         some.plan.splits = std::min(j.plan.together, splits - first);
-        const cudaError_t e = product_into<float>(some, j.parts, part_ld, part, s);
+        const cudaError_t e = product_into<float, false>(some, j.parts, part_ld, part, s);
         if (e != cudaSuccess) return e;
         const float* const before = first ? sum : nullptr;
         if (first + some.plan.splits < splits) launch_after(k_add_parts<float>, ctas, 256, 0, s, before, j.parts, some.plan.splits, part, j.m, j.n, part_ld, sum, part_ld);

@@ -269,16 +269,17 @@ extern "C" int dg_product(dg_ctx* ctx, void* stream, const dg_rows8* a, const dg
         return map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, r.values, dim, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B);
     };
     if (!operand(&j.a, *a, kProductTileM / 2) || !operand(&j.b, *b, j.plan.tile_n / 2)) return fail(DG_E_CUDA, "cuTensorMapEncodeTiled rejected an operand");
-    {  // the output, or the parts of a launch; rows that do not start at multiples of 16 bytes are stored without a map
+    {  // the output, or the parts of a launch; rows that do not start at multiples of 16 bytes are stored without a map.  A map stores whole sixteens of
+       // bytes, also where its rows end inside one: it has the columns of whole ones only.
         const bool split = j.plan.splits > 1;
         void* const at = split ? workspace : out->data;
         const int32_t dtype = split ? (int32_t)DG_F32 : out->dtype;
-        const uint64_t ld = (split ? product_part_ld(b->rows) : out->ld) * element(dtype);
-        const cuuint64_t dim[3] = {b->rows, a->rows, j.plan.together}, pitch[2] = {ld, ld * a->rows};
+        const uint64_t ld = (split ? product_part_ld(b->rows) : out->ld) * element(dtype), cols = split ? product_part_ld(b->rows) : b->rows - b->rows % (16 / element(dtype));
+        const cuuint64_t dim[3] = {cols, a->rows, j.plan.together}, pitch[2] = {ld, ld * a->rows};
         const cuuint32_t box[3] = {(cuuint32_t)(64 / element(dtype)), 32, 1};
         const CUtensorMapDataType types[3] = {CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16};
-        j.out_by_map = ((uintptr_t)at | ld) % 16 == 0 && pitch[1] < 1ull << 40 &&
-                       map(&j.out_map, types[dtype], 3, at, dim, pitch, box, CU_TENSOR_MAP_SWIZZLE_64B);
+        if (cols && ((uintptr_t)at | ld) % 16 == 0 && pitch[1] < 1ull << 40 && map(&j.out_map, types[dtype], 3, at, dim, pitch, box, CU_TENSOR_MAP_SWIZZLE_64B))
+            j.map_cols = std::min<uint64_t>(cols, b->rows);
     }
     j.a_by_column = a->by_column != 0; j.b_by_column = b->by_column != 0;
     j.a_scales = a->scales; j.b_scales = b->scales;

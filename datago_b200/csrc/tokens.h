@@ -97,7 +97,8 @@ struct ProductJob {
     const uint8_t *a_scales, *b_scales;
     uint64_t a_scale_ld, b_scale_ld, m, n, k, ld;
     uint32_t a_block, b_block;
-    bool a_by_column, b_by_column, out_by_map;
+    bool a_by_column, b_by_column;
+    uint64_t map_cols;  // columns that leave through out_map; 0: none
     void* out;
     int32_t dtype;
     float* parts;

@@ -4,7 +4,7 @@ include/datago_b200.h), on torch tensors.
 Every function takes the Context of the tensors' device first, launches on torch's current stream of that device and returns
 without waiting; nothing is kept between calls, so calls can be captured into CUDA graphs.  Results are new tensors unless `out` is given; the
 rows of new ones (dropout's apart) begin at multiples of 16 bytes, so those whose rows are no multiple of that long are not contiguous (a product of
-124515 x 685 in bfloat16 then takes 71 us, into contiguous rows 171).  Matrices are 2-d tensors of float32, bfloat16 or float16 whose columns
+124515 x 685 over 768 columns in bfloat16 takes 87 us, into contiguous rows 170).  Matrices are 2-d tensors of float32, bfloat16 or float16 whose columns
 are neighbours in memory; their rows, those of `out` too, may be any distance apart.
 Gradients are calls of their own (rms_norm_backward, dropout on the gradient, product on operands quantised along the contraction);
 PatchStem puts them together for the stem of a model.  Autograd knows nothing of these calls: while it records, tensors that require a gradient are

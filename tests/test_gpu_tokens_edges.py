@@ -241,6 +241,18 @@ def test_products_of_whole_numbers_are_exact(ctx, m, n, k, most, scales, a_turne
     assert torch.equal(tk.product(ctx, a, b, F32).double(), sum_of_products(a, b))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 7, 8, 9, 15, 33, 250, 685, 894])
+def test_product_leaves_what_lies_behind_the_columns(ctx, dtype, n):
+    # rows of the output begin at multiples of 16 bytes, and end anywhere; what lies between them belongs to the caller
+    for m, k, gap in ((5, 200, 0), (300, 128, 16), (70, 9000, 8)):
+        a, b = whole_numbers(m, k, 1, 0, m + k), whole_numbers(n, k, 1, 0, n + k)
+        big = torch.full((m, -(-n // 8) * 8 + gap), 7.0, dtype=dtype, device="cuda")
+        tk.product(ctx, a, b, dtype, out=big[:, :n])
+        want = sum_of_products(a, b).float().to(dtype)
+        assert torch.equal(big[:, :n], want) and bool((big[:, n:] == 7).all()), (m, k)
+
+
 def one_and_ones(rows, groups):
     """2^15 in the first column, nothing in the rest of its group, ones elsewhere."""
     r = tk.Rows8.empty(rows, 128 * groups, "cuda")
