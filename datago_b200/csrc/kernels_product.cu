@@ -16,8 +16,8 @@
 //   4 storers read the sums of a finished tile out of tensor memory, one lane a row, round them and send them out through shared memory
 //             with tensor-map copies of 32 rows x 64 bytes, while the issuer is at the next tile (two accumulators up to 224 columns).
 // An operand whose rows are neighbours in memory (dg_rows8.by_column) is copied as 128 rows x 128 columns too, and the instruction told.
-// Measured: 8192 x 8192 x 8192 432 us, 2.5 PFLOP/s; 131072 x 1152 x 768 into bf16 126 us, 1.8 (its 302 MB of output alone take 80 at the 3.8 TB/s of a plain
-// fill, its multiplications alone 80, its copies 55: they do not quite hide one another); 1152 x 768 x 57600 61 us, where copies out of L2 end at
+// Measured: 8192 x 8192 x 8192 432 us, 2.5 PFLOP/s; 131072 x 1152 x 768 into bf16 120 to 126 us over the same operands again, 142 to 149 over others in every
+// call, 1.6 (its 302 MB of output alone take 80 at the 3.8 TB/s of a plain fill, its multiplications alone 80, its copies 55: they do not quite hide one another); 1152 x 768 x 57600 61 us, where copies out of L2 end at
 // 10 TB/s; 7 x 1024 x 768 6 us, all latency.  Accuracy: 1.5e-8 of the result over 128 columns, 3e-7 over 8192,
 // which no part of a contraction exceeds (dg::plan_product).
 // Waits are bounded: a CTA that runs out of patience counts itself (dg_product_status) and leaves.

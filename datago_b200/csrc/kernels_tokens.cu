@@ -309,7 +309,7 @@ void rows8(const dg_matrix& m, const dg_rows8& out, cudaStream_t s) {
 // ---- patches ---------------------------------------------------------------------------------------------------------------
 // A thread makes sixteen neighbouring features of a patch, eight lanes the 128 of a scale.  A patch's row of pixels is `segment` = patch * C
 // neighbouring bytes, of which features 16 k .. 16 k + 15 are sixteen neighbouring ones where the segment is a multiple of sixteen.  48 images of
-// 1152 x 896 x 3 in patches of 16: 64 us, 4.6 TB/s; instructions bound it (eight features a thread and a division each took 206 us, one patch a
+// 1152 x 896 x 3 in patches of 16: 60 to 64 us, 4.7 to 5.0 TB/s; instructions bound it, 74 % of the places to issue one (eight features a thread and a division each took 206 us, one patch a
 // thread 76).
 // Out: uint8_t for 8-bit rows, else the type of the matrix.
 template <int C> struct PatchView {
@@ -806,7 +806,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) k_rms_norm(co
 // Rows of 16-bit elements that start at multiples of 16 bytes, up to 1280 of them: a warp per row, whose next row is copied into shared memory while it
 // works on this one (cp.async, sixteen bytes a lane; a lane reads what it has copied itself, so nothing but its own copies is waited for).  What is
 // under way then costs no registers, and half as many warps again fit as with rows waiting in registers.  131072 x 1152 bf16 with positions, sum and 8-bit
-// output: 144 us, 5.3 TB/s of which 3.1 are writes (159 with the next row in registers; rows shared by five warps, which meet at a barrier,
+// output: 135 to 145 us, 5.3 to 5.7 TB/s, six tenths of it writes (159 with the next row in registers; rows shared by five warps, which meet at a barrier,
 // took 224 and more).
 constexpr uint32_t kStagedCols = 1280;
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
@@ -1315,7 +1315,8 @@ __device__ __forceinline__ void bits_of_8(uint64_t index, uint64_t seed, uint32_
     }
 }
 
-// 131072 x 1152 bf16: 101 us, 6.0 TB/s; ten rounds are 40 of about 110 instructions for eight elements.
+// 131072 x 1152 bf16: 107 to 116 us over inputs that differ from call to call, 5.2 to 5.6 TB/s, 70 % of the places to issue an instruction; ten rounds are 40
+// of about 110 instructions for eight elements.  Whole tokens go the same way, with a generator's block for every eight columns: 1571 x 777 f32 7 us.
 // One row: the matrix without gaps, as long as need be.  EIGHTS: every vector of eight begins with an index that is a multiple of eight.
 constexpr int kDropoutVecs = 2;  // of a thread under way at once
 

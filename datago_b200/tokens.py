@@ -258,8 +258,8 @@ def patch_rows(ctx, pixels, patch, mean, std, dtype=None, out=None):
 
 
 def quantize_rows(ctx, x, transpose=False, block=1, out=None):
-    """A matrix, or its transpose, as Rows8, with a scale for each 128 columns of `block` (1 or 128) rows of the result.  The transpose
-    keeps the matrix's order in memory."""
+    """A matrix, or its transpose, as Rows8, with a scale for each 128 columns of `block` (1 or 128) rows of the result (`out` has a
+    block of its own).  The transpose keeps the matrix's order in memory."""
     src = _matrix(ctx, x, "x")
     rows, cols = x.shape
     given = out is not None
@@ -377,8 +377,8 @@ class PatchStem:
         self.weight8 = quantize_rows(self.ctx, weight.detach(), block=GROUP, out=kept)
 
     def forward(self, pixels, positions, offset=0):
-        """(Norm with Rows8 for the first layer, what backward wants).  positions: [tokens of an image, width] of the stem's dtype.  offset: where this batch's
-        elements begin in the run's count (see dropout)."""
+        """(Norm with Rows8 for the first layer, what backward wants).  positions: [tokens of an image, width] of the stem's dtype (row r of all takes row
+        r % len(positions)).  offset: where this batch's elements begin in the run's count (see dropout)."""
         norm_weight = None if self.norm_weight is None else self.norm_weight.detach()
         x = product(self.ctx, patch_rows(self.ctx, pixels, self.patch, self.mean, self.std), self.weight8, self.dtype)
         if self.p:

@@ -398,7 +398,8 @@ DG_API int dg_product_status(dg_ctx* ctx, void* stream);
 /* h = x + residual (row r takes residual row r % residual->rows, so positions can be shared by all images of a bucket; residual may be
  * NULL), rstd = 1 / sqrt(mean(h^2) + eps), y = h * rstd * weight (NULL: ones).  x, residual, sum and y have one dtype, weight (1 x cols) any.
  * Each output may be NULL: sum receives h, y the norm, y8 (block 1) the norm as 8-bit rows, rstd `rows` floats.  sum may be x.
- * y and y8 come from h before it is rounded to sum's type.  cols at most 16384 (in the backward pass too). */
+ * y and y8 come from h before it is rounded to sum's type.  The squares are added up in 32 bits: a row whose sum of squares passes 2^128 is normed to zeros.
+ * cols at most 16384 (in the backward pass too). */
 DG_API int dg_rms_norm(dg_ctx* ctx, void* stream, const dg_matrix* x, const dg_matrix* residual, const dg_matrix* weight, float eps,
                        const dg_matrix* sum, const dg_matrix* y, const dg_rows8* y8, float* rstd);
 /* Its backward pass, from dy (gradient of y or, straight through the rounding, of y8), h (what sum received), rstd and weight:
