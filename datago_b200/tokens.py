@@ -357,6 +357,10 @@ def dropout(ctx, x, p, seed, offset=0, per_row=False, out=None):
     return out
 
 
+def _detached(t):
+    return t.detach() if isinstance(t, torch.Tensor) else t  # (what is no tensor is refused where it is used)
+
+
 class PatchStem:
     """The stem of a model that reads buckets: patches as 8-bit rows, the product with the embedding weight, dropout, positions (shared by
     the images of a bucket), norm, 8-bit rows for the first layer.
@@ -373,17 +377,18 @@ class PatchStem:
     def set_weight(self, weight):
         """After an optimizer step: the new weight in 8 bits, on torch's current stream.  One of the same shape takes the old one's place in memory, so that
         captured forward passes read it too."""
-        kept = self.weight8 if self.weight8 is not None and self.weight8.shape == weight.shape else None
-        self.weight8 = quantize_rows(self.ctx, weight.detach(), block=GROUP, out=kept)
+        weight = _detached(weight)
+        kept = self.weight8 if self.weight8 is not None and self.weight8.shape == getattr(weight, "shape", None) else None
+        self.weight8 = quantize_rows(self.ctx, weight, block=GROUP, out=kept)
 
     def forward(self, pixels, positions, offset=0):
         """(Norm with Rows8 for the first layer, what backward wants).  positions: [tokens of an image, width] of the stem's dtype (row r of all takes row
         r % len(positions)).  offset: where this batch's elements begin in the run's count (see dropout)."""
-        norm_weight = None if self.norm_weight is None else self.norm_weight.detach()
+        norm_weight = _detached(self.norm_weight)
         x = product(self.ctx, patch_rows(self.ctx, pixels, self.patch, self.mean, self.std), self.weight8, self.dtype)
         if self.p:
             dropout(self.ctx, x, self.p, self.seed, offset, out=x)
-        norm = rms_norm(self.ctx, x, norm_weight, residual=positions.detach(), eps=self.eps, eight_bit=True, sum_out=x)
+        norm = rms_norm(self.ctx, x, norm_weight, residual=_detached(positions), eps=self.eps, eight_bit=True, sum_out=x)
         # what later changes of the stem's attributes must not change: the same draws and the same weight go into the gradients
         return norm, (pixels, norm.sum, norm.rstd, len(positions), offset, self.p, self.seed, norm_weight)
 

@@ -127,6 +127,19 @@ def test_autograd_notices_results_that_are_written_into_its_tensors(ctx):
         tk.dropout(ctx, x, 0.5, 1, out=x)
 
 
+def test_a_stem_refuses_what_is_no_tensor(ctx):
+    stem, pixels = stem_of(ctx), some_pixels((1, 14, 14, 3), 70)
+    before = stem.weight8
+    for call in (lambda: stem.set_weight([1.0]), lambda: stem.set_weight(None), lambda: stem.forward(pixels, [[0.0] * 96]), lambda: stem.forward(pixels, rand((1, 96), F32, 1).cpu()),
+                 lambda: tk.PatchStem(ctx, 14, MEAN, STD, "weight")):
+        with pytest.raises(dg.DatagoB200Error):
+            call()
+    assert stem.weight8 is before
+    stem.norm_weight = [1.0] * 96
+    with pytest.raises(dg.DatagoB200Error):
+        stem.forward(pixels, rand((1, 96), F32, 1))
+
+
 # ---- single rows and none --------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("block", [1, 128])
 @pytest.mark.parametrize("m,n", [(768, 33), (33, 47), (16, 1), (1, 768), (1, 1), (1000, 300)])
