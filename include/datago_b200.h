@@ -349,7 +349,7 @@ DG_API void dg_host_release(void* block);
 enum { DG_F32 = 0, DG_BF16 = 1, DG_F16 = 2 };
 
 /* A matrix in device memory: row r begins `ld` elements behind row r - 1; data is aligned to its elements (16-byte aligned rows are
- * faster). */
+ * faster).  What lies behind the last column is neither read nor written. */
 typedef struct dg_matrix {
     void* data;
     uint64_t rows, cols, ld;
